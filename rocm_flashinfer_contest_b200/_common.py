@@ -1,6 +1,7 @@
 """Argument handling shared by the decode and prefill ``run`` shims."""
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -53,3 +54,77 @@ def stream_handle(device: torch.device) -> int:
 
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+# ---- the decay operators and the state cache ----
+
+_no_guard = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` current for a launch where it is not already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _no_guard
+    return torch.cuda.device(device)
+
+
+def require16(t, name: str, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """``require`` for a read-only operand of a kernel that loads 16 bytes at a
+    time: a view that starts off a 16-byte boundary is copied."""
+    t = require(t, name, dtype, device)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def require_out(t, name: str, dtype: torch.dtype, shape, device: torch.device) -> torch.Tensor:
+    """A tensor the kernel writes (or updates in place): taken as it is or refused."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def require_log_decay(g, lead, HV: int, device: torch.device):
+    """``log_decay`` as ([HV] or [*lead, HV]) fp32 -> (tensor, 1 if per token)."""
+    g = require(g, "log_decay", torch.float32, device)
+    if tuple(g.shape) == (HV,):
+        return g, 0
+    if tuple(g.shape) == (*lead, HV):
+        return g, 1
+    raise ValueError(f"log_decay must be {(HV,)} or {(*lead, HV)}, got {tuple(g.shape)}")
+
+
+def require_heads(q, k, v, lead):
+    """Head counts and sizes of q, k [*lead, H, K] and v [*lead, HV, V] -> (H, HV, K, V)."""
+    n = len(lead)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t is not None and (t.dim() != n + 2 or tuple(t.shape[:n]) != tuple(lead)):
+            raise ValueError(f"{name} must be {tuple(lead)} + (heads, size), got {tuple(t.shape)}")
+    H, K = k.shape[n:]
+    if q is not None and tuple(q.shape) != tuple(k.shape):
+        raise ValueError(f"q and k must have one shape, got {tuple(q.shape)} and {tuple(k.shape)}")
+    HV, V = v.shape[n:]
+    if H < 1 or HV < 1:
+        raise ValueError("at least one q/k head and one v head are needed")
+    return H, HV, K, V
+
+
+def require_pool(pool, HV: int, V: int, K: int, device: torch.device, name: str = "initial_state"):
+    """A pool of states [slots, HV, V, K], fp32 or bf16, contiguous (it is updated in place)."""
+    if not isinstance(pool, torch.Tensor) or pool.dtype not in (torch.float32, torch.bfloat16) \
+            or pool.device != device:
+        raise TypeError(f"{name} must be an fp32 or bf16 tensor on {device}")
+    if pool.dim() != 4 or tuple(pool.shape[1:]) != (HV, V, K) or not pool.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [slots, {HV}, {V}, {K}] tensor, got {tuple(pool.shape)}")
+    return pool
+
+
+def require_indices(idx, B: int, device: torch.device, name: str, like=None):
+    """[B] int32/int64 indices on the device, as the type of ``like`` where given."""
+    if not isinstance(idx, torch.Tensor) or idx.dtype not in (torch.int32, torch.int64) \
+            or idx.device != device or tuple(idx.shape) != (B,):
+        raise ValueError(f"{name} must be an int32/int64 [{B}] tensor on {device}")
+    if like is not None and idx.dtype != like.dtype:
+        idx = idx.to(like.dtype)
+    return idx.contiguous()

@@ -1,5 +1,5 @@
 """Loads ``libgdn_b200.so`` (the sm_100a kernels behind the C ABI of
-``include/gdn_b200.h``) with ctypes and declares its entry points.
+``include/gdn_b200.h`` and ``include/gdn_decay_b200.h``) with ctypes and declares its entry points.
 
 There is no fallback: if the library is missing or cannot be loaded, every
 call raises, so a run never silently takes another path.
@@ -47,6 +47,17 @@ SIGNATURES = {
                                      _i, _i, _f, _i, _i, _i, _i, _vp, _vp, _vp]),
     "gdn_mtp_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _f,
                          _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _vp]),
+    "gdn_decay_prefill_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _f, _i, _i, _i, _i,
+                                   _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "gdn_decay_prefill_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i]),
+    "gdn_decay_decode_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _f,
+                                  _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    "gdn_decay_verify_fwd": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _f,
+                                  _i, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    "gdn_decay_commit": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i,
+                              _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "gdn_state_cache_store": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp, _i, ctypes.c_longlong, _i, _i, _vp]),
+    "gdn_state_cache_load": (_i, [_vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, ctypes.c_longlong, _i, _i, _vp]),
     "gdn_umma_selftest": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "gdn_umma_selftest_ex": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, ctypes.c_longlong, _vp]),
 }

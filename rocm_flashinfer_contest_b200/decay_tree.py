@@ -1,0 +1,100 @@
+"""Trees of drafted tokens for linear attention with a decay per head.
+
+Speculative decoding drafts several continuations of each sequence at once.
+``run`` scores all nodes of each entry's tree against the entry's pooled state
+without changing it; ``commit`` then advances the state over the accepted path.
+
+``run(q, k, v, initial_state, initial_state_indices, parents, log_decay,
+scale=None, output=None) -> output``
+    Node t of entry i continues from node ``parents[i, t]`` (before it, in
+    [0, t)) or, for -1, from pool slot ``initial_state_indices[i]``:
+    output[i, t] = scale * S q_t with S the state after the path down to node t,
+    advanced at each node as S' = exp(log_decay) S + v k^T.  A chain of tokens is
+    ``parents[i, t] = t - 1``.  A parent below -1 or not before its node marks
+    padding, which extends to whatever hangs below it: zero output, and its q, k
+    and v are not used.  An index outside the pool: the entry's outputs are zero.
+    Entries may share a slot.
+
+``commit(k, v, initial_state, initial_state_indices, parents, accepted,
+log_decay, output_state_indices=None) -> initial_state``
+    Advances each entry's slot in place over the path down to node
+    ``accepted[i]`` (or writes slot ``output_state_indices[i]``).  -1, or a node
+    that does not exist or is padding, accepts nothing.  No slot may be written
+    by one entry and read or written by another.
+
+q, k [B, T, H, 128] bf16; v, output [B, T, HV, 128] bf16; T <= 64; pool
+[slots, HV, 128, 128] fp32 or bf16; indices [B] int32 or int64; parents [B, T]
+and accepted [B] int32; log_decay [HV] or [B, T, HV] fp32; scale float or 0-d
+tensor, None / 0 -> 1/sqrt(128).  One kernel launch each on the current stream
+of the inputs' device, no host synchronisation (unless ``scale`` is a device
+tensor, which is read with ``.item()``), no gradients.  A value of v that is not
+finite, at a node that is not padding, spoils the outputs of its entry's tree.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _common as C
+from ._lib import check, lib
+
+MAX_NODES = 64  # GDN_DECAY_TREE_MAX (include/gdn_decay_b200.h)
+
+
+def _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay):
+    dev = C.cuda_device_of(k)
+    bf = torch.bfloat16
+    k, v = C.require16(k, "k", bf, dev), C.require16(v, "v", bf, dev)
+    if q is not None:
+        q = C.require16(q, "q", bf, dev)
+    if k.dim() != 4:
+        raise ValueError(f"k must be [B, T, H, K], got {tuple(k.shape)}")
+    B, T = k.shape[:2]
+    H, HV, K, V = C.require_heads(q, k, v, (B, T))
+    if T > MAX_NODES:
+        raise ValueError(f"a tree has at most {MAX_NODES} nodes, got {T}")
+    g, per_token = C.require_log_decay(log_decay, (B, T), HV, dev)
+    pool = C.require_pool(initial_state, HV, V, K, dev)
+    idx = C.require_indices(initial_state_indices, B, dev, "initial_state_indices")
+    parents = C.require(parents, "parents", torch.int32, dev)
+    if tuple(parents.shape) != (B, T):
+        raise ValueError(f"parents must be {(B, T)}, got {tuple(parents.shape)}")
+    return dev, (q, k, v, pool, idx, parents, g), per_token, (B, T, H, HV, K, V)
+
+
+def run(q, k, v, initial_state, initial_state_indices, parents, log_decay, scale=None, output=None):
+    """See the module docstring."""
+    if q is None:
+        raise TypeError("q must be a torch.Tensor, got NoneType")
+    dev, tensors, per_token, dims = _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay)
+    q, k, v, pool, idx, parents, g = tensors
+    B, T, H, HV, K, V = dims
+    if output is None:
+        output = torch.empty((B, T, HV, V), dtype=torch.bfloat16, device=dev)
+    else:
+        C.require_out(output, "output", torch.bfloat16, (B, T, HV, V), dev)
+    with C.on_device(dev):
+        st = lib().gdn_decay_verify_fwd(
+            C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(pool), int(pool.dtype == torch.bfloat16), C.ptr(idx),
+            int(idx.dtype == torch.int64), C.ptr(parents), C.ptr(g), per_token, C.normalize_scale(scale, K),
+            B, T, H, HV, K, V, pool.shape[0], C.ptr(output), C.stream_handle(dev))
+    check("gdn_decay_verify_fwd", st)
+    return output
+
+
+def commit(k, v, initial_state, initial_state_indices, parents, accepted, log_decay, output_state_indices=None):
+    """See the module docstring."""
+    dev, tensors, per_token, dims = _inputs(None, k, v, initial_state, initial_state_indices, parents, log_decay)
+    _, k, v, pool, idx, parents, g = tensors
+    B, T, H, HV, K, V = dims
+    accepted = C.require(accepted, "accepted", torch.int32, dev)
+    if tuple(accepted.shape) != (B,):
+        raise ValueError(f"accepted must be {(B,)}, got {tuple(accepted.shape)}")
+    out_idx = None if output_state_indices is None else \
+        C.require_indices(output_state_indices, B, dev, "output_state_indices", like=idx)
+    with C.on_device(dev):
+        st = lib().gdn_decay_commit(
+            C.ptr(k), C.ptr(v), C.ptr(pool), int(pool.dtype == torch.bfloat16), C.ptr(idx), C.ptr(out_idx),
+            int(idx.dtype == torch.int64), C.ptr(parents), C.ptr(accepted), C.ptr(g), per_token,
+            B, T, H, HV, K, V, pool.shape[0], C.stream_handle(dev))
+    check("gdn_decay_commit", st)
+    return initial_state
