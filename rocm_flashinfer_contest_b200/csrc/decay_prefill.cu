@@ -1,21 +1,57 @@
 // decay_prefill.cu — prefill of packed prompts for linear attention with a
 // decay per head (sm_100a).
+//
+// Over a chunk of 64 tokens with log decays g, c_i = g_0 + .. + g_i, and the
+// state S [V, K] before it:
+//   o_i = scale * ( e^{c_i} S q_i  +  sum_{j <= i} e^{c_i - c_j} (q_i . k_j) v_j )
+//   S'  = e^{c_63} S + sum_j v_j (w_j k_j)^T,     w_j = e^{c_63 - c_j}
+//
+// One CTA walks the chunks of one segment (up to seg_len tokens of one
+// sequence) of one v-head.  Long sequences are cut into segments so that about
+// 148 CTAs have work: a first launch sums every segment's own contribution to
+// the state (the same kernel without queries, kStateOnly), a second turns these
+// into the state before each segment, and the third does everything.  A call
+// whose T fits one segment launches the third only.
+//
+// Products, all on tcgen05 with fp32 accumulators in tensor memory and every
+// operand in the layout in which it arrives (token-major tiles from TMA):
+//   U   [v, k] = V^T (wK)       A: V tile (MN-major), B: scaled K (MN-major)
+//   P   [i, j] = Q K^T          rows 64..127 of the M = 128 tile are not used
+//   O2^T[v, i] = S Q^T          A: S as bf16 in tensor memory, B: Q tile
+//   O1^T[v, i] = V^T P^T        A: V tile (MN-major), B: decayed P
+//
+// Precision: inputs are bf16; every other factor is split into bf16 terms so
+// that nothing is lost beside the fp32 accumulation: wK into three (off by
+// 2^-25 or so: the state is an fp32 result), S and P into two (2^-17: the output
+// is rounded to bf16, 2^-9).
+#include <cuda.h>
+
+#include <atomic>
+#include <mutex>
+
 #include "decay_common.cuh"
+#include "umma.cuh"
 
 namespace gdn {
 namespace decay {
 
+using namespace umma;
+
+constexpr int C = 64;                // tokens per chunk
+constexpr uint32_t kTile = C * 256;  // bytes of a [64][128] bf16 tile
+constexpr int kSms = 148;
+
 struct PrefillParams {
-    const __nv_bfloat16* q;
-    const __nv_bfloat16* k;
-    const __nv_bfloat16* v;
     const float* state;  // nullable: zero
     const float* log_decay;
     const void* cu;
     __nv_bfloat16* out;
     float* new_state;
+    float* ws_state;  // [ws slots][HV][V][K]: the state before a segment (of its predecessor, after the first launch)
+    float* ws_decay;  // [ws slots][HV]: e^(sum of a segment's log decays), at its successor's place
     float scale;
-    int cu64, per_token, N, T, H, HV, rep;
+    int cu64, per_token, N, T, H, HV, rep, seg_len, slots;
+    int first_from_ws;  // new_state is state: the first of several segments reads the copy in ws_state
 };
 
 __device__ __forceinline__ int cu_at(const void* cu, int is64, int i, int T) {
@@ -23,63 +59,636 @@ __device__ __forceinline__ int cu_at(const void* cu, int is64, int i, int T) {
     return (int)(x < 0 ? 0 : x > T ? T : x);
 }
 
-// Token-serial form: 32 rows of one sequence's v-head per CTA, 8 lanes to a
-// row, the state in registers over all tokens.
-__global__ void __launch_bounds__(128) decay_prefill_serial_kernel(const PrefillParams p) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
-    const int rb = blockIdx.x % 4, nh = blockIdx.x / 4, n = nh / p.HV, h = nh % p.HV, hq = h / p.rep;
-    const int row = rb * 32 + warp * 8 + (lane >> 3);
-    if (n == p.N) {  // tokens of no sequence: zero outputs
+// A segment: tokens [t0, t1) of sequence n, number s of nseg, workspace slot of
+// the sequence's first segment (sequences of one segment have none).
+struct Item {
+    int n, s, nseg, t0, t1, ws;
+};
+
+__device__ __forceinline__ int n_segments(const PrefillParams& p, int n, int& t0, int& len) {
+    t0 = cu_at(p.cu, p.cu64, n, p.T);
+    const int t1 = cu_at(p.cu, p.cu64, n + 1, p.T);
+    len = t1 > t0 ? t1 - t0 : 0;
+    return len > p.seg_len ? (len + p.seg_len - 1) / p.seg_len : 1;
+}
+
+// The slot-th segment, counted over the sequences (kInner: over those segments
+// that another one follows); one warp, all lanes get it.  n = N: there is none.
+// Malformed cu_seqlens can make the sequences overlap; the workspace slots are
+// then cut off at the workspace's end.
+template <bool kInner>
+__device__ __forceinline__ Item find_item(const PrefillParams& p, int slot, int ws_slots) {
+    const int lane = threadIdx.x & 31;
+    Item it{p.N, 0, 0, 0, 0, 0};
+    int before = 0, ws = 0;
+    for (int base = 0; base < p.N; base += 32) {
+        int t0 = 0, len = 0, nseg = 0;
+        if (base + lane < p.N) nseg = n_segments(p, base + lane, t0, len);
+        const int cnt = kInner ? (nseg > 1 ? nseg - 1 : 0) : nseg, wcnt = nseg > 1 ? nseg : 0;
+        int cs = cnt, wsum = wcnt;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, cs, d), y = __shfl_up_sync(0xffffffffu, wsum, d);
+            if (lane >= d) cs += x, wsum += y;
+        }
+        const bool here = slot >= before + cs - cnt && slot < before + cs;
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        if (who) {
+            const int src = __ffs(who) - 1;
+            it.n = base + src;
+            it.s = slot - (before + __shfl_sync(0xffffffffu, cs - cnt, src));
+            it.nseg = __shfl_sync(0xffffffffu, nseg, src);
+            it.ws = ws + __shfl_sync(0xffffffffu, wsum - wcnt, src);
+            t0 = __shfl_sync(0xffffffffu, t0, src), len = __shfl_sync(0xffffffffu, len, src);
+            it.t0 = t0 + it.s * p.seg_len;
+            it.t1 = min(t0 + len, it.t0 + p.seg_len);
+            if (it.nseg > 1 && it.ws + it.nseg > ws_slots) it.n = p.N;
+            return it;
+        }
+        before += __shfl_sync(0xffffffffu, cs, 31);
+        ws += __shfl_sync(0xffffffffu, wsum, 31);
+    }
+    return it;
+}
+
+// ---------------------------------------------------------------------------
+
+constexpr int kThreads = 18 * 32;  // 8 state warps, 4 scaling warps, 4 score/output warps, loads, products
+
+template <bool kStateOnly>
+struct Lay {
+    static constexpr int kStages = kStateOnly ? 3 : 2;
+    static constexpr int kGates = kStages + 2;  // gates outlive their tiles (read by the state and output warps)
+    static constexpr int kU = kStateOnly ? 2 : 1;
+    static constexpr uint32_t kStage = (kStateOnly ? 2 : 3) * kTile;
+    static constexpr uint32_t oK = kStateOnly ? 0 : kTile, oV = oK + kTile;  // inside a stage; q at 0
+    static constexpr uint32_t kw = kStages * kStage;                        // three terms of the scaled k
+    static constexpr uint32_t ps = kw + 3 * kTile;                          // two buffers of P's two terms
+    static constexpr uint32_t kP = C * C * 2;
+    static constexpr uint32_t gates = ps + (kStateOnly ? 0 : 4 * kP);
+    static constexpr uint32_t kGate = 3 * C * 4 + 16;
+    static constexpr uint32_t bars = gates + kGates * kGate;
+    static constexpr uint32_t total = bars + 256;
+};
+
+struct Gate {
+    float c2[C];  // c_i / ln 2
+    float e[C];   // e^{c_i}
+    float w[C];   // e^{c_63 - c_i}
+    float a;      // e^{c_63}
+};
+static_assert(sizeof(Gate) <= 3 * C * 4 + 16, "gate slot");
+
+struct Bars {
+    uint64_t full[3], empty[3], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready, s_ready, o_full, o_free, drain;
+    uint32_t tmem;
+    volatile int abort;
+    Item item;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+constexpr long long kWaitBudget = 1ll << 30;  // cycles, about half a second
+
+// Bounded wait: false once it, or any other wait of this CTA, has run out.
+__device__ __forceinline__ bool wait_bar(Bars& B, uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity & 1u)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity & 1u)) {
+        if (B.abort) return false;
+        if (clock64() - t0 > kWaitBudget) {
+            B.abort = 1;
+            atomicOr(&g_device_status, kDevStatTimeout);
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// One [64 tokens][64] box of a [T, heads, 128] bf16 tensor, 128-byte swizzle.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int head, int t, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(t), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Tensor-memory columns
+constexpr uint32_t kColU = 0, kColSHi = 128, kColSLo = 192, kColP = 256, kColO1 = 384, kColO2 = 448;
+
+template <bool kStateOnly>
+__global__ void __launch_bounds__(kThreads, 1)
+    decay_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mq,
+                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, int ws_slots) {
+    using L = Lay<kStateOnly>;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int slot = blockIdx.x / p.HV, h = blockIdx.x % p.HV, hq = h / p.rep;
+    const uint32_t sb = smem_u32(sm);
+
+    if (!kStateOnly && slot == p.slots) {  // tokens of no sequence: zero outputs
         const int c0 = cu_at(p.cu, p.cu64, 0, p.T), c1 = cu_at(p.cu, p.cu64, p.N, p.T);
-        for (int t = warp; t < p.T; t += 4)
-            if (t < c0 || t >= c1) p.out[((size_t)t * p.HV + h) * kDim + rb * 32 + lane] = __float2bfloat16_rn(0.f);
+        for (int t = tid >> 4; t < p.T; t += kThreads / 16) {
+            if (t < c0 || t >= c1)
+                *reinterpret_cast<uint4*>(p.out + ((size_t)t * p.HV + h) * kDim + 8 * (tid & 15)) = make_uint4(0, 0, 0, 0);
+        }
         return;
     }
-    const int t0 = cu_at(p.cu, p.cu64, n, p.T), t1 = cu_at(p.cu, p.cu64, n + 1, p.T);
-    float4 s[2][4];
+
+    if (warp == 16) {
+        const Item it = find_item<kStateOnly>(p, slot, ws_slots);
+        if (lane == 0) {
+            B.item = it;
+            B.abort = 0;
 #pragma unroll
-    for (int ps = 0; ps < 2; ++ps) {
-        if (p.state != nullptr)
-            StateRow<false>::load(p.state, (size_t)nh * kDim + row + 4 * ps, sub, s[ps]);
-        else
+            for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[ps][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    for (int t = t0; t < t1; ++t) {
-        const size_t qk = ((size_t)t * p.H + hq) * kDim, vo = ((size_t)t * p.HV + h) * kDim + row;
-        const float a = expf(clamp_log_decay(p.log_decay[p.per_token ? (size_t)t * p.HV + h : h]));
-        float4 q[4], k[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            q[j] = load_bf16x4(p.q + qk + 4 * sub + 32 * j);
-            k[j] = load_bf16x4(p.k + qk + 4 * sub + 32 * j);
-        }
-#pragma unroll
-        for (int ps = 0; ps < 2; ++ps) {
-            const float vv = bf16_to_f32(p.v[vo + 4 * ps]);
-            float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[ps][j] = gs_plus_dk(a, s[ps][j], vv, k[j]);
-                acc = dot4_acc2(s[ps][j], q[j], acc);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&B.qk_full[i], 1), mbar_init(&B.p_ready[i], 64);
+                mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
             }
-            float o = acc.x + acc.y;
-            o += __shfl_xor_sync(0xffffffffu, o, 1);
-            o += __shfl_xor_sync(0xffffffffu, o, 2);
-            o += __shfl_xor_sync(0xffffffffu, o, 4);
-            if (sub == 0) p.out[vo + 4 * ps] = __float2bfloat16_rn(p.scale * o);
+            mbar_init(&B.kw_ready, 128);
+            mbar_init(&B.s_ready, 256);
+            mbar_init(&B.o_full, 1);
+            mbar_init(&B.o_free, 128);
+            mbar_init(&B.drain, 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+    }
+    if (warp == 17) {
+        tmem_alloc(&B.tmem, kStateOnly ? 256 : 512);
+        tmem_relinquish();
+    }
+    if (!kStateOnly && tid < 256) {  // the upper right quarter of P (rows 0..31, columns 32..63) stays zero
+        const int buf = tid >> 6, row = (tid & 63) >> 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int chunk = 4 + 2 * (tid & 1) + i;
+            *reinterpret_cast<uint4*>(sm + L::ps + buf * L::kP + row * 128 + ((chunk ^ (row & 7)) << 4)) =
+                make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const Item it = B.item;
+    const uint32_t tm = B.tmem;
+    const int nch = it.n < p.N ? (it.t1 - it.t0 + C - 1) / C : 0;
+    const size_t seq_head = (size_t)it.n * p.HV + h;
+
+    if (it.n >= p.N) {
+        // no such segment
+    } else if (warp < 8) {
+        // ---- state: row v of 128, half the columns, in registers ----
+        const int v = 32 * (warp & 3) + lane, half = warp >> 2;
+        const uint32_t tl = tm + ((uint32_t)(32 * (warp & 3)) << 16);
+        float s[64];
+        const size_t at = (size_t)v * kDim + 64 * half;
+        const float* src = nullptr;
+        if (!kStateOnly) {
+            if (it.s > 0 || (it.nseg > 1 && p.first_from_ws))
+                src = p.ws_state + ((size_t)(it.ws + it.s) * p.HV + h) * kDim * kDim + at;
+            else if (p.state != nullptr)
+                src = p.state + seq_head * kDim * kDim + at;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 x = src ? __ldcs(reinterpret_cast<const float4*>(src) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
+        }
+        auto put_terms = [&]() {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float x = s[32 * i + 2 * j], y = s[32 * i + 2 * j + 1];
+                    hi[j] = pack_bf16(x, y);
+                    const float2 b = widen2(hi[j]);
+                    lo[j] = pack_bf16(x - b.x, y - b.y);
+                }
+                tmem_st16_u32_nowait(tl + kColSHi + 32 * half + 16 * i, hi);
+                tmem_st16_u32_nowait(tl + kColSLo + 32 * half + 16 * i, lo);
+            }
+            tmem_wait_st();
+            fence_before_sync();
+            arrive(&B.s_ready);
+        };
+        if (!kStateOnly && nch > 0) put_terms();
+        float prod = 1.f;
+        for (int c = 0; c < nch; ++c) {
+            const int ub = kStateOnly ? c & 1 : 0;
+            if (!wait_bar(B, &B.u_full[ub], kStateOnly ? c >> 1 : c)) break;
+            fence_after_sync();
+            const float a = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate)->a;
+            prod *= a;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float u[16];
+                tmem_ld16(tl + kColU + 128 * ub + 64 * half + 16 * i, u);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[16 * i + j] = fmaf(a, s[16 * i + j], u[j]);
+            }
+            fence_before_sync();
+            arrive(&B.u_free[ub]);
+            if (!kStateOnly && c + 1 < nch) {
+                if (!wait_bar(B, &B.o_full, c)) break;  // S's terms are free once the products with them are done
+                fence_after_sync();
+                put_terms();
+            }
+        }
+        float* dst = nullptr;
+        if (kStateOnly)
+            dst = p.ws_state + ((size_t)(it.ws + it.s + 1) * p.HV + h) * kDim * kDim + at;
+        else if (it.s == it.nseg - 1)
+            dst = p.new_state + seq_head * kDim * kDim + at;
+        if (dst != nullptr)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                reinterpret_cast<float4*>(dst)[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+        if (kStateOnly && tid == 0) p.ws_decay[(size_t)(it.ws + it.s + 1) * p.HV + h] = prod;
+    } else if (warp < 12) {
+        // ---- w_j k_j in three terms, at the same place of three tiles ----
+        const int x = tid - 256;
+        for (int c = 0; c < nch; ++c) {
+            const int st = c % L::kStages;
+            if (!wait_bar(B, &B.full[st], c / L::kStages)) break;
+            const int live = it.t1 - it.t0 - c * C;  // rows of this chunk that belong to the segment
+            const Gate* gt = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
+            if (live < C)  // what follows the segment must not meet a zero weight as 0 * NaN
+                for (int i = x; i < 2 * C * 8; i += 128)
+                    if ((i >> 3 & (C - 1)) >= live)
+                        *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
+            if (c > 0 && !wait_bar(B, &B.u_full[kStateOnly ? (c - 1) & 1 : 0], kStateOnly ? (c - 1) >> 1 : c - 1)) break;
+            const uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
+            uint8_t* kw = sm + L::kw + 16 * x;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = (16 * i + (x >> 3)) & (C - 1);
+                const uint4 r = *reinterpret_cast<const uint4*>(ks + 2048 * i);
+                const uint32_t in[4] = {r.x, r.y, r.z, r.w};
+                const float w = gt->w[row];
+                const float2 w2 = make_float2(w, w);
+                uint32_t t0[4], t1[4], t2[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float2 y = __fmul2_rn(w2, widen2(in[e]));
+                    if (row >= live) y = make_float2(0.f, 0.f);
+                    t0[e] = pack_bf16(y.x, y.y);
+                    float2 b = widen2(t0[e]);
+                    y = make_float2(y.x - b.x, y.y - b.y);
+                    t1[e] = pack_bf16(y.x, y.y);
+                    b = widen2(t1[e]);
+                    t2[e] = pack_bf16(y.x - b.x, y.y - b.y);
+                }
+                *reinterpret_cast<uint4*>(kw + 2048 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
+                *reinterpret_cast<uint4*>(kw + kTile + 2048 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
+                *reinterpret_cast<uint4*>(kw + 2 * kTile + 2048 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
+            }
+            fence_proxy_async_smem();
+            arrive(&B.kw_ready);
+        }
+    } else if (warp < 16) {
+        if (!kStateOnly) {
+            // ---- decayed scores (two warps: 64 rows), then outputs (four warps: 128 v) ----
+            const int wq = warp - 12, i = 32 * wq + lane;
+            const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
+            auto scores = [&](int c) -> bool {
+                if (wq >= 2) return true;
+                if (!wait_bar(B, &B.qk_full[c & 1], c >> 1)) return false;
+                fence_after_sync();
+                const Gate* gt = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
+                const float ci = gt->c2[i];
+                uint8_t* row = sm + L::ps + (c & 1) * 2 * L::kP + i * 128;
+                for (int jb = 0; jb <= wq; ++jb) {
+                    float x[32];
+                    tmem_ld32(tl + kColP + 64 * (c & 1) + 32 * jb, x);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[32 * jb + j]);
+                        x[j] = jb < wq || j <= lane ? x[j] * ex2(ci - cj.x) : 0.f;
+                        x[j + 1] = jb < wq || j + 1 <= lane ? x[j + 1] * ex2(ci - cj.y) : 0.f;
+                        x[j + 2] = jb < wq || j + 2 <= lane ? x[j + 2] * ex2(ci - cj.z) : 0.f;
+                        x[j + 3] = jb < wq || j + 3 <= lane ? x[j + 3] * ex2(ci - cj.w) : 0.f;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float a = x[8 * q + 2 * e], b = x[8 * q + 2 * e + 1];
+                            hi[e] = pack_bf16(a, b);
+                            const float2 r = widen2(hi[e]);
+                            lo[e] = pack_bf16(a - r.x, b - r.y);
+                        }
+                        const uint32_t o = ((4 * jb + q) ^ (i & 7)) << 4;
+                        *reinterpret_cast<uint4*>(row + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(row + L::kP + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+                fence_before_sync();
+                fence_proxy_async_smem();
+                arrive(&B.p_ready[c & 1]);
+                return true;
+            };
+            bool ok = nch == 0 || scores(0);
+            for (int c = 0; ok && c < nch; ++c) {
+                if (c + 1 < nch && !scores(c + 1)) break;
+                if (!wait_bar(B, &B.o_full, c)) break;
+                fence_after_sync();
+                const Gate* gt = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
+                const int live = min(C, it.t1 - it.t0 - c * C);
+                __nv_bfloat16* dst = p.out + ((size_t)(it.t0 + c * C) * p.HV + h) * kDim + 32 * wq + lane;
+                const size_t step = (size_t)p.HV * kDim;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    float x1[32], x2[32];
+                    tmem_ld32x2(tl + kColO1 + 32 * b, tl + kColO2 + 32 * b, x1, x2);
+                    if (b == 1) {
+                        fence_before_sync();
+                        arrive(&B.o_free);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 e = *reinterpret_cast<const float4*>(&gt->e[32 * b + j]);
+                        x1[j] = p.scale * fmaf(e.x, x2[j], x1[j]);
+                        x1[j + 1] = p.scale * fmaf(e.y, x2[j + 1], x1[j + 1]);
+                        x1[j + 2] = p.scale * fmaf(e.z, x2[j + 2], x1[j + 2]);
+                        x1[j + 3] = p.scale * fmaf(e.w, x2[j + 3], x1[j + 3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (32 * b + j < live) dst[(32 * b + j) * step] = __float2bfloat16_rn(x1[j]);
+                }
+            }
+        }
+    } else if (warp == 16) {
+        // ---- loads and gates: lane l has tokens 2 l and 2 l + 1 ----
+        const int len = it.t1 - it.t0;
+        auto gates_of = [&](int c, float& g0, float& g1) {
+            const int a = c * C + 2 * lane;
+            g0 = g1 = 0.f;
+            if (a < len) g0 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a) * p.HV + h : h]);
+            if (a + 1 < len) g1 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a + 1) * p.HV + h : h]);
+        };
+        float g0 = 0.f, g1 = 0.f;
+        if (nch > 0) gates_of(0, g0, g1);
+        int c = 0;
+        for (; c < nch; ++c) {
+            const int st = c % L::kStages;
+            if (c >= L::kStages && !wait_bar(B, &B.empty[st], c / L::kStages - 1)) break;
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&B.full[st], L::kStage);
+                const uint32_t d = sb + st * L::kStage;
+                const int t = it.t0 + c * C;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
+                    tma_box(d + L::oK + x * (kTile / 2), &mk, 64 * x, hq, t, &B.full[st]);
+                    tma_box(d + L::oV + x * (kTile / 2), &mv, 64 * x, h, t, &B.full[st]);
+                }
+            }
+            float pre = g0 + g1, suf = g0 + g1;  // inclusive sums up to and from this lane
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const float a = __shfl_up_sync(0xffffffffu, pre, d), b = __shfl_down_sync(0xffffffffu, suf, d);
+                if (lane >= d) pre += a;
+                if (lane + d < 32) suf += b;
+            }
+            const float tot = __shfl_sync(0xffffffffu, suf, 0);
+            float behind = __shfl_down_sync(0xffffffffu, suf, 1);
+            if (lane == 31) behind = 0.f;
+            const float c1 = pre, c0 = lane == 0 ? g0 : pre - g1;
+            Gate* gt = reinterpret_cast<Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
+            constexpr float kLog2e = 1.4426950408889634f;
+            *reinterpret_cast<float2*>(&gt->c2[2 * lane]) = make_float2(c0 * kLog2e, c1 * kLog2e);
+            *reinterpret_cast<float2*>(&gt->e[2 * lane]) = make_float2(expf(c0), expf(c1));
+            *reinterpret_cast<float2*>(&gt->w[2 * lane]) = make_float2(expf(behind + g1), expf(behind));
+            if (lane == 0) gt->a = expf(tot);
+            __syncwarp();
+            if (lane == 0) arrive(&B.full[st]);
+            if (c + 1 < nch) gates_of(c + 1, g0, g1);
+        }
+        if (c < nch && lane == 0)  // given up: copies in flight land before the CTA ends
+            for (int k = c > L::kStages ? c - L::kStages : 0; k < c; ++k) {
+                const long long t0 = clock64();
+                while (!mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && clock64() - t0 < kWaitBudget) {}
+            }
+    } else {
+      if (lane == 0) {
+        // ---- products, issued by one thread ----
+        constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
+                           id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
+        auto scores = [&](int c) {
+            const uint32_t d = sb + (c % L::kStages) * L::kStage;
+            const uint64_t dq = desc_kmaj(d, C, 0), dk = desc_kmaj(d + L::oK, C, 0);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+                mma_f16(tm + kColP + 64 * (c & 1), desc_add(dq, koff_kmaj(C, 16 * ks)),
+                        desc_add(dk, koff_kmaj(C, 16 * ks)), id_qk, ks > 0);
+            mma_commit(&B.qk_full[c & 1]);
+        };
+        bool ok = true;
+        if (!kStateOnly && nch > 0) {
+            ok = wait_bar(B, &B.full[0], 0);
+            fence_after_sync();
+            if (ok) scores(0);
+        }
+        for (int c = 0; ok && c < nch; ++c) {
+            const int st = c % L::kStages, ub = kStateOnly ? c & 1 : 0;
+            const uint32_t d = sb + st * L::kStage;
+            const uint64_t dv = desc_mnmaj(d + L::oV, C, 0);
+            if (!wait_bar(B, &B.kw_ready, c)) break;
+            if (c >= L::kU && !wait_bar(B, &B.u_free[ub], kStateOnly ? (c >> 1) - 1 : c - 1)) break;
+            fence_after_sync();
+#pragma unroll
+            for (int term = 2; term >= 0; --term)  // small terms first
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    mma_f16(tm + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
+                            desc_add(desc_mnmaj(sb + L::kw + term * kTile, C, 0), koff_mnmaj(16 * ks)), id_u,
+                            term < 2 || ks > 0);
+            mma_commit(&B.u_full[ub]);
+            if (kStateOnly) {
+                mma_commit(&B.empty[st]);
+                continue;
+            }
+            if (c + 1 < nch) {
+                if (!wait_bar(B, &B.full[(c + 1) % L::kStages], (c + 1) / L::kStages)) break;
+                fence_after_sync();
+                scores(c + 1);
+            }
+            if (!wait_bar(B, &B.s_ready, c)) break;
+            if (c > 0 && !wait_bar(B, &B.o_free, c - 1)) break;
+            fence_after_sync();
+            const uint64_t dq = desc_kmaj(d, C, 0);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                mma_f16_ts(tm + kColO2, tm + kColSHi + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, ks > 0);
+                mma_f16_ts(tm + kColO2, tm + kColSLo + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, true);
+            }
+            if (!wait_bar(B, &B.p_ready[c & 1], c >> 1)) break;
+            fence_after_sync();
+            const uint32_t ps = sb + L::ps + (c & 1) * 2 * L::kP;
+#pragma unroll
+            for (int term = 1; term >= 0; --term)
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    mma_f16(tm + kColO1, desc_add(dv, koff_mnmaj(16 * ks)),
+                            desc_add(desc_kmaj(ps + term * L::kP, C, 0), koff_kmaj(C, 16 * ks)), id_pv,
+                            term < 1 || ks > 0);
+            mma_commit(&B.o_full);
+            mma_commit(&B.empty[st]);
+        }
+        if (B.abort) {  // products in flight end before the tensor memory is given back
+            mma_commit(&B.drain);
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitBudget) {}
+        }
+      }
+      __syncwarp();
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    if (warp == 17) tmem_dealloc(tm, kStateOnly ? 256 : 512);
+}
+
+// The state before every segment of the sequences that have several: ws[0] = S,
+// ws[s + 1] = decay[s + 1] ws[s] + ws[s + 1].  1,024 elements of one sequence's
+// v-head per CTA.
+__global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillParams p, int ws_slots) {
+    const int part = blockIdx.x & 15, nh = blockIdx.x >> 4, n = nh / p.HV, h = nh % p.HV;
+    __shared__ Item s_item;
+    // the sequence's place in the workspace: the segments of those before it
+    if (threadIdx.x < 32) {
+        int ws = 0;
+        for (int i = threadIdx.x; i < n; i += 32) {
+            int t0, len;
+            const int k = n_segments(p, i, t0, len);
+            ws += k > 1 ? k : 0;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) ws += __shfl_xor_sync(0xffffffffu, ws, d);
+        if (threadIdx.x == 0) {
+            int t0, len;
+            s_item.nseg = n_segments(p, n, t0, len);
+            s_item.ws = ws;
         }
     }
-#pragma unroll
-    for (int ps = 0; ps < 2; ++ps) StateRow<false>::store(p.new_state, (size_t)nh * kDim + row + 4 * ps, sub, s[ps]);
+    __syncthreads();
+    const int nseg = s_item.nseg, ws = s_item.ws;
+    if (nseg < 2 || ws + nseg > ws_slots) return;
+    const size_t at = (size_t)part * 1024 + 4 * threadIdx.x, step = (size_t)p.HV * kDim * kDim;
+    float* w = p.ws_state + ((size_t)ws * p.HV + h) * kDim * kDim + at;
+    float4 s = p.state ? *reinterpret_cast<const float4*>(p.state + (size_t)nh * kDim * kDim + at)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.first_from_ws) *reinterpret_cast<float4*>(w) = s;
+    float4 u = *reinterpret_cast<const float4*>(w + step);
+    for (int i = 1; i < nseg; ++i) {
+        float4 next = u;
+        if (i + 1 < nseg) next = *reinterpret_cast<const float4*>(w + (i + 1) * step);
+        const float a = p.ws_decay[(size_t)(ws + i) * p.HV + h];
+        s = make_float4(fmaf(a, s.x, u.x), fmaf(a, s.y, u.y), fmaf(a, s.z, u.z), fmaf(a, s.w, u.w));
+        *reinterpret_cast<float4*>(w + i * step) = s;
+        u = next;
+    }
+}
+
+// ---------------------------------------------------------------------------
+
+// The driver's tensor-map encoder, looked up through the runtime once (no
+// link-time dependency on the driver library).
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+    static std::once_flag once;
+    static EncodeFn fn = nullptr;
+    std::call_once(once, []() {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(ptr);
+    });
+    return fn;
+}
+
+// [T, heads, 128] bf16 in boxes of 64 tokens x 64 elements, 128-byte swizzle.
+static bool encode(CUtensorMap* map, const void* x, int heads, int T) {
+    const EncodeFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)kDim, (cuuint64_t)heads, (cuuint64_t)T};
+    const cuuint64_t strides[2] = {(cuuint64_t)kDim * 2, (cuuint64_t)heads * kDim * 2};
+    const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)C}, estr[3] = {1u, 1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Kernel attributes, once per device (again after a failure).
+static bool set_attributes() {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load() & bit)) return true;
+    if (cudaFuncSetAttribute(decay_prefill_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Lay<true>::total) != cudaSuccess ||
+        cudaFuncSetAttribute(decay_prefill_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Lay<false>::total) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    if (dev < 64) done.fetch_or(bit);
+    return true;
+}
+
+// Tokens of a segment: T * HV head-tokens over 148 CTAs, at least 256.
+static int segment_tokens(int T, int HV) {
+    const long long x = ((long long)T * HV + kSms - 1) / kSms, r = (x + C - 1) / C * C;
+    return (int)(r < 256 ? 256 : r > 1 << 30 ? 1 << 30 : r);
+}
+// Workspace slots: a sequence of n > 1 segments has n of them, at most 2 len / segment.
+static int workspace_slots(int T, int HV) {
+    const int seg = segment_tokens(T, HV);
+    return T > seg ? (int)(2ll * T / seg) : 0;
+}
+
+static int status_bits(bool clear) {
+    unsigned int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(v)) != cudaSuccess) return -1;
+    if (clear && v) {
+        const unsigned int z = 0;
+        if (cudaMemcpyToSymbol(g_device_status, &z, sizeof(z)) != cudaSuccess) return -1;
+    }
+    return (int)v;
 }
 
 }  // namespace decay
+
+int decay_prefill_status(bool clear) { return decay::status_bits(clear); }
+
 }  // namespace gdn
 
 extern "C" size_t gdn_decay_prefill_workspace_bytes(int N, int T, int HV) {
-    (void)N, (void)T, (void)HV;
-    return 0;
+    if (N <= 0 || T <= 0 || HV <= 0) return 0;
+    const size_t slots = gdn::decay::workspace_slots(T, HV);
+    return slots * HV * (gdn::kDim * gdn::kDim + 1) * sizeof(float);
 }
 
 extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v, const float* state,
@@ -92,7 +701,8 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         (decay_per_token != 0 && decay_per_token != 1))
         return GDN_ERR_INVALID;
     if (K != gdn::kDim || V != gdn::kDim || HV % H != 0) return GDN_ERR_UNSUPPORTED;
-    if (((long long)N + 1) * HV > (1ll << 27)) return GDN_ERR_UNSUPPORTED;  // grid index
+    const int seg = segment_tokens(T, HV), slots = T / seg + N, ws_slots = N > 0 ? workspace_slots(T, HV) : 0;
+    if (((long long)slots + 1) * HV > (1ll << 27)) return GDN_ERR_UNSUPPORTED;  // grid index
     if (N == 0 && T == 0) return GDN_OK;
     if (!cu_seqlens || (T > 0 && (!q || !k || !v || !out)) || !log_decay || (N > 0 && !new_state))
         return GDN_ERR_INVALID;
@@ -102,16 +712,15 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         return GDN_ERR_ALIGN;
     const size_t need = gdn_decay_prefill_workspace_bytes(N, T, HV);
     if (need && (!workspace || workspace_bytes < need)) return GDN_ERR_INVALID;
-    if (!gdn_aligned(workspace, 16)) return GDN_ERR_ALIGN;
+    if (need && !gdn_aligned(workspace, 16)) return GDN_ERR_ALIGN;
     PrefillParams p;
-    p.q = static_cast<const __nv_bfloat16*>(q);
-    p.k = static_cast<const __nv_bfloat16*>(k);
-    p.v = static_cast<const __nv_bfloat16*>(v);
     p.state = state;
     p.log_decay = log_decay;
     p.cu = cu_seqlens;
     p.out = static_cast<__nv_bfloat16*>(out);
     p.new_state = new_state;
+    p.ws_state = static_cast<float*>(workspace);
+    p.ws_decay = p.ws_state + (size_t)ws_slots * HV * gdn::kDim * gdn::kDim;
     p.scale = scale == 0.0f ? 1.0f / sqrtf((float)K) : scale;
     p.cu64 = cu_seqlens_is_int64;
     p.per_token = decay_per_token;
@@ -120,6 +729,17 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
     p.H = H;
     p.HV = HV;
     p.rep = HV / H;
-    decay_prefill_serial_kernel<<<(unsigned)((N + 1) * HV * 4), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    p.seg_len = seg;
+    p.slots = slots;
+    p.first_from_ws = state != nullptr && state == new_state;
+    CUtensorMap mq{}, mk{}, mv{};
+    if (T > 0 && (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T))) return GDN_ERR_CUDA;
+    if (!set_attributes()) return GDN_ERR_CUDA;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (ws_slots > 0) {
+        decay_prefill_kernel<true><<<(unsigned)(T / seg * HV), kThreads, Lay<true>::total, st>>>(p, mq, mk, mv, ws_slots);
+        decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p, ws_slots);
+    }
+    decay_prefill_kernel<false><<<(unsigned)((slots + 1) * HV), kThreads, Lay<false>::total, st>>>(p, mq, mk, mv, ws_slots);
     return gdn_launch_status();
 }

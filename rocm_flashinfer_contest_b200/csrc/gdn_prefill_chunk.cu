@@ -1868,11 +1868,12 @@ int launch_prefill_chunk(const PrefillParams& p, void* workspace, size_t workspa
 }  // namespace gdn
 
 namespace gdn {
-int mtp_stream_status(bool clear);  // gdn_mtp_stream.cu
+int mtp_stream_status(bool clear);     // gdn_mtp_stream.cu
+int decay_prefill_status(bool clear);  // decay_prefill.cu
 }
 
-// The status words of the prefill's and of the streaming MTP kernel's
-// translation units, or-ed.
+// The status words of the translation units with bounded waits (the prefill,
+// the streaming MTP kernel, the decay prefill), or-ed.
 extern "C" int gdn_device_status(int clear) {
     unsigned int v = 0;
     if (cudaMemcpyFromSymbol(&v, gdn::g_device_status, sizeof(v)) != cudaSuccess) return -1;
@@ -1881,6 +1882,7 @@ extern "C" int gdn_device_status(int clear) {
         if (cudaMemcpyToSymbol(gdn::g_device_status, &z, sizeof(z)) != cudaSuccess) return -1;
     }
     const int m = gdn::mtp_stream_status(clear != 0);
-    if (m < 0) return -1;
-    return (int)(v | (unsigned int)m);
+    const int d = gdn::decay_prefill_status(clear != 0);
+    if (m < 0 || d < 0) return -1;
+    return (int)(v | (unsigned int)m | (unsigned int)d);
 }
