@@ -50,7 +50,7 @@ struct PrefillParams {
     float* ws_state;  // [ws slots][HV][V][K]: the state before a segment (of its predecessor, after the first launch)
     float* ws_decay;  // [ws slots][HV]: e^(sum of a segment's log decays), at its successor's place
     float scale;
-    int cu64, per_token, N, T, H, HV, rep, seg_len, slots;
+    int cu64, per_token, N, T, HV, rep, seg_len, ws_slots;
     int first_from_ws;  // new_state is state: the first of several segments reads the copy in ws_state
 };
 
@@ -59,8 +59,15 @@ __device__ __forceinline__ int cu_at(const void* cu, int is64, int i, int T) {
     return (int)(x < 0 ? 0 : x > T ? T : x);
 }
 
-// A segment: tokens [t0, t1) of sequence n, number s of nseg, workspace slot of
-// the sequence's first segment (sequences of one segment have none).
+// Segments in order of their sequences, found by one warp that asks for
+// ascending numbers: it keeps the block of 32 sequences where it last looked
+// and what came before it.
+struct Finder {
+    int base = 0, before = 0, ws = 0;
+};
+
+// A segment: tokens [t0, t1) of sequence n, number s of nseg, and the workspace
+// slot of the sequence's first segment (sequences of one segment have none).
 struct Item {
     int n, s, nseg, t0, t1, ws;
 };
@@ -72,18 +79,16 @@ __device__ __forceinline__ int n_segments(const PrefillParams& p, int n, int& t0
     return len > p.seg_len ? (len + p.seg_len - 1) / p.seg_len : 1;
 }
 
-// The slot-th segment, counted over the sequences (kInner: over those segments
-// that another one follows); one warp, all lanes get it.  n = N: there is none.
-// Malformed cu_seqlens can make the sequences overlap; the workspace slots are
-// then cut off at the workspace's end.
+// The slot-th segment (kInner: of those that another one follows); n = N: there
+// is none.  Malformed cu_seqlens can make sequences overlap; segments whose
+// workspace slots would lie past the end are then left out.
 template <bool kInner>
-__device__ __forceinline__ Item find_item(const PrefillParams& p, int slot, int ws_slots) {
+__device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int slot) {
     const int lane = threadIdx.x & 31;
     Item it{p.N, 0, 0, 0, 0, 0};
-    int before = 0, ws = 0;
-    for (int base = 0; base < p.N; base += 32) {
+    for (; f.base < p.N; f.base += 32) {
         int t0 = 0, len = 0, nseg = 0;
-        if (base + lane < p.N) nseg = n_segments(p, base + lane, t0, len);
+        if (f.base + lane < p.N) nseg = n_segments(p, f.base + lane, t0, len);
         const int cnt = kInner ? (nseg > 1 ? nseg - 1 : 0) : nseg, wcnt = nseg > 1 ? nseg : 0;
         int cs = cnt, wsum = wcnt;
 #pragma unroll
@@ -91,29 +96,41 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, int slot, int 
             const int x = __shfl_up_sync(0xffffffffu, cs, d), y = __shfl_up_sync(0xffffffffu, wsum, d);
             if (lane >= d) cs += x, wsum += y;
         }
-        const bool here = slot >= before + cs - cnt && slot < before + cs;
-        const unsigned who = __ballot_sync(0xffffffffu, here);
+        const unsigned who = __ballot_sync(0xffffffffu, slot >= f.before + cs - cnt && slot < f.before + cs);
         if (who) {
             const int src = __ffs(who) - 1;
-            it.n = base + src;
-            it.s = slot - (before + __shfl_sync(0xffffffffu, cs - cnt, src));
+            it.n = f.base + src;
+            it.s = slot - (f.before + __shfl_sync(0xffffffffu, cs - cnt, src));
             it.nseg = __shfl_sync(0xffffffffu, nseg, src);
-            it.ws = ws + __shfl_sync(0xffffffffu, wsum - wcnt, src);
+            it.ws = f.ws + __shfl_sync(0xffffffffu, wsum - wcnt, src);
             t0 = __shfl_sync(0xffffffffu, t0, src), len = __shfl_sync(0xffffffffu, len, src);
             it.t0 = t0 + it.s * p.seg_len;
             it.t1 = min(t0 + len, it.t0 + p.seg_len);
-            if (it.nseg > 1 && it.ws + it.nseg > ws_slots) it.n = p.N;
+            if (it.nseg > 1 && it.ws + it.nseg > p.ws_slots) it.n = p.N;
             return it;
         }
-        before += __shfl_sync(0xffffffffu, cs, 31);
-        ws += __shfl_sync(0xffffffffu, wsum, 31);
+        f.before += __shfl_sync(0xffffffffu, cs, 31);
+        f.ws += __shfl_sync(0xffffffffu, wsum, 31);
     }
     return it;
 }
 
 // ---------------------------------------------------------------------------
+// The kernel: one CTA per SM, walking the chunks of segment after segment
+// without a break (a segment without tokens is one chunk without tokens).  24
+// warps, each chunk going through all of them:
+//   warps  0..7   state: half a row of S each thread, fp32, in registers
+//   warps  8..15  w_j k_j in three bf16 terms
+//   warps 16..19  outputs: one v each thread, written 32 v (64 bytes) at a time
+//   warps 20, 21  decayed scores: one row i each thread
+//   warp  22      TMA loads, gates, and what the chunk belongs to
+//   warp  23      one thread that issues the products
+// ---------------------------------------------------------------------------
 
-constexpr int kThreads = 18 * 32;  // 8 state warps, 4 scaling warps, 4 score/output warps, loads, products
+constexpr int kThreads = 24 * 32;
+// Registers per thread by warpgroup; 256 * 112 + 256 * 56 + 128 * (72 + 64) is
+// below the 768 * 80 the CTA is launched with.
+constexpr int kRegsState = 112, kRegsScale = 56, kRegsOut = 72, kRegsRest = 64;
 
 template <bool kStateOnly>
 struct Lay {
@@ -125,32 +142,42 @@ struct Lay {
     static constexpr uint32_t kw = kStages * kStage;                        // three terms of the scaled k
     static constexpr uint32_t ps = kw + 3 * kTile;                          // two buffers of P's two terms
     static constexpr uint32_t kP = C * C * 2;
-    static constexpr uint32_t gates = ps + (kStateOnly ? 0 : 4 * kP);
-    static constexpr uint32_t kGate = 3 * C * 4 + 16;
-    static constexpr uint32_t bars = gates + kGates * kGate;
+    static constexpr uint32_t turn = ps + (kStateOnly ? 0 : 4 * kP);  // 4 KiB for each state warp
+    static constexpr uint32_t gates = turn + 8 * 4096;
+    static constexpr uint32_t bars = gates + kGates * 832;
     static constexpr uint32_t total = bars + 256;
 };
+static_assert(Lay<false>::total <= 227 * 1024 && Lay<true>::total <= 227 * 1024, "shared memory");
 
+enum : int { kFirst = 1, kLast = 2, kFinal = 4 };
+
+// What a chunk's warps need to know of it.
 struct Gate {
     float c2[C];  // c_i / ln 2
-    float e[C];   // e^{c_i}
+    float e[C];   // scale * e^{c_i}
     float w[C];   // e^{c_63 - c_i}
     float a;      // e^{c_63}
+    int flags;    // first / last chunk of its segment, last chunk of this CTA
+    int t, live;  // first token; tokens of the segment from there on, at most 64
+    const float* src;  // first chunk: the state before it (null: zero)
+    float* dst;        // last chunk: where the state after it goes (null: nowhere)
+    float* decay;      // last chunk, kStateOnly: where the segment's decay goes
+    int h;
 };
-static_assert(sizeof(Gate) <= 3 * C * 4 + 16, "gate slot");
+static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
     uint64_t full[3], empty[3], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready, s_ready, o_full, o_free, drain;
     uint32_t tmem;
     volatile int abort;
-    Item item;
+    int none;
 };
 static_assert(sizeof(Bars) <= 256, "barrier block");
 
 constexpr long long kWaitBudget = 1ll << 30;  // cycles, about half a second
 
 // Bounded wait: false once it, or any other wait of this CTA, has run out.
-__device__ __forceinline__ bool wait_bar(Bars& B, uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool wait_one(Bars& B, uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity & 1u)) return true;
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity & 1u)) {
@@ -162,6 +189,10 @@ __device__ __forceinline__ bool wait_bar(Bars& B, uint64_t* bar, uint32_t parity
         }
     }
     return true;
+}
+// The same for a whole warp, which goes on together.
+__device__ __forceinline__ bool wait_bar(Bars& B, uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait_one(B, bar, parity));
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -182,33 +213,43 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The upper halves of two floats, packed: their first 8 significant bits.
+__device__ __forceinline__ uint32_t upper2(float2 x) {
+    return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+}
+// What is left of two floats behind those bits (exact).
+__device__ __forceinline__ float2 below2(float2 x) {
+    const float a = __uint_as_float(__float_as_uint(x.x) & 0xffff0000u), b = __uint_as_float(__float_as_uint(x.y) & 0xffff0000u);
+    return __fadd2_rn(x, make_float2(-a, -b));
+}
+
+template <int kN>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kN));
+}
+template <int kN>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kN));
+}
+
 // Tensor-memory columns
 constexpr uint32_t kColU = 0, kColSHi = 128, kColSLo = 192, kColP = 256, kColO1 = 384, kColO2 = 448;
 
 template <bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     decay_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mq,
-                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, int ws_slots) {
+                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
     using L = Lay<kStateOnly>;
     extern __shared__ __align__(1024) uint8_t sm[];
     Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int slot = blockIdx.x / p.HV, h = blockIdx.x % p.HV, hq = h / p.rep;
     const uint32_t sb = smem_u32(sm);
+    auto gate = [&](int m) { return reinterpret_cast<Gate*>(sm + L::gates + (m % L::kGates) * 832); };
 
-    if (!kStateOnly && slot == p.slots) {  // tokens of no sequence: zero outputs
-        const int c0 = cu_at(p.cu, p.cu64, 0, p.T), c1 = cu_at(p.cu, p.cu64, p.N, p.T);
-        for (int t = tid >> 4; t < p.T; t += kThreads / 16) {
-            if (t < c0 || t >= c1)
-                *reinterpret_cast<uint4*>(p.out + ((size_t)t * p.HV + h) * kDim + 8 * (tid & 15)) = make_uint4(0, 0, 0, 0);
-        }
-        return;
-    }
-
-    if (warp == 16) {
-        const Item it = find_item<kStateOnly>(p, slot, ws_slots);
+    Finder finder;
+    Item it{p.N, 0, 0, 0, 0, 0};
+    if (warp == 22) {
         if (lane == 0) {
-            B.item = it;
             B.abort = 0;
 #pragma unroll
             for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 1);
@@ -217,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_init(&B.qk_full[i], 1), mbar_init(&B.p_ready[i], 64);
                 mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
             }
-            mbar_init(&B.kw_ready, 128);
+            mbar_init(&B.kw_ready, 256);
             mbar_init(&B.s_ready, 256);
             mbar_init(&B.o_full, 1);
             mbar_init(&B.o_free, 128);
@@ -225,8 +266,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_mbar_init();
         }
         __syncwarp();
+        it = find_item<kStateOnly>(p, finder, blockIdx.x / p.HV);
+        if (lane == 0) B.none = it.n >= p.N;
     }
-    if (warp == 17) {
+    if (warp == 23) {
         tmem_alloc(&B.tmem, kStateOnly ? 256 : 512);
         tmem_relinquish();
     }
@@ -243,336 +286,420 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-    const Item it = B.item;
     const uint32_t tm = B.tmem;
-    const int nch = it.n < p.N ? (it.t1 - it.t0 + C - 1) / C : 0;
-    const size_t seq_head = (size_t)it.n * p.HV + h;
+    const bool work = B.none == 0;
 
-    if (it.n >= p.N) {
-        // no such segment
-    } else if (warp < 8) {
+    if (warp < 8) {
         // ---- state: row v of 128, half the columns, in registers ----
-        const int v = 32 * (warp & 3) + lane, half = warp >> 2;
-        const uint32_t tl = tm + ((uint32_t)(32 * (warp & 3)) << 16);
+        more_registers<kRegsState>();
+        const int half = warp >> 2, v0 = 32 * (warp & 3);
+        const uint32_t tl = tm + ((uint32_t)v0 << 16);
+        // rows v0 .. v0 + 31 by 32 columns at a time are turned in shared memory, so that eight
+        // lanes read or write 128 bytes of one row in global memory
+        uint8_t* turn = sm + L::turn + 4096 * warp;
+        const size_t off = (size_t)(v0 + (lane >> 3)) * kDim + 64 * half + 4 * (lane & 7);
+        const int wr = (lane >> 3) * 128, wc = lane & 7, rd = lane * 128;
         float s[64];
-        const size_t at = (size_t)v * kDim + 64 * half;
-        const float* src = nullptr;
-        if (!kStateOnly) {
-            if (it.s > 0 || (it.nseg > 1 && p.first_from_ws))
-                src = p.ws_state + ((size_t)(it.ws + it.s) * p.HV + h) * kDim * kDim + at;
-            else if (p.state != nullptr)
-                src = p.state + seq_head * kDim * kDim + at;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float4 x = src ? __ldcs(reinterpret_cast<const float4*>(src) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
-        }
-        auto put_terms = [&]() {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float x = s[32 * i + 2 * j], y = s[32 * i + 2 * j + 1];
-                    hi[j] = pack_bf16(x, y);
-                    const float2 b = widen2(hi[j]);
-                    lo[j] = pack_bf16(x - b.x, y - b.y);
-                }
-                tmem_st16_u32_nowait(tl + kColSHi + 32 * half + 16 * i, hi);
-                tmem_st16_u32_nowait(tl + kColSLo + 32 * half + 16 * i, lo);
-            }
-            tmem_wait_st();
-            fence_before_sync();
-            arrive(&B.s_ready);
-        };
-        if (!kStateOnly && nch > 0) put_terms();
         float prod = 1.f;
-        for (int c = 0; c < nch; ++c) {
-            const int ub = kStateOnly ? c & 1 : 0;
-            if (!wait_bar(B, &B.u_full[ub], kStateOnly ? c >> 1 : c)) break;
+        for (int m = 0; work; ++m) {
+            const Gate* gt = gate(m);
+            if (!kStateOnly) {
+                if (!wait_bar(B, &B.full[m % L::kStages], m / L::kStages)) break;
+                if (gt->flags & kFirst) {
+                    const float* src = gt->src;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float4 x = src ? __ldcs(reinterpret_cast<const float4*>(src + off + (i & 7) * 4 * kDim + 32 * (i >> 3)))
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+                        s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
+                    }
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(turn + wr + 512 * i + ((wc ^ ((4 * i + (lane >> 3)) & 7)) << 4)) =
+                                make_float4(s[32 * b + 4 * i], s[32 * b + 4 * i + 1], s[32 * b + 4 * i + 2], s[32 * b + 4 * i + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float4 x = *reinterpret_cast<const float4*>(turn + rd + ((i ^ (lane & 7)) << 4));
+                            s[32 * b + 4 * i] = x.x, s[32 * b + 4 * i + 1] = x.y, s[32 * b + 4 * i + 2] = x.z, s[32 * b + 4 * i + 3] = x.w;
+                        }
+                    }
+                }
+                // S's terms are free once the products with them are done
+                if (m > 0 && !wait_bar(B, &B.o_full, m - 1)) break;
+                fence_after_sync();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 x = make_float2(s[16 * i + 2 * j], s[16 * i + 2 * j + 1]), y = below2(x);
+                        hi[j] = upper2(x);
+                        lo[j] = pack_bf16(y.x, y.y);
+                    }
+                    tmem_st8_u32_nowait(tl + kColSHi + 32 * half + 8 * i, hi);
+                    tmem_st8_u32_nowait(tl + kColSLo + 32 * half + 8 * i, lo);
+                }
+                tmem_wait_st();
+                fence_before_sync();
+                arrive(&B.s_ready);
+            }
+            const int ub = kStateOnly ? m & 1 : 0;
+            if (!wait_bar(B, &B.u_full[ub], kStateOnly ? m >> 1 : m)) break;
             fence_after_sync();
-            const float a = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate)->a;
+            const float a = gt->a;
+            const int flags = gt->flags;
+            float* dst = gt->dst;
+            float* decay = gt->decay;
+            if (kStateOnly && (flags & kFirst)) {
+                prod = 1.f;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) s[i] = 0.f;
+            }
             prod *= a;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float u[16];
                 tmem_ld16(tl + kColU + 128 * ub + 64 * half + 16 * i, u);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) s[16 * i + j] = fmaf(a, s[16 * i + j], u[j]);
+                for (int j = 0; j < 16; j += 2) {
+                    const float2 x = __ffma2_rn(make_float2(a, a), make_float2(s[16 * i + j], s[16 * i + j + 1]), make_float2(u[j], u[j + 1]));
+                    s[16 * i + j] = x.x, s[16 * i + j + 1] = x.y;
+                }
             }
             fence_before_sync();
             arrive(&B.u_free[ub]);
-            if (!kStateOnly && c + 1 < nch) {
-                if (!wait_bar(B, &B.o_full, c)) break;  // S's terms are free once the products with them are done
-                fence_after_sync();
-                put_terms();
-            }
-        }
-        float* dst = nullptr;
-        if (kStateOnly)
-            dst = p.ws_state + ((size_t)(it.ws + it.s + 1) * p.HV + h) * kDim * kDim + at;
-        else if (it.s == it.nseg - 1)
-            dst = p.new_state + seq_head * kDim * kDim + at;
-        if (dst != nullptr)
+            if ((flags & kLast) && dst != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                reinterpret_cast<float4*>(dst)[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-        if (kStateOnly && tid == 0) p.ws_decay[(size_t)(it.ws + it.s + 1) * p.HV + h] = prod;
-    } else if (warp < 12) {
-        // ---- w_j k_j in three terms, at the same place of three tiles ----
+                for (int b = 0; b < 2; ++b) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<float4*>(turn + rd + ((i ^ (lane & 7)) << 4)) =
+                            make_float4(s[32 * b + 4 * i], s[32 * b + 4 * i + 1], s[32 * b + 4 * i + 2], s[32 * b + 4 * i + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<float4*>(dst + off + i * 4 * kDim + 32 * b) =
+                            *reinterpret_cast<const float4*>(turn + wr + 512 * i + ((wc ^ ((4 * i + (lane >> 3)) & 7)) << 4));
+                }
+                if (kStateOnly && tid == 0) *decay = prod;
+            }
+            if (flags & kFinal) break;
+        }
+    } else if (warp < 16) {
+        // ---- w_j k_j in three terms of 8 bits each (exact), at the same place of three tiles ----
+        fewer_registers<kRegsScale>();
         const int x = tid - 256;
-        for (int c = 0; c < nch; ++c) {
-            const int st = c % L::kStages;
-            if (!wait_bar(B, &B.full[st], c / L::kStages)) break;
-            const int live = it.t1 - it.t0 - c * C;  // rows of this chunk that belong to the segment
-            const Gate* gt = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
+        for (int m = 0; work; ++m) {
+            const int st = m % L::kStages;
+            if (!wait_bar(B, &B.full[st], m / L::kStages)) break;
+            const Gate* gt = gate(m);
+            const int live = gt->live, flags = gt->flags;
             if (live < C)  // what follows the segment must not meet a zero weight as 0 * NaN
-                for (int i = x; i < 2 * C * 8; i += 128)
+                for (int i = x; i < 2 * C * 8; i += 256)
                     if ((i >> 3 & (C - 1)) >= live)
                         *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
-            if (c > 0 && !wait_bar(B, &B.u_full[kStateOnly ? (c - 1) & 1 : 0], kStateOnly ? (c - 1) >> 1 : c - 1)) break;
+            if (m > 0 && !wait_bar(B, &B.u_full[kStateOnly ? (m - 1) & 1 : 0], kStateOnly ? (m - 1) >> 1 : m - 1)) break;
             const uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
             uint8_t* kw = sm + L::kw + 16 * x;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = (16 * i + (x >> 3)) & (C - 1);
-                const uint4 r = *reinterpret_cast<const uint4*>(ks + 2048 * i);
+#pragma unroll 2
+            for (int i = 0; i < 4; ++i) {
+                const int row = (32 * i + (x >> 3)) & (C - 1);
+                const uint4 r = *reinterpret_cast<const uint4*>(ks + 4096 * i);
                 const uint32_t in[4] = {r.x, r.y, r.z, r.w};
                 const float w = gt->w[row];
-                const float2 w2 = make_float2(w, w);
                 uint32_t t0[4], t1[4], t2[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float2 y = __fmul2_rn(w2, widen2(in[e]));
-                    if (row >= live) y = make_float2(0.f, 0.f);
-                    t0[e] = pack_bf16(y.x, y.y);
-                    float2 b = widen2(t0[e]);
-                    y = make_float2(y.x - b.x, y.y - b.y);
-                    t1[e] = pack_bf16(y.x, y.y);
-                    b = widen2(t1[e]);
-                    t2[e] = pack_bf16(y.x - b.x, y.y - b.y);
+                    float2 y = __fmul2_rn(make_float2(w, w), widen2(row < live ? in[e] : 0u));
+                    t0[e] = upper2(y);
+                    y = below2(y);
+                    t1[e] = upper2(y);
+                    t2[e] = upper2(below2(y));
                 }
-                *reinterpret_cast<uint4*>(kw + 2048 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
-                *reinterpret_cast<uint4*>(kw + kTile + 2048 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
-                *reinterpret_cast<uint4*>(kw + 2 * kTile + 2048 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
+                *reinterpret_cast<uint4*>(kw + 4096 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
+                *reinterpret_cast<uint4*>(kw + kTile + 4096 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
+                *reinterpret_cast<uint4*>(kw + 2 * kTile + 4096 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
             }
             fence_proxy_async_smem();
             arrive(&B.kw_ready);
+            if (flags & kFinal) break;
         }
-    } else if (warp < 16) {
+    } else if (warp < 20) {
+        fewer_registers<kRegsOut>();
         if (!kStateOnly) {
-            // ---- decayed scores (two warps: 64 rows), then outputs (four warps: 128 v) ----
-            const int wq = warp - 12, i = 32 * wq + lane;
+            // ---- outputs ----
+            const int wq = warp - 16;
             const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
-            auto scores = [&](int c) -> bool {
-                if (wq >= 2) return true;
-                if (!wait_bar(B, &B.qk_full[c & 1], c >> 1)) return false;
-                fence_after_sync();
-                const Gate* gt = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
-                const float ci = gt->c2[i];
-                uint8_t* row = sm + L::ps + (c & 1) * 2 * L::kP + i * 128;
-                for (int jb = 0; jb <= wq; ++jb) {
-                    float x[32];
-                    tmem_ld32(tl + kColP + 64 * (c & 1) + 32 * jb, x);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[32 * jb + j]);
-                        x[j] = jb < wq || j <= lane ? x[j] * ex2(ci - cj.x) : 0.f;
-                        x[j + 1] = jb < wq || j + 1 <= lane ? x[j + 1] * ex2(ci - cj.y) : 0.f;
-                        x[j + 2] = jb < wq || j + 2 <= lane ? x[j + 2] * ex2(ci - cj.z) : 0.f;
-                        x[j + 3] = jb < wq || j + 3 <= lane ? x[j + 3] * ex2(ci - cj.w) : 0.f;
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float a = x[8 * q + 2 * e], b = x[8 * q + 2 * e + 1];
-                            hi[e] = pack_bf16(a, b);
-                            const float2 r = widen2(hi[e]);
-                            lo[e] = pack_bf16(a - r.x, b - r.y);
-                        }
-                        const uint32_t o = ((4 * jb + q) ^ (i & 7)) << 4;
-                        *reinterpret_cast<uint4*>(row + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(row + L::kP + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    }
+            const size_t step = (size_t)p.HV * kDim;
+            {  // tokens of no sequence: zeros
+                const int c0 = cu_at(p.cu, p.cu64, 0, p.T), c1 = max(c0, cu_at(p.cu, p.cu64, p.N, p.T));
+                const long long rows = (long long)(c0 + p.T - c1) * p.HV;
+                for (long long i = (long long)blockIdx.x * 8 + ((tid - 512) >> 4); i < rows; i += (long long)gridDim.x * 8) {
+                    const long long r = i / p.HV;
+                    *reinterpret_cast<uint4*>(p.out + ((r < c0 ? r : r - c0 + c1) * p.HV + i % p.HV) * kDim + 8 * (tid & 15)) =
+                        make_uint4(0, 0, 0, 0);
                 }
-                fence_before_sync();
-                fence_proxy_async_smem();
-                arrive(&B.p_ready[c & 1]);
-                return true;
-            };
-            bool ok = nch == 0 || scores(0);
-            for (int c = 0; ok && c < nch; ++c) {
-                if (c + 1 < nch && !scores(c + 1)) break;
-                if (!wait_bar(B, &B.o_full, c)) break;
+            }
+            for (int m = 0; work; ++m) {
+                if (!wait_bar(B, &B.o_full, m)) break;
                 fence_after_sync();
-                const Gate* gt = reinterpret_cast<const Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
-                const int live = min(C, it.t1 - it.t0 - c * C);
-                __nv_bfloat16* dst = p.out + ((size_t)(it.t0 + c * C) * p.HV + h) * kDim + 32 * wq + lane;
-                const size_t step = (size_t)p.HV * kDim;
+                const Gate* gt = gate(m);
+                const int live = gt->live, flags = gt->flags;
+                __nv_bfloat16* dst = p.out + ((size_t)gt->t * p.HV + gt->h) * kDim + 32 * wq + lane;
+#pragma unroll 1
+                for (int b = 0; b < 4; ++b) {
+                    float x1[16], x2[16];
+                    tmem_ld16x2(tl + kColO1 + 16 * b, tl + kColO2 + 16 * b, x1, x2);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    float x1[32], x2[32];
-                    tmem_ld32x2(tl + kColO1 + 32 * b, tl + kColO2 + 32 * b, x1, x2);
-                    if (b == 1) {
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 e = *reinterpret_cast<const float4*>(&gt->e[16 * b + j]);
+                        x1[j] = fmaf(e.x, x2[j], p.scale * x1[j]);
+                        x1[j + 1] = fmaf(e.y, x2[j + 1], p.scale * x1[j + 1]);
+                        x1[j + 2] = fmaf(e.z, x2[j + 2], p.scale * x1[j + 2]);
+                        x1[j + 3] = fmaf(e.w, x2[j + 3], p.scale * x1[j + 3]);
+                    }
+                    if (b == 3) {
                         fence_before_sync();
                         arrive(&B.o_free);
                     }
+                    if (live == C) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 e = *reinterpret_cast<const float4*>(&gt->e[32 * b + j]);
-                        x1[j] = p.scale * fmaf(e.x, x2[j], x1[j]);
-                        x1[j + 1] = p.scale * fmaf(e.y, x2[j + 1], x1[j + 1]);
-                        x1[j + 2] = p.scale * fmaf(e.z, x2[j + 2], x1[j + 2]);
-                        x1[j + 3] = p.scale * fmaf(e.w, x2[j + 3], x1[j + 3]);
+                        for (int j = 0; j < 16; ++j) dst[j * step] = __float2bfloat16_rn(x1[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (16 * b + j < live) dst[j * step] = __float2bfloat16_rn(x1[j]);
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (32 * b + j < live) dst[(32 * b + j) * step] = __float2bfloat16_rn(x1[j]);
+                    dst += 16 * step;
                 }
+                if (flags & kFinal) break;
             }
         }
-    } else if (warp == 16) {
-        // ---- loads and gates: lane l has tokens 2 l and 2 l + 1 ----
-        const int len = it.t1 - it.t0;
-        auto gates_of = [&](int c, float& g0, float& g1) {
-            const int a = c * C + 2 * lane;
-            g0 = g1 = 0.f;
-            if (a < len) g0 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a) * p.HV + h : h]);
-            if (a + 1 < len) g1 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a + 1) * p.HV + h : h]);
-        };
-        float g0 = 0.f, g1 = 0.f;
-        if (nch > 0) gates_of(0, g0, g1);
-        int c = 0;
-        for (; c < nch; ++c) {
-            const int st = c % L::kStages;
-            if (c >= L::kStages && !wait_bar(B, &B.empty[st], c / L::kStages - 1)) break;
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&B.full[st], L::kStage);
-                const uint32_t d = sb + st * L::kStage;
-                const int t = it.t0 + c * C;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
-                    tma_box(d + L::oK + x * (kTile / 2), &mk, 64 * x, hq, t, &B.full[st]);
-                    tma_box(d + L::oV + x * (kTile / 2), &mv, 64 * x, h, t, &B.full[st]);
-                }
-            }
-            float pre = g0 + g1, suf = g0 + g1;  // inclusive sums up to and from this lane
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const float a = __shfl_up_sync(0xffffffffu, pre, d), b = __shfl_down_sync(0xffffffffu, suf, d);
-                if (lane >= d) pre += a;
-                if (lane + d < 32) suf += b;
-            }
-            const float tot = __shfl_sync(0xffffffffu, suf, 0);
-            float behind = __shfl_down_sync(0xffffffffu, suf, 1);
-            if (lane == 31) behind = 0.f;
-            const float c1 = pre, c0 = lane == 0 ? g0 : pre - g1;
-            Gate* gt = reinterpret_cast<Gate*>(sm + L::gates + (c % L::kGates) * L::kGate);
-            constexpr float kLog2e = 1.4426950408889634f;
-            *reinterpret_cast<float2*>(&gt->c2[2 * lane]) = make_float2(c0 * kLog2e, c1 * kLog2e);
-            *reinterpret_cast<float2*>(&gt->e[2 * lane]) = make_float2(expf(c0), expf(c1));
-            *reinterpret_cast<float2*>(&gt->w[2 * lane]) = make_float2(expf(behind + g1), expf(behind));
-            if (lane == 0) gt->a = expf(tot);
-            __syncwarp();
-            if (lane == 0) arrive(&B.full[st]);
-            if (c + 1 < nch) gates_of(c + 1, g0, g1);
-        }
-        if (c < nch && lane == 0)  // given up: copies in flight land before the CTA ends
-            for (int k = c > L::kStages ? c - L::kStages : 0; k < c; ++k) {
-                const long long t0 = clock64();
-                while (!mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && clock64() - t0 < kWaitBudget) {}
-            }
     } else {
-      if (lane == 0) {
-        // ---- products, issued by one thread ----
-        constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
-                           id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
-        auto scores = [&](int c) {
-            const uint32_t d = sb + (c % L::kStages) * L::kStage;
-            const uint64_t dq = desc_kmaj(d, C, 0), dk = desc_kmaj(d + L::oK, C, 0);
+        fewer_registers<kRegsRest>();
+        if (warp < 22) {
+            if (!kStateOnly) {
+                // ---- decayed scores ----
+                const int wq = warp - 20, i = 32 * wq + lane;
+                const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
+                for (int m = 0; work; ++m) {
+                    if (!wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
+                    fence_after_sync();
+                    const Gate* gt = gate(m);
+                    const int flags = gt->flags;
+                    const float ci = gt->c2[i];
+                    uint8_t* row = sm + L::ps + (m & 1) * 2 * L::kP + i * 128;
+                    // this buffer's last product is that of chunk m - 2
+                    if (m > 1 && !wait_bar(B, &B.empty[(m - 2) % L::kStages], (m - 2) / L::kStages)) break;
+#pragma unroll 1
+                    for (int jb = 0; jb < 2 * wq + 2; ++jb) {  // 16 columns at a time
+                        float x[16];
+                        tmem_ld16(tl + kColP + 64 * (m & 1) + 16 * jb, x);
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-                mma_f16(tm + kColP + 64 * (c & 1), desc_add(dq, koff_kmaj(C, 16 * ks)),
-                        desc_add(dk, koff_kmaj(C, 16 * ks)), id_qk, ks > 0);
-            mma_commit(&B.qk_full[c & 1]);
-        };
-        bool ok = true;
-        if (!kStateOnly && nch > 0) {
-            ok = wait_bar(B, &B.full[0], 0);
-            fence_after_sync();
-            if (ok) scores(0);
-        }
-        for (int c = 0; ok && c < nch; ++c) {
-            const int st = c % L::kStages, ub = kStateOnly ? c & 1 : 0;
-            const uint32_t d = sb + st * L::kStage;
-            const uint64_t dv = desc_mnmaj(d + L::oV, C, 0);
-            if (!wait_bar(B, &B.kw_ready, c)) break;
-            if (c >= L::kU && !wait_bar(B, &B.u_free[ub], kStateOnly ? (c >> 1) - 1 : c - 1)) break;
-            fence_after_sync();
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[16 * jb + j]);
+                            x[j] = 16 * jb + j <= i ? x[j] * ex2(ci - cj.x) : 0.f;
+                            x[j + 1] = 16 * jb + j + 1 <= i ? x[j + 1] * ex2(ci - cj.y) : 0.f;
+                            x[j + 2] = 16 * jb + j + 2 <= i ? x[j + 2] * ex2(ci - cj.z) : 0.f;
+                            x[j + 3] = 16 * jb + j + 3 <= i ? x[j + 3] * ex2(ci - cj.w) : 0.f;
+                        }
 #pragma unroll
-            for (int term = 2; term >= 0; --term)  // small terms first
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_f16(tm + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
-                            desc_add(desc_mnmaj(sb + L::kw + term * kTile, C, 0), koff_mnmaj(16 * ks)), id_u,
-                            term < 2 || ks > 0);
-            mma_commit(&B.u_full[ub]);
-            if (kStateOnly) {
-                mma_commit(&B.empty[st]);
-                continue;
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 a = make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]), r = below2(a);
+                                hi[e] = upper2(a);
+                                lo[e] = pack_bf16(r.x, r.y);
+                            }
+                            const uint32_t o = ((2 * jb + q) ^ (i & 7)) << 4;
+                            *reinterpret_cast<uint4*>(row + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(row + L::kP + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
+                    }
+                    fence_before_sync();
+                    fence_proxy_async_smem();
+                    arrive(&B.p_ready[m & 1]);
+                    if (flags & kFinal) break;
+                }
             }
-            if (c + 1 < nch) {
-                if (!wait_bar(B, &B.full[(c + 1) % L::kStages], (c + 1) / L::kStages)) break;
-                fence_after_sync();
-                scores(c + 1);
+        } else if (warp == 22) {
+            // ---- loads and gates: lane l has tokens 2 l and 2 l + 1 of a chunk ----
+            int m = 0, idx = blockIdx.x;
+            bool ok = work;
+            while (ok && it.n < p.N) {
+                const int h = idx % p.HV, hq = h / p.rep, len = it.t1 - it.t0, nch = len > C ? (len + C - 1) / C : 1;
+                const size_t mat = (size_t)kDim * kDim, wsi = (size_t)(it.ws + it.s) * p.HV + h;
+                const float* src = nullptr;
+                float *dst = nullptr, *decay = nullptr;
+                if (kStateOnly) {
+                    dst = p.ws_state + (wsi + p.HV) * mat;
+                    decay = p.ws_decay + wsi + p.HV;
+                } else {
+                    if (it.s > 0 || (it.nseg > 1 && p.first_from_ws))
+                        src = p.ws_state + wsi * mat;
+                    else if (p.state != nullptr)
+                        src = p.state + ((size_t)it.n * p.HV + h) * mat;
+                    if (it.s == it.nseg - 1) dst = p.new_state + ((size_t)it.n * p.HV + h) * mat;
+                    if (src != nullptr && lane == 0)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
+                }
+                auto gates_of = [&](int c, float& g0, float& g1) {
+                    const int a = c * C + 2 * lane;
+                    g0 = g1 = 0.f;
+                    if (a < len) g0 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a) * p.HV + h : h]);
+                    if (a + 1 < len) g1 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a + 1) * p.HV + h : h]);
+                };
+                float g0, g1;
+                gates_of(0, g0, g1);
+                idx += gridDim.x;
+                const Item next = find_item<kStateOnly>(p, finder, idx / p.HV);
+                for (int c = 0; c < nch; ++c, ++m) {
+                    const int st = m % L::kStages;
+                    if (m >= L::kStages && !wait_bar(B, &B.empty[st], m / L::kStages - 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const int t = it.t0 + c * C;
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&B.full[st], L::kStage);
+                        const uint32_t d = sb + st * L::kStage;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
+                            tma_box(d + L::oK + x * (kTile / 2), &mk, 64 * x, hq, t, &B.full[st]);
+                            tma_box(d + L::oV + x * (kTile / 2), &mv, 64 * x, h, t, &B.full[st]);
+                        }
+                    }
+                    float pre = g0 + g1, suf = g0 + g1;  // inclusive sums up to and from this lane
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) {
+                        const float a = __shfl_up_sync(0xffffffffu, pre, d), b = __shfl_down_sync(0xffffffffu, suf, d);
+                        if (lane >= d) pre += a;
+                        if (lane + d < 32) suf += b;
+                    }
+                    float behind = __shfl_down_sync(0xffffffffu, suf, 1);
+                    if (lane == 31) behind = 0.f;
+                    const float c0 = lane == 0 ? g0 : pre - g1;
+                    Gate* gt = gate(m);
+                    constexpr float kLog2e = 1.4426950408889634f;
+                    *reinterpret_cast<float2*>(&gt->c2[2 * lane]) = make_float2(c0 * kLog2e, pre * kLog2e);
+                    *reinterpret_cast<float2*>(&gt->e[2 * lane]) = make_float2(p.scale * expf(c0), p.scale * expf(pre));
+                    *reinterpret_cast<float2*>(&gt->w[2 * lane]) = make_float2(expf(behind + g1), expf(behind));
+                    if (lane == 0) {
+                        gt->a = expf(suf);
+                        gt->flags = (c == 0 ? kFirst : 0) | (c == nch - 1 ? kLast : 0) |
+                                    (c == nch - 1 && next.n >= p.N ? kFinal : 0);
+                        gt->t = t, gt->live = min(C, len - c * C);
+                        gt->src = src, gt->dst = dst, gt->decay = decay, gt->h = h;
+                    }
+                    __syncwarp();
+                    if (lane == 0) arrive(&B.full[st]);
+                    if (c + 1 < nch) gates_of(c + 1, g0, g1);
+                }
+                it = next;
             }
-            if (!wait_bar(B, &B.s_ready, c)) break;
-            if (c > 0 && !wait_bar(B, &B.o_free, c - 1)) break;
-            fence_after_sync();
-            const uint64_t dq = desc_kmaj(d, C, 0);
+            if (!ok && lane == 0)  // given up: copies in flight land before the CTA ends
+                for (int k = m > L::kStages ? m - L::kStages : 0; k < m; ++k) {
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && clock64() - t0 < kWaitBudget) {}
+                }
+        } else {
+            if (lane == 0 && work) {
+                // ---- products, issued by one thread ----
+                constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
+                                   id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
+                const uint64_t dkw = desc_mnmaj(sb + L::kw, C, 0);
+                auto scores = [&](int m) {
+                    const uint32_t d = sb + (m % L::kStages) * L::kStage;
+                    const uint64_t dq = desc_kmaj(d, C, 0), dk = desc_kmaj(d + L::oK, C, 0);
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                mma_f16_ts(tm + kColO2, tm + kColSHi + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, ks > 0);
-                mma_f16_ts(tm + kColO2, tm + kColSLo + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, true);
+                    for (int ks = 0; ks < 8; ++ks)
+                        mma_f16(tm + kColP + 64 * (m & 1), desc_add(dq, koff_kmaj(C, 16 * ks)),
+                                desc_add(dk, koff_kmaj(C, 16 * ks)), id_qk, ks > 0);
+                    mma_commit(&B.qk_full[m & 1]);
+                };
+                bool ok = true;
+                if (!kStateOnly) {
+                    ok = wait_one(B, &B.full[0], 0);
+                    fence_after_sync();
+                    if (ok) scores(0);
+                }
+                for (int m = 0; ok; ++m) {
+                    const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
+                    const uint32_t d = sb + st * L::kStage;
+                    const uint64_t dv = desc_mnmaj(d + L::oV, C, 0);
+                    if (!wait_one(B, &B.kw_ready, m)) break;
+                    const bool final = gate(m)->flags & kFinal;
+                    if (m >= L::kU && !wait_one(B, &B.u_free[ub], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int term = 2; term >= 0; --term)  // small terms first
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_f16(tm + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
+                                    desc_add(dkw, term * kTile + koff_mnmaj(16 * ks)), id_u, term < 2 || ks > 0);
+                    mma_commit(&B.u_full[ub]);
+                    if (kStateOnly) {
+                        mma_commit(&B.empty[st]);
+                        if (final) break;
+                        continue;
+                    }
+                    if (!final) {
+                        if (!wait_one(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
+                        fence_after_sync();
+                        scores(m + 1);
+                    }
+                    if (!wait_one(B, &B.s_ready, m)) break;
+                    if (m > 0 && !wait_one(B, &B.o_free, m - 1)) break;
+                    fence_after_sync();
+                    const uint64_t dq = desc_kmaj(d, C, 0);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        mma_f16_ts(tm + kColO2, tm + kColSHi + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, ks > 0);
+                        mma_f16_ts(tm + kColO2, tm + kColSLo + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, true);
+                    }
+                    if (!wait_one(B, &B.p_ready[m & 1], m >> 1)) break;
+                    fence_after_sync();
+                    const uint64_t dp = desc_kmaj(sb + L::ps + (m & 1) * 2 * L::kP, C, 0);
+#pragma unroll
+                    for (int term = 1; term >= 0; --term)
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_f16(tm + kColO1, desc_add(dv, koff_mnmaj(16 * ks)),
+                                    desc_add(dp, term * L::kP + koff_kmaj(C, 16 * ks)), id_pv, term < 1 || ks > 0);
+                    mma_commit(&B.o_full);
+                    mma_commit(&B.empty[st]);
+                    if (final) break;
+                }
+                if (B.abort) {  // products in flight end before the tensor memory is given back
+                    mma_commit(&B.drain);
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitBudget) {}
+                }
             }
-            if (!wait_bar(B, &B.p_ready[c & 1], c >> 1)) break;
-            fence_after_sync();
-            const uint32_t ps = sb + L::ps + (c & 1) * 2 * L::kP;
-#pragma unroll
-            for (int term = 1; term >= 0; --term)
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    mma_f16(tm + kColO1, desc_add(dv, koff_mnmaj(16 * ks)),
-                            desc_add(desc_kmaj(ps + term * L::kP, C, 0), koff_kmaj(C, 16 * ks)), id_pv,
-                            term < 1 || ks > 0);
-            mma_commit(&B.o_full);
-            mma_commit(&B.empty[st]);
+            __syncwarp();
         }
-        if (B.abort) {  // products in flight end before the tensor memory is given back
-            mma_commit(&B.drain);
-            const long long t0 = clock64();
-            while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitBudget) {}
-        }
-      }
-      __syncwarp();
     }
+    __syncwarp();
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-    if (warp == 17) tmem_dealloc(tm, kStateOnly ? 256 : 512);
+    if (warp == 23) tmem_dealloc(tm, kStateOnly ? 256 : 512);
 }
 
 // The state before every segment of the sequences that have several: ws[0] = S,
 // ws[s + 1] = decay[s + 1] ws[s] + ws[s + 1].  1,024 elements of one sequence's
 // v-head per CTA.
-__global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillParams p, int ws_slots) {
+__global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillParams p) {
     const int part = blockIdx.x & 15, nh = blockIdx.x >> 4, n = nh / p.HV, h = nh % p.HV;
-    __shared__ Item s_item;
+    __shared__ int s_nseg, s_ws;
     // the sequence's place in the workspace: the segments of those before it
     if (threadIdx.x < 32) {
         int ws = 0;
@@ -585,13 +712,13 @@ __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillP
         for (int d = 16; d > 0; d /= 2) ws += __shfl_xor_sync(0xffffffffu, ws, d);
         if (threadIdx.x == 0) {
             int t0, len;
-            s_item.nseg = n_segments(p, n, t0, len);
-            s_item.ws = ws;
+            s_nseg = n_segments(p, n, t0, len);
+            s_ws = ws;
         }
     }
     __syncthreads();
-    const int nseg = s_item.nseg, ws = s_item.ws;
-    if (nseg < 2 || ws + nseg > ws_slots) return;
+    const int nseg = s_nseg, ws = s_ws;
+    if (nseg < 2 || ws + nseg > p.ws_slots) return;
     const size_t at = (size_t)part * 1024 + 4 * threadIdx.x, step = (size_t)p.HV * kDim * kDim;
     float* w = p.ws_state + ((size_t)ws * p.HV + h) * kDim * kDim + at;
     float4 s = p.state ? *reinterpret_cast<const float4*>(p.state + (size_t)nh * kDim * kDim + at)
@@ -658,10 +785,11 @@ static bool set_attributes() {
     return true;
 }
 
-// Tokens of a segment: T * HV head-tokens over 148 CTAs, at least 256.
+// Tokens of a segment: T over as many as give 148 CTAs one each, at least 256.
 static int segment_tokens(int T, int HV) {
-    const long long x = ((long long)T * HV + kSms - 1) / kSms, r = (x + C - 1) / C * C;
-    return (int)(r < 256 ? 256 : r > 1 << 30 ? 1 << 30 : r);
+    const int parts = HV < kSms ? kSms / HV : 1;
+    const int x = T / parts + (T % parts != 0), r = x > 1 << 30 ? 1 << 30 : (x + C - 1) / C * C;
+    return r < 256 ? 256 : r;
 }
 // Workspace slots: a sequence of n > 1 segments has n of them, at most 2 len / segment.
 static int workspace_slots(int T, int HV) {
@@ -702,7 +830,7 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         return GDN_ERR_INVALID;
     if (K != gdn::kDim || V != gdn::kDim || HV % H != 0) return GDN_ERR_UNSUPPORTED;
     const int seg = segment_tokens(T, HV), slots = T / seg + N, ws_slots = N > 0 ? workspace_slots(T, HV) : 0;
-    if (((long long)slots + 1) * HV > (1ll << 27)) return GDN_ERR_UNSUPPORTED;  // grid index
+    if (((long long)slots + 1) * HV > (1ll << 26)) return GDN_ERR_UNSUPPORTED;  // grid index
     if (N == 0 && T == 0) return GDN_OK;
     if (!cu_seqlens || (T > 0 && (!q || !k || !v || !out)) || !log_decay || (N > 0 && !new_state))
         return GDN_ERR_INVALID;
@@ -726,20 +854,30 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
     p.per_token = decay_per_token;
     p.N = N;
     p.T = T;
-    p.H = H;
     p.HV = HV;
     p.rep = HV / H;
     p.seg_len = seg;
-    p.slots = slots;
+    p.ws_slots = ws_slots;
     p.first_from_ws = state != nullptr && state == new_state;
-    CUtensorMap mq{}, mk{}, mv{};
-    if (T > 0 && (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T))) return GDN_ERR_CUDA;
-    if (!set_attributes()) return GDN_ERR_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (ws_slots > 0) {
-        decay_prefill_kernel<true><<<(unsigned)(T / seg * HV), kThreads, Lay<true>::total, st>>>(p, mq, mk, mv, ws_slots);
-        decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p, ws_slots);
+    if (T == 0) {  // every sequence keeps its state
+        const size_t bytes = (size_t)N * HV * gdn::kDim * gdn::kDim * sizeof(float);
+        cudaError_t e = cudaSuccess;
+        if (state == nullptr)
+            e = cudaMemsetAsync(new_state, 0, bytes, st);
+        else if (state != new_state)
+            e = cudaMemcpyAsync(new_state, state, bytes, cudaMemcpyDeviceToDevice, st);
+        return e == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
     }
-    decay_prefill_kernel<false><<<(unsigned)((slots + 1) * HV), kThreads, Lay<false>::total, st>>>(p, mq, mk, mv, ws_slots);
+    CUtensorMap mq{}, mk{}, mv{};
+    if (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T)) return GDN_ERR_CUDA;
+    if (!set_attributes()) return GDN_ERR_CUDA;
+    if (ws_slots > 0) {
+        const int inner = T / seg * HV;
+        decay_prefill_kernel<true><<<inner < kSms ? inner : kSms, kThreads, Lay<true>::total, st>>>(p, mq, mk, mv);
+        decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p);
+    }
+    const int items = slots * HV;
+    decay_prefill_kernel<false><<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, Lay<false>::total, st>>>(p, mq, mk, mv);
     return gdn_launch_status();
 }
