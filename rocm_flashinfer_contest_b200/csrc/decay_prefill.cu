@@ -117,33 +117,36 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 
 // ---------------------------------------------------------------------------
 // The kernel: one CTA per SM, walking the chunks of segment after segment
-// without a break (a segment without tokens is one chunk without tokens).  24
-// warps, each chunk going through all of them:
-//   warps  0..7   state: half a row of S each thread, fp32, in registers
-//   warps  8..15  w_j k_j in three bf16 terms
-//   warps 16..19  outputs: one v each thread, written 32 v (64 bytes) at a time
-//   warps 20, 21  decayed scores: one row i each thread
-//   warp  22      TMA loads, gates, and what the chunk belongs to
-//   warp  23      one thread that issues the products
+// without a break (a segment without tokens is one chunk without tokens).  Each
+// chunk goes through all of its warps:
+//   warps  0..7       state: half a row of S each thread, fp32, in registers
+//   warps  8..15      w_j k_j in three bf16 terms
+//   warps 16..19      outputs: one v each thread, written 32 v (64 bytes) at a time
+//   warps 20, 21, 25  decayed scores: one row i each thread, 32 columns j
+//   warp  22          TMA loads
+//   warp  23          one thread that issues the products
+//   warp  24          gates, and what the chunk belongs to
+// (a warp reads the 32 tensor-memory lanes of its number modulo 4, hence 25).
 // ---------------------------------------------------------------------------
 
-constexpr int kThreads = 24 * 32;
-// Registers per thread by warpgroup; 256 * 112 + 256 * 56 + 128 * (72 + 64) is
-// below the 768 * 80 the CTA is launched with.
-constexpr int kRegsState = 112, kRegsScale = 56, kRegsOut = 72, kRegsRest = 64;
+constexpr int kThreads = 28 * 32;
+// Registers per thread by warpgroup; 256 * (112 + 48) + 128 * (64 + 56 + 56) is
+// below the 896 * 72 the CTA is launched with.
+constexpr int kRegsState = 112, kRegsScale = 48, kRegsOut = 64, kRegsRest = 56;
+static_assert(256 * (kRegsState + kRegsScale) + 128 * (kRegsOut + 2 * kRegsRest) <= kThreads * 72, "register split");
 
 template <bool kStateOnly>
 struct Lay {
-    static constexpr int kStages = kStateOnly ? 3 : 2;
-    static constexpr int kGates = kStages + 2;  // gates outlive their tiles (read by the state and output warps)
-    static constexpr int kU = kStateOnly ? 2 : 1;
+    static constexpr int kStages = 3;
+    static constexpr int kGates = kStages + 2;       // gates outlive their tiles (read by the state and output warps)
+    static constexpr int kBuf = kStateOnly ? 2 : 1;  // buffers of U and of the scaled k's lower terms
     static constexpr uint32_t kStage = (kStateOnly ? 2 : 3) * kTile;
     static constexpr uint32_t oK = kStateOnly ? 0 : kTile, oV = oK + kTile;  // inside a stage; q at 0
-    static constexpr uint32_t kw = kStages * kStage;                        // three terms of the scaled k
-    static constexpr uint32_t ps = kw + 3 * kTile;                          // two buffers of P's two terms
+    static constexpr uint32_t kw = kStages * kStage;  // the scaled k's two lower terms (the first takes k's own place)
+    static constexpr uint32_t ps = kw + kBuf * 2 * kTile;  // two buffers of P's two terms
     static constexpr uint32_t kP = C * C * 2;
-    static constexpr uint32_t turn = ps + (kStateOnly ? 0 : 4 * kP);  // 4 KiB for each state warp
-    static constexpr uint32_t gates = turn + 8 * 4096;
+    static constexpr uint32_t turn = ps + (kStateOnly ? 0 : 4 * kP);  // 1 KiB for each state warp
+    static constexpr uint32_t gates = turn + 8 * 1024;
     static constexpr uint32_t bars = gates + kGates * 832;
     static constexpr uint32_t total = bars + 256;
 };
@@ -167,7 +170,7 @@ struct Gate {
 static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
-    uint64_t full[3], empty[3], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready, s_ready, o_full, o_free, drain;
+    uint64_t full[3], empty[3], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready[2], s_ready, s_free, o_full, o_free, drain;
     uint32_t tmem;
     volatile int abort;
     int none;
@@ -207,6 +210,13 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
         : "memory");
 }
 
+// True in one lane of a converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t x;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+    return x != 0;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -242,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using L = Lay<kStateOnly>;
     extern __shared__ __align__(1024) uint8_t sm[];
     Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t sb = smem_u32(sm);
     auto gate = [&](int m) { return reinterpret_cast<Gate*>(sm + L::gates + (m % L::kGates) * 832); };
 
@@ -255,11 +265,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 1);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&B.qk_full[i], 1), mbar_init(&B.p_ready[i], 64);
+                mbar_init(&B.qk_full[i], 1), mbar_init(&B.p_ready[i], 96), mbar_init(&B.kw_ready[i], 256);
                 mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
             }
-            mbar_init(&B.kw_ready, 256);
             mbar_init(&B.s_ready, 256);
+            mbar_init(&B.s_free, 1);
             mbar_init(&B.o_full, 1);
             mbar_init(&B.o_free, 128);
             mbar_init(&B.drain, 1);
@@ -294,11 +304,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         more_registers<kRegsState>();
         const int half = warp >> 2, v0 = 32 * (warp & 3);
         const uint32_t tl = tm + ((uint32_t)v0 << 16);
-        // rows v0 .. v0 + 31 by 32 columns at a time are turned in shared memory, so that eight
-        // lanes read or write 128 bytes of one row in global memory
-        uint8_t* turn = sm + L::turn + 4096 * warp;
-        const size_t off = (size_t)(v0 + (lane >> 3)) * kDim + 64 * half + 4 * (lane & 7);
-        const int wr = (lane >> 3) * 128, wc = lane & 7, rd = lane * 128;
+        // rows v0 .. v0 + 31 are turned in shared memory by 8 columns at a time, so that two
+        // lanes read or write 32 bytes of one row in global memory
+        uint8_t* turn = sm + L::turn + 1024 * warp;
+        const size_t off = (size_t)(v0 + (lane >> 1)) * kDim + 64 * half + 4 * (lane & 1);
+        uint8_t* by_row = turn + lane * 32;  // 16-byte place x of row r holds column group x ^ (r >> 2 & 1)
+        uint8_t* by_pair = turn + (lane >> 1) * 32 + (((lane ^ lane >> 3) & 1) << 4);  // row lane / 2; + 512: 16 rows on
+        const int sw = (lane >> 2 & 1) << 4;
         float s[64];
         float prod = 1.f;
         for (int m = 0; work; ++m) {
@@ -309,27 +321,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float* src = gt->src;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float4 x = src ? __ldcs(reinterpret_cast<const float4*>(src + off + (i & 7) * 4 * kDim + 32 * (i >> 3)))
+                        const float4 x = src ? __ldcs(reinterpret_cast<const float4*>(src + off + (i & 1) * 16 * kDim + 8 * (i >> 1)))
                                              : make_float4(0.f, 0.f, 0.f, 0.f);
                         s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
                     }
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
+                    for (int b = 0; b < 8; ++b) {
+                        float* y = s + 8 * b;
                         __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<float4*>(turn + wr + 512 * i + ((wc ^ ((4 * i + (lane >> 3)) & 7)) << 4)) =
-                                make_float4(s[32 * b + 4 * i], s[32 * b + 4 * i + 1], s[32 * b + 4 * i + 2], s[32 * b + 4 * i + 3]);
+                        *reinterpret_cast<float4*>(by_pair) = make_float4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<float4*>(by_pair + 512) = make_float4(y[4], y[5], y[6], y[7]);
                         __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float4 x = *reinterpret_cast<const float4*>(turn + rd + ((i ^ (lane & 7)) << 4));
-                            s[32 * b + 4 * i] = x.x, s[32 * b + 4 * i + 1] = x.y, s[32 * b + 4 * i + 2] = x.z, s[32 * b + 4 * i + 3] = x.w;
-                        }
+                        const float4 x0 = *reinterpret_cast<const float4*>(by_row + sw);
+                        const float4 x1 = *reinterpret_cast<const float4*>(by_row + (sw ^ 16));
+                        y[0] = x0.x, y[1] = x0.y, y[2] = x0.z, y[3] = x0.w;
+                        y[4] = x1.x, y[5] = x1.y, y[6] = x1.z, y[7] = x1.w;
                     }
                 }
                 // S's terms are free once the products with them are done
-                if (m > 0 && !wait_bar(B, &B.o_full, m - 1)) break;
+                if (m > 0 && !wait_bar(B, &B.s_free, m - 1)) break;
                 fence_after_sync();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -374,17 +384,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             arrive(&B.u_free[ub]);
             if ((flags & kLast) && dst != nullptr) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
+                for (int b = 0; b < 8; ++b) {
+                    const float* y = s + 8 * b;
                     __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<float4*>(turn + rd + ((i ^ (lane & 7)) << 4)) =
-                            make_float4(s[32 * b + 4 * i], s[32 * b + 4 * i + 1], s[32 * b + 4 * i + 2], s[32 * b + 4 * i + 3]);
+                    *reinterpret_cast<float4*>(by_row + sw) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(by_row + (sw ^ 16)) = make_float4(y[4], y[5], y[6], y[7]);
                     __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<float4*>(dst + off + i * 4 * kDim + 32 * b) =
-                            *reinterpret_cast<const float4*>(turn + wr + 512 * i + ((wc ^ ((4 * i + (lane >> 3)) & 7)) << 4));
+                    *reinterpret_cast<float4*>(dst + off + 8 * b) = *reinterpret_cast<const float4*>(by_pair);
+                    *reinterpret_cast<float4*>(dst + off + 16 * kDim + 8 * b) = *reinterpret_cast<const float4*>(by_pair + 512);
                 }
                 if (kStateOnly && tid == 0) *decay = prod;
             }
@@ -403,9 +410,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = x; i < 2 * C * 8; i += 256)
                     if ((i >> 3 & (C - 1)) >= live)
                         *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
-            if (m > 0 && !wait_bar(B, &B.u_full[kStateOnly ? (m - 1) & 1 : 0], kStateOnly ? (m - 1) >> 1 : m - 1)) break;
-            const uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
-            uint8_t* kw = sm + L::kw + 16 * x;
+            // the lower terms' buffer is free after the last product with it, k's place after its scores
+            if (m >= L::kBuf && !wait_bar(B, &B.u_full[kStateOnly ? m & 1 : 0], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
+            if (!kStateOnly && !wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
+            uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
+            uint8_t* kw = sm + L::kw + (kStateOnly ? (m & 1) * 2 * kTile : 0) + 16 * x;
 #pragma unroll 2
             for (int i = 0; i < 4; ++i) {
                 const int row = (32 * i + (x >> 3)) & (C - 1);
@@ -421,12 +430,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     t1[e] = upper2(y);
                     t2[e] = upper2(below2(y));
                 }
-                *reinterpret_cast<uint4*>(kw + 4096 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
-                *reinterpret_cast<uint4*>(kw + kTile + 4096 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
-                *reinterpret_cast<uint4*>(kw + 2 * kTile + 4096 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
+                *reinterpret_cast<uint4*>(ks + 4096 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
+                *reinterpret_cast<uint4*>(kw + 4096 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
+                *reinterpret_cast<uint4*>(kw + kTile + 4096 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
             }
             fence_proxy_async_smem();
-            arrive(&B.kw_ready);
+            arrive(&B.kw_ready[kStateOnly ? m & 1 : 0]);
             if (flags & kFinal) break;
         }
     } else if (warp < 20) {
@@ -458,10 +467,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         const float4 e = *reinterpret_cast<const float4*>(&gt->e[16 * b + j]);
-                        x1[j] = fmaf(e.x, x2[j], p.scale * x1[j]);
-                        x1[j + 1] = fmaf(e.y, x2[j + 1], p.scale * x1[j + 1]);
-                        x1[j + 2] = fmaf(e.z, x2[j + 2], p.scale * x1[j + 2]);
-                        x1[j + 3] = fmaf(e.w, x2[j + 3], p.scale * x1[j + 3]);
+                        const float2 a = __ffma2_rn(make_float2(e.x, e.y), make_float2(x2[j], x2[j + 1]), make_float2(x1[j], x1[j + 1]));
+                        const float2 c = __ffma2_rn(make_float2(e.z, e.w), make_float2(x2[j + 2], x2[j + 3]), make_float2(x1[j + 2], x1[j + 3]));
+                        x1[j] = a.x, x1[j + 1] = a.y, x1[j + 2] = c.x, x1[j + 3] = c.y;
                     }
                     if (b == 3) {
                         fence_before_sync();
@@ -482,10 +490,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         fewer_registers<kRegsRest>();
-        if (warp < 22) {
+        if (warp < 22 || warp == 25) {
             if (!kStateOnly) {
                 // ---- decayed scores ----
-                const int wq = warp - 20, i = 32 * wq + lane;
+                const int wq = warp & 1, i = 32 * wq + lane, jb0 = warp == 25 ? 2 : 0;
                 const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
                 for (int m = 0; work; ++m) {
                     if (!wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
@@ -497,16 +505,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // this buffer's last product is that of chunk m - 2
                     if (m > 1 && !wait_bar(B, &B.empty[(m - 2) % L::kStages], (m - 2) / L::kStages)) break;
 #pragma unroll 1
-                    for (int jb = 0; jb < 2 * wq + 2; ++jb) {  // 16 columns at a time
+                    for (int jb = jb0; jb < jb0 + 2; ++jb) {  // 16 columns at a time
                         float x[16];
                         tmem_ld16(tl + kColP + 64 * (m & 1) + 16 * jb, x);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[16 * jb + j]);
-                            x[j] = 16 * jb + j <= i ? x[j] * ex2(ci - cj.x) : 0.f;
-                            x[j + 1] = 16 * jb + j + 1 <= i ? x[j + 1] * ex2(ci - cj.y) : 0.f;
-                            x[j + 2] = 16 * jb + j + 2 <= i ? x[j + 2] * ex2(ci - cj.z) : 0.f;
-                            x[j + 3] = 16 * jb + j + 3 <= i ? x[j + 3] * ex2(ci - cj.w) : 0.f;
+                            const float2 a = __fmul2_rn(make_float2(p.scale * ex2(ci - cj.x), p.scale * ex2(ci - cj.y)), make_float2(x[j], x[j + 1]));
+                            const float2 c = __fmul2_rn(make_float2(p.scale * ex2(ci - cj.z), p.scale * ex2(ci - cj.w)), make_float2(x[j + 2], x[j + 3]));
+                            x[j] = 16 * jb + j <= i ? a.x : 0.f;
+                            x[j + 1] = 16 * jb + j + 1 <= i ? a.y : 0.f;
+                            x[j + 2] = 16 * jb + j + 2 <= i ? c.x : 0.f;
+                            x[j + 3] = 16 * jb + j + 3 <= i ? c.y : 0.f;
                         }
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
@@ -528,10 +538,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (flags & kFinal) break;
                 }
             }
-        } else if (warp == 22) {
-            // ---- loads and gates: lane l has tokens 2 l and 2 l + 1 of a chunk ----
+        } else if (warp == 22 || warp == 24) {
+            // ---- one warp starts the loads, another writes the gates and what the chunk belongs to ----
+            const bool loads = warp == 22;
             int m = 0, idx = blockIdx.x;
             bool ok = work;
+            if (!loads) it = find_item<kStateOnly>(p, finder, idx / p.HV);
             while (ok && it.n < p.N) {
                 const int h = idx % p.HV, hq = h / p.rep, len = it.t1 - it.t0, nch = len > C ? (len + C - 1) / C : 1;
                 const size_t mat = (size_t)kDim * kDim, wsi = (size_t)(it.ws + it.s) * p.HV + h;
@@ -546,37 +558,49 @@ __global__ void __launch_bounds__(kThreads, 1)
                     else if (p.state != nullptr)
                         src = p.state + ((size_t)it.n * p.HV + h) * mat;
                     if (it.s == it.nseg - 1) dst = p.new_state + ((size_t)it.n * p.HV + h) * mat;
-                    if (src != nullptr && lane == 0)
+                    if (loads && src != nullptr && lane == 0)
                         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
                 }
-                auto gates_of = [&](int c, float& g0, float& g1) {
+                idx += gridDim.x;
+                if (loads) {
+                    for (int c = 0; c < nch; ++c, ++m) {
+                        const int st = m % L::kStages;
+                        if (m >= L::kStages && !wait_bar(B, &B.empty[st], m / L::kStages - 1)) {
+                            ok = false;
+                            break;
+                        }
+                        const int t = it.t0 + c * C;
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(&B.full[st], L::kStage);
+                            const uint32_t d = sb + st * L::kStage;
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
+                                tma_box(d + L::oK + x * (kTile / 2), &mk, 64 * x, hq, t, &B.full[st]);
+                                tma_box(d + L::oV + x * (kTile / 2), &mv, 64 * x, h, t, &B.full[st]);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    it = find_item<kStateOnly>(p, finder, idx / p.HV);
+                    continue;
+                }
+                // lane l has tokens 2 l and 2 l + 1 of a chunk; a chunk's log decays are asked for one chunk ahead
+                const float* gl = p.log_decay + (p.per_token ? (size_t)(it.t0 + 2 * lane) * p.HV + h : h);
+                const size_t one = p.per_token ? p.HV : 0;
+                auto ask = [&](int c, float& g0, float& g1) {
                     const int a = c * C + 2 * lane;
                     g0 = g1 = 0.f;
-                    if (a < len) g0 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a) * p.HV + h : h]);
-                    if (a + 1 < len) g1 = clamp_log_decay(p.log_decay[p.per_token ? (size_t)(it.t0 + a + 1) * p.HV + h : h]);
+                    if (a < len) g0 = gl[c * C * one];
+                    if (a + 1 < len) g1 = gl[c * C * one + one];
                 };
-                float g0, g1;
-                gates_of(0, g0, g1);
-                idx += gridDim.x;
+                float n0, n1;
+                ask(0, n0, n1);
                 const Item next = find_item<kStateOnly>(p, finder, idx / p.HV);
                 for (int c = 0; c < nch; ++c, ++m) {
                     const int st = m % L::kStages;
-                    if (m >= L::kStages && !wait_bar(B, &B.empty[st], m / L::kStages - 1)) {
-                        ok = false;
-                        break;
-                    }
-                    const int t = it.t0 + c * C;
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&B.full[st], L::kStage);
-                        const uint32_t d = sb + st * L::kStage;
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
-                            tma_box(d + L::oK + x * (kTile / 2), &mk, 64 * x, hq, t, &B.full[st]);
-                            tma_box(d + L::oV + x * (kTile / 2), &mv, 64 * x, h, t, &B.full[st]);
-                        }
-                    }
+                    const float g0 = clamp_log_decay(n0), g1 = clamp_log_decay(n1);
+                    if (c + 1 < nch) ask(c + 1, n0, n1);
                     float pre = g0 + g1, suf = g0 + g1;  // inclusive sums up to and from this lane
 #pragma unroll
                     for (int d = 1; d < 32; d *= 2) {
@@ -587,102 +611,129 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float behind = __shfl_down_sync(0xffffffffu, suf, 1);
                     if (lane == 31) behind = 0.f;
                     const float c0 = lane == 0 ? g0 : pre - g1;
-                    Gate* gt = gate(m);
                     constexpr float kLog2e = 1.4426950408889634f;
+                    const float2 e = make_float2(p.scale * expf(c0), p.scale * expf(pre));
+                    const float2 w = make_float2(expf(behind + g1), expf(behind));
+                    const float all = expf(suf);
+                    if (m >= L::kStages && !wait_bar(B, &B.empty[st], m / L::kStages - 1)) {
+                        ok = false;
+                        break;
+                    }
+                    Gate* gt = gate(m);
                     *reinterpret_cast<float2*>(&gt->c2[2 * lane]) = make_float2(c0 * kLog2e, pre * kLog2e);
-                    *reinterpret_cast<float2*>(&gt->e[2 * lane]) = make_float2(p.scale * expf(c0), p.scale * expf(pre));
-                    *reinterpret_cast<float2*>(&gt->w[2 * lane]) = make_float2(expf(behind + g1), expf(behind));
+                    *reinterpret_cast<float2*>(&gt->e[2 * lane]) = e;
+                    *reinterpret_cast<float2*>(&gt->w[2 * lane]) = w;
                     if (lane == 0) {
-                        gt->a = expf(suf);
+                        gt->a = all;
                         gt->flags = (c == 0 ? kFirst : 0) | (c == nch - 1 ? kLast : 0) |
                                     (c == nch - 1 && next.n >= p.N ? kFinal : 0);
-                        gt->t = t, gt->live = min(C, len - c * C);
+                        gt->t = it.t0 + c * C, gt->live = min(C, len - c * C);
                         gt->src = src, gt->dst = dst, gt->decay = decay, gt->h = h;
                     }
                     __syncwarp();
                     if (lane == 0) arrive(&B.full[st]);
-                    if (c + 1 < nch) gates_of(c + 1, g0, g1);
                 }
                 it = next;
             }
-            if (!ok && lane == 0)  // given up: copies in flight land before the CTA ends
+            if (loads && !ok && lane == 0)  // given up: copies in flight land before the CTA ends
                 for (int k = m > L::kStages ? m - L::kStages : 0; k < m; ++k) {
+                    // (their gates may be missing: only the bytes are waited for, as long as they can take)
                     const long long t0 = clock64();
-                    while (!mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && clock64() - t0 < kWaitBudget) {}
+                    while (!mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && clock64() - t0 < (1ll << 24)) {}
                 }
-        } else {
-            if (lane == 0 && work) {
-                // ---- products, issued by one thread ----
-                constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
-                                   id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
-                const uint64_t dkw = desc_mnmaj(sb + L::kw, C, 0);
-                auto scores = [&](int m) {
-                    const uint32_t d = sb + (m % L::kStages) * L::kStage;
-                    const uint64_t dq = desc_kmaj(d, C, 0), dk = desc_kmaj(d + L::oK, C, 0);
+        } else if (warp == 23) {
+            // ---- products, issued by one elected thread ----
+            constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
+                               id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
+            const uint32_t tu = __shfl_sync(0xffffffffu, tm, 0), su = __shfl_sync(0xffffffffu, sb, 0);
+            const uint64_t dkw = desc_mnmaj(su + L::kw, C, 0), dps = desc_kmaj(su + L::ps, C, 0);
+            const uint64_t dq0 = desc_kmaj(su, C, 0), dk0 = desc_kmaj(su + L::oK, C, 0), dv0 = desc_mnmaj(su + L::oV, C, 0);
+            const uint64_t dk0w = desc_mnmaj(su + L::oK, C, 0);  // k as U's operand
+            auto scores = [&](int m) {
+                if (elect_one()) {
+                    const uint64_t dq = desc_add(dq0, (m % L::kStages) * L::kStage), dk = desc_add(dk0, (m % L::kStages) * L::kStage);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        mma_f16(tm + kColP + 64 * (m & 1), desc_add(dq, koff_kmaj(C, 16 * ks)),
-                                desc_add(dk, koff_kmaj(C, 16 * ks)), id_qk, ks > 0);
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_f16(tu + kColP + 64 * (m & 1), desc_add(dq, x * (kTile / 2) + 32 * ks),
+                                    desc_add(dk, x * (kTile / 2) + 32 * ks), id_qk, (x | ks) > 0);
                     mma_commit(&B.qk_full[m & 1]);
-                };
-                bool ok = true;
-                if (!kStateOnly) {
-                    ok = wait_one(B, &B.full[0], 0);
-                    fence_after_sync();
-                    if (ok) scores(0);
                 }
-                for (int m = 0; ok; ++m) {
-                    const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
-                    const uint32_t d = sb + st * L::kStage;
-                    const uint64_t dv = desc_mnmaj(d + L::oV, C, 0);
-                    if (!wait_one(B, &B.kw_ready, m)) break;
-                    const bool final = gate(m)->flags & kFinal;
-                    if (m >= L::kU && !wait_one(B, &B.u_free[ub], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
-                    fence_after_sync();
+                __syncwarp();
+            };
+            bool ok = work;
+            if (!kStateOnly && ok) {
+                ok = wait_bar(B, &B.full[0], 0);
+                fence_after_sync();
+                if (ok) scores(0);
+            }
+            for (int m = 0; ok; ++m) {
+                const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
+                const uint64_t dv = desc_add(dv0, st * L::kStage), dk = desc_add(dk0w, st * L::kStage);
+                bool final;
+                if (!kStateOnly) {
+                    final = gate(m)->flags & kFinal;
+                    if (!final) {
+                        if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
+                        fence_after_sync();
+                        scores(m + 1);
+                    }
+                }
+                if (!wait_bar(B, &B.kw_ready[ub], kStateOnly ? m >> 1 : m)) break;
+                if (kStateOnly) final = gate(m)->flags & kFinal;
+                if (m >= L::kBuf && !wait_bar(B, &B.u_free[ub], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
+                fence_after_sync();
+                if (elect_one()) {
 #pragma unroll
                     for (int term = 2; term >= 0; --term)  // small terms first
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tm + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
-                                    desc_add(dkw, term * kTile + koff_mnmaj(16 * ks)), id_u, term < 2 || ks > 0);
+                            mma_f16(tu + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
+                                    desc_add(term ? desc_add(dkw, (ub * 2 + term - 1) * kTile) : dk, koff_mnmaj(16 * ks)), id_u,
+                                    term < 2 || ks > 0);
                     mma_commit(&B.u_full[ub]);
-                    if (kStateOnly) {
-                        mma_commit(&B.empty[st]);
-                        if (final) break;
-                        continue;
-                    }
-                    if (!final) {
-                        if (!wait_one(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
-                        fence_after_sync();
-                        scores(m + 1);
-                    }
-                    if (!wait_one(B, &B.s_ready, m)) break;
-                    if (m > 0 && !wait_one(B, &B.o_free, m - 1)) break;
-                    fence_after_sync();
-                    const uint64_t dq = desc_kmaj(d, C, 0);
+                    if (kStateOnly) mma_commit(&B.empty[st]);
+                }
+                __syncwarp();
+                if (kStateOnly) {
+                    if (final) break;
+                    continue;
+                }
+                if (!wait_bar(B, &B.s_ready, m)) break;
+                if (m > 0 && !wait_bar(B, &B.o_free, m - 1)) break;
+                fence_after_sync();
+                if (elect_one()) {
+                    const uint64_t dq = desc_add(dq0, st * L::kStage);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        mma_f16_ts(tm + kColO2, tm + kColSHi + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, ks > 0);
-                        mma_f16_ts(tm + kColO2, tm + kColSLo + 8 * ks, desc_add(dq, koff_kmaj(C, 16 * ks)), id_qs, true);
-                    }
-                    if (!wait_one(B, &B.p_ready[m & 1], m >> 1)) break;
-                    fence_after_sync();
-                    const uint64_t dp = desc_kmaj(sb + L::ps + (m & 1) * 2 * L::kP, C, 0);
+                    for (int x = 0; x < 4; ++x)  // terms and halves of K: columns kColSHi + 64 * term + 32 * half
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_f16_ts(tu + kColO2, tu + kColSHi + 32 * x + 8 * ks,
+                                       desc_add(dq, (x & 1) * (kTile / 2) + 32 * ks), id_qs, (x | ks) > 0);
+                    mma_commit(&B.s_free);
+                }
+                __syncwarp();
+                if (!wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;
+                fence_after_sync();
+                if (elect_one()) {
+                    const uint64_t dp = desc_add(dps, (m & 1) * 2 * L::kP);
 #pragma unroll
                     for (int term = 1; term >= 0; --term)
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tm + kColO1, desc_add(dv, koff_mnmaj(16 * ks)),
+                            mma_f16(tu + kColO1, desc_add(dv, koff_mnmaj(16 * ks)),
                                     desc_add(dp, term * L::kP + koff_kmaj(C, 16 * ks)), id_pv, term < 1 || ks > 0);
                     mma_commit(&B.o_full);
                     mma_commit(&B.empty[st]);
-                    if (final) break;
                 }
-                if (B.abort) {  // products in flight end before the tensor memory is given back
-                    mma_commit(&B.drain);
-                    const long long t0 = clock64();
-                    while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitBudget) {}
-                }
+                __syncwarp();
+                if (final) break;
+            }
+            if (B.abort && elect_one()) {  // products in flight end before the tensor memory is given back
+                mma_commit(&B.drain);
+                const long long t0 = clock64();
+                while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitBudget) {}
             }
             __syncwarp();
         }
