@@ -17,13 +17,17 @@
 // operand in the layout in which it arrives (token-major tiles from TMA):
 //   U   [v, k] = V^T (wK)       A: V tile (MN-major), B: scaled K (MN-major)
 //   P   [i, j] = Q K^T          rows 64..127 of the M = 128 tile are not used
-//   O2^T[v, i] = S Q^T          A: S as bf16 in tensor memory, B: Q tile
-//   O1^T[v, i] = V^T P^T        A: V tile (MN-major), B: decayed P
+//   O2^T[v, i] = S Q^T          A: S (bf16) in tensor memory, B: Q tile
+//   O1^T[v, i] = V^T P^T        A: V tile (MN-major), B: decayed P (bf16)
 //
-// Precision: inputs are bf16; every other factor is split into bf16 terms so
-// that nothing is lost beside the fp32 accumulation: wK into three (off by
-// 2^-25 or so: the state is an fp32 result), S and P into two (2^-17: the output
-// is rounded to bf16, 2^-9).
+// Precision: inputs are bf16.  wK is split into three bf16 terms of 8 bits each
+// (exact), so the fp32 state loses nothing beside its accumulation: 8e-8 of it
+// measured, where two terms would give 3e-6.  S and P only meet the output, which
+// is rounded to bf16 itself; they are rounded to bf16 once each, one for each of
+// the output's two parts, so the output's error is sqrt(2) times that of the last
+// rounding alone (measured 0.0023 against 0.0017 of the output; second terms
+// bring it to 0.0017 and cost 12 more products and 1,000 more instructions a
+// chunk).
 #include <cuda.h>
 
 #include <atomic>
@@ -86,6 +90,7 @@ template <bool kInner>
 __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int slot) {
     const int lane = threadIdx.x & 31;
     Item it{p.N, 0, 0, 0, 0, 0};
+#pragma unroll 1
     for (; f.base < p.N; f.base += 32) {
         int t0 = 0, len = 0, nseg = 0;
         if (f.base + lane < p.N) nseg = n_segments(p, f.base + lane, t0, len);
@@ -126,13 +131,14 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 //   warp  22          TMA loads
 //   warp  23          one thread that issues the products
 //   warp  24          gates, and what the chunk belongs to
+//   warp  26          finished states on their way out
 // (a warp reads the 32 tensor-memory lanes of its number modulo 4, hence 25).
 // ---------------------------------------------------------------------------
 
 constexpr int kThreads = 28 * 32;
-// Registers per thread by warpgroup; 256 * (112 + 48) + 128 * (64 + 56 + 56) is
-// below the 896 * 72 the CTA is launched with.
-constexpr int kRegsState = 112, kRegsScale = 48, kRegsOut = 64, kRegsRest = 56;
+// Registers per thread by warpgroup; 256 * (112 + 48) + 128 * (72 + 56 + 56) is
+// the 896 * 72 the CTA is launched with.
+constexpr int kRegsState = 112, kRegsScale = 48, kRegsOut = 72, kRegsRest = 56;
 static_assert(256 * (kRegsState + kRegsScale) + 128 * (kRegsOut + 2 * kRegsRest) <= kThreads * 72, "register split");
 
 template <bool kStateOnly>
@@ -143,12 +149,13 @@ struct Lay {
     static constexpr uint32_t kStage = (kStateOnly ? 2 : 3) * kTile;
     static constexpr uint32_t oK = kStateOnly ? 0 : kTile, oV = oK + kTile;  // inside a stage; q at 0
     static constexpr uint32_t kw = kStages * kStage;  // the scaled k's two lower terms (the first takes k's own place)
-    static constexpr uint32_t ps = kw + kBuf * 2 * kTile;  // two buffers of P's two terms
+    static constexpr uint32_t ps = kw + kBuf * 2 * kTile;  // two buffers of P
     static constexpr uint32_t kP = C * C * 2;
-    static constexpr uint32_t turn = ps + (kStateOnly ? 0 : 4 * kP);  // 1 KiB for each state warp
+    static constexpr uint32_t spare = ps + (kStateOnly ? 0 : 2 * kP);  // the last columns of a state on its way out
+    static constexpr uint32_t turn = spare + (kStateOnly ? 0 : 16384);  // 1 KiB for each state warp
     static constexpr uint32_t gates = turn + 8 * 1024;
     static constexpr uint32_t bars = gates + kGates * 832;
-    static constexpr uint32_t total = bars + 256;
+    static constexpr uint32_t total = bars + 320;
 };
 static_assert(Lay<false>::total <= 227 * 1024 && Lay<true>::total <= 227 * 1024, "shared memory");
 
@@ -162,35 +169,34 @@ struct Gate {
     float a;      // e^{c_63}
     int flags;    // first / last chunk of its segment, last chunk of this CTA
     int t, live;  // first token; tokens of the segment from there on, at most 64
-    const float* src;  // first chunk: the state before it (null: zero)
-    float* dst;        // last chunk: where the state after it goes (null: nowhere)
-    float* decay;      // last chunk, kStateOnly: where the segment's decay goes
     int h;
+    const float* src;  // first chunk: the state before it (null: zero)
+    int out;       // last chunk: the state's number in new_state (-1: it goes nowhere), kStateOnly: in the workspace
 };
 static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
-    uint64_t full[3], empty[3], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready[2], s_ready, s_free, o_full, o_free, drain;
+    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready[2], s_ready,
+        s_free, o_full[2], o_free[2], st_full, st_free, drain;
     uint32_t tmem;
     volatile int abort;
     int none;
+    int st_out, st_m, st_final;  // for the store warp: the state's number, its last chunk, no more to come
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+static_assert(sizeof(Bars) <= 320, "barrier block");
 
-constexpr long long kWaitBudget = 1ll << 30;  // cycles, about half a second
-
-// Bounded wait: false once it, or any other wait of this CTA, has run out.
+// Bounded wait: false once it, or any other wait of this CTA, has run out (2^30
+// cycles, about half a second).  Kept short and rolled: the warps run some 25
+// waits, and the kernel's instructions should fit the instruction cache.
 __device__ __forceinline__ bool wait_one(Bars& B, uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity & 1u)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity & 1u)) {
-        if (B.abort) return false;
-        if (clock64() - t0 > kWaitBudget) {
+    const int t0 = (int)clock();
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity & 1u))
+        if (B.abort || (int)clock() - t0 > 1 << 30) {
             B.abort = 1;
-            atomicOr(&g_device_status, kDevStatTimeout);
             return false;
         }
-    }
     return true;
 }
 // The same for a whole warp, which goes on together.
@@ -208,6 +214,15 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
             dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(t), "r"(smem_u32(bar))
         : "memory");
+}
+
+// 32 columns of all 128 rows of one state ([states, 128, 128] fp32), 128-byte swizzle.
+constexpr uint32_t kBox = 128 * 32 * 4;
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int number) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(0),
+                 "r"(number), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 // True in one lane of a converged warp, always the same.
@@ -229,9 +244,12 @@ __device__ __forceinline__ uint32_t upper2(float2 x) {
 }
 // What is left of two floats behind those bits (exact).
 __device__ __forceinline__ float2 below2(float2 x) {
-    const float a = __uint_as_float(__float_as_uint(x.x) & 0xffff0000u), b = __uint_as_float(__float_as_uint(x.y) & 0xffff0000u);
-    return __fadd2_rn(x, make_float2(-a, -b));
+    const float a = __uint_as_float((__float_as_uint(x.x) & 0xffff0000u) ^ 0x80000000u);
+    const float b = __uint_as_float((__float_as_uint(x.y) & 0xffff0000u) ^ 0x80000000u);
+    return __fadd2_rn(x, make_float2(a, b));
 }
+
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 template <int kN>
 __device__ __forceinline__ void more_registers() {
@@ -243,12 +261,13 @@ __device__ __forceinline__ void fewer_registers() {
 }
 
 // Tensor-memory columns
-constexpr uint32_t kColU = 0, kColSHi = 128, kColSLo = 192, kColP = 256, kColO1 = 384, kColO2 = 448;
+constexpr uint32_t kColU = 0, kColS = 128, kColP = 192, kColO1 = 256, kColO2 = 320;  // (O: a second buffer 128 on)
 
 template <bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     decay_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mq,
-                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
+                         const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                         const __grid_constant__ CUtensorMap m_new) {
     using L = Lay<kStateOnly>;
     extern __shared__ __align__(1024) uint8_t sm[];
     Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
@@ -264,14 +283,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 1);
 #pragma unroll
+            for (int i = 0; i < 5; ++i) mbar_init(&B.pv_done[i], 1);
+#pragma unroll
             for (int i = 0; i < 2; ++i) {
-                mbar_init(&B.qk_full[i], 1), mbar_init(&B.p_ready[i], 96), mbar_init(&B.kw_ready[i], 256);
+                mbar_init(&B.qk_full[i], 1), mbar_init(&B.o_full[i], 1), mbar_init(&B.o_free[i], 128);
+                mbar_init(&B.p_ready[i], 96), mbar_init(&B.kw_ready[i], 256);
                 mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
             }
             mbar_init(&B.s_ready, 256);
             mbar_init(&B.s_free, 1);
-            mbar_init(&B.o_full, 1);
-            mbar_init(&B.o_free, 128);
+            mbar_init(&B.st_full, 256);
+            mbar_init(&B.st_free, 1);
             mbar_init(&B.drain, 1);
             fence_mbar_init();
         }
@@ -283,16 +305,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(&B.tmem, kStateOnly ? 256 : 512);
         tmem_relinquish();
     }
-    if (!kStateOnly && tid < 256) {  // the upper right quarter of P (rows 0..31, columns 32..63) stays zero
-        const int buf = tid >> 6, row = (tid & 63) >> 1;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int chunk = 4 + 2 * (tid & 1) + i;
-            *reinterpret_cast<uint4*>(sm + L::ps + buf * L::kP + row * 128 + ((chunk ^ (row & 7)) << 4)) =
-                make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-    }
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
@@ -302,22 +314,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp < 8) {
         // ---- state: row v of 128, half the columns, in registers ----
         more_registers<kRegsState>();
-        const int half = warp >> 2, v0 = 32 * (warp & 3);
+        const int half = warp >> 2, v0 = 32 * (warp & 3), v = v0 + lane;
         const uint32_t tl = tm + ((uint32_t)v0 << 16);
-        // rows v0 .. v0 + 31 are turned in shared memory by 8 columns at a time, so that two
-        // lanes read or write 32 bytes of one row in global memory
-        uint8_t* turn = sm + L::turn + 1024 * warp;
-        const size_t off = (size_t)(v0 + (lane >> 1)) * kDim + 64 * half + 4 * (lane & 1);
-        uint8_t* by_row = turn + lane * 32;  // 16-byte place x of row r holds column group x ^ (r >> 2 & 1)
-        uint8_t* by_pair = turn + (lane >> 1) * 32 + (((lane ^ lane >> 3) & 1) << 4);  // row lane / 2; + 512: 16 rows on
+        // rows v0 .. v0 + 31 are turned in shared memory by 8 columns at a time, so that two lanes
+        // read or write 32 bytes of one row; 16-byte place x of row r holds columns of x ^ (r >> 2 & 1)
+        uint8_t* by_row = sm + L::turn + 1024 * warp + lane * 32;
+        uint8_t* by_pair = sm + L::turn + 1024 * warp + (lane >> 1) * 32 + (((lane ^ lane >> 3) & 1) << 4);
         const int sw = (lane >> 2 & 1) << 4;
+        const int off = (v0 + (lane >> 1)) * kDim + 64 * half + 4 * (lane & 1);
         float s[64];
         float prod = 1.f;
+        bool first = true;
+        int stored = 0;
+#pragma unroll 1
         for (int m = 0; work; ++m) {
             const Gate* gt = gate(m);
             if (!kStateOnly) {
-                if (!wait_bar(B, &B.full[m % L::kStages], m / L::kStages)) break;
-                if (gt->flags & kFirst) {
+                if (first) {
+                    if (!wait_bar(B, &B.full[m % L::kStages], m / L::kStages)) break;
                     const float* src = gt->src;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -342,16 +356,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (m > 0 && !wait_bar(B, &B.s_free, m - 1)) break;
                 fence_after_sync();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t hi[8], lo[8];
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t x[16];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 x = make_float2(s[16 * i + 2 * j], s[16 * i + 2 * j + 1]), y = below2(x);
-                        hi[j] = upper2(x);
-                        lo[j] = pack_bf16(y.x, y.y);
-                    }
-                    tmem_st8_u32_nowait(tl + kColSHi + 32 * half + 8 * i, hi);
-                    tmem_st8_u32_nowait(tl + kColSLo + 32 * half + 8 * i, lo);
+                    for (int j = 0; j < 16; ++j) x[j] = pack_bf16(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]);
+                    tmem_st16_u32_nowait(tl + kColS + 32 * half + 16 * i, x);
                 }
                 tmem_wait_st();
                 fence_before_sync();
@@ -361,10 +370,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait_bar(B, &B.u_full[ub], kStateOnly ? m >> 1 : m)) break;
             fence_after_sync();
             const float a = gt->a;
-            const int flags = gt->flags;
-            float* dst = gt->dst;
-            float* decay = gt->decay;
-            if (kStateOnly && (flags & kFirst)) {
+            const int flags = gt->flags, out = gt->out;
+            if (kStateOnly && first) {
                 prod = 1.f;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) s[i] = 0.f;
@@ -372,17 +379,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             prod *= a;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float u[16];
-                tmem_ld16(tl + kColU + 128 * ub + 64 * half + 16 * i, u);
+                float x[16];
+                tmem_ld16(tl + kColU + 128 * ub + 64 * half + 16 * i, x);
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) {
-                    const float2 x = __ffma2_rn(make_float2(a, a), make_float2(s[16 * i + j], s[16 * i + j + 1]), make_float2(u[j], u[j + 1]));
-                    s[16 * i + j] = x.x, s[16 * i + j + 1] = x.y;
+                    const float2 y = __ffma2_rn(make_float2(a, a), make_float2(s[16 * i + j], s[16 * i + j + 1]), make_float2(x[j], x[j + 1]));
+                    s[16 * i + j] = y.x, s[16 * i + j + 1] = y.y;
                 }
             }
             fence_before_sync();
             arrive(&B.u_free[ub]);
-            if ((flags & kLast) && dst != nullptr) {
+            first = flags & kLast;
+            if (kStateOnly && first) {
+                float* dst = p.ws_state + (size_t)out * kDim * kDim + off;
 #pragma unroll
                 for (int b = 0; b < 8; ++b) {
                     const float* y = s + 8 * b;
@@ -390,10 +399,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                     *reinterpret_cast<float4*>(by_row + sw) = make_float4(y[0], y[1], y[2], y[3]);
                     *reinterpret_cast<float4*>(by_row + (sw ^ 16)) = make_float4(y[4], y[5], y[6], y[7]);
                     __syncwarp();
-                    *reinterpret_cast<float4*>(dst + off + 8 * b) = *reinterpret_cast<const float4*>(by_pair);
-                    *reinterpret_cast<float4*>(dst + off + 16 * kDim + 8 * b) = *reinterpret_cast<const float4*>(by_pair + 512);
+                    *reinterpret_cast<float4*>(dst + 8 * b) = *reinterpret_cast<const float4*>(by_pair);
+                    *reinterpret_cast<float4*>(dst + 16 * kDim + 8 * b) = *reinterpret_cast<const float4*>(by_pair + 512);
                 }
-                if (kStateOnly && tid == 0) *decay = prod;
+                if (tid == 0) p.ws_decay[out] = prod;
+            }
+            if (!kStateOnly && first) {
+                // the state leaves by way of its last chunk's stage (48 KiB, free after that chunk's last products)
+                // and 16 KiB beside it; the store warp sends it on and gives the stage back
+                if (!wait_bar(B, &B.pv_done[m % 5], m / 5)) break;
+                if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
+                ++stored;
+                if (out >= 0) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint8_t* row = sm + (half && x ? L::spare : (m % L::kStages) * L::kStage + (2 * half + x) * kBox) + v * 128;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<float4*>(row + ((i ^ (v & 7)) << 4)) =
+                                make_float4(s[32 * x + 4 * i], s[32 * x + 4 * i + 1], s[32 * x + 4 * i + 2], s[32 * x + 4 * i + 3]);
+                    }
+                    fence_proxy_async_smem();
+                }
+                if (tid == 0) B.st_out = out, B.st_m = m, B.st_final = flags & kFinal;
+                arrive(&B.st_full);
             }
             if (flags & kFinal) break;
         }
@@ -401,12 +430,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- w_j k_j in three terms of 8 bits each (exact), at the same place of three tiles ----
         fewer_registers<kRegsScale>();
         const int x = tid - 256;
+#pragma unroll 1
         for (int m = 0; work; ++m) {
             const int st = m % L::kStages;
             if (!wait_bar(B, &B.full[st], m / L::kStages)) break;
             const Gate* gt = gate(m);
             const int live = gt->live, flags = gt->flags;
             if (live < C)  // what follows the segment must not meet a zero weight as 0 * NaN
+#pragma unroll 1
                 for (int i = x; i < 2 * C * 8; i += 256)
                     if ((i >> 3 & (C - 1)) >= live)
                         *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
@@ -447,15 +478,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             const size_t step = (size_t)p.HV * kDim;
             {  // tokens of no sequence: zeros
                 const int c0 = cu_at(p.cu, p.cu64, 0, p.T), c1 = max(c0, cu_at(p.cu, p.cu64, p.N, p.T));
-                const long long rows = (long long)(c0 + p.T - c1) * p.HV;
-                for (long long i = (long long)blockIdx.x * 8 + ((tid - 512) >> 4); i < rows; i += (long long)gridDim.x * 8) {
-                    const long long r = i / p.HV;
-                    *reinterpret_cast<uint4*>(p.out + ((r < c0 ? r : r - c0 + c1) * p.HV + i % p.HV) * kDim + 8 * (tid & 15)) =
-                        make_uint4(0, 0, 0, 0);
-                }
+                const int rows = c0 + p.T - c1;  // a row is HV * 16 pieces of 16 bytes
+#pragma unroll 1
+                for (int r = blockIdx.x; r < rows; r += gridDim.x)
+#pragma unroll 1
+                    for (int i = tid - 512; i < p.HV * 16; i += 128)
+                        *reinterpret_cast<uint4*>(p.out + (size_t)(r < c0 ? r : r - c0 + c1) * step + 8 * i) = make_uint4(0, 0, 0, 0);
             }
+#pragma unroll 1
             for (int m = 0; work; ++m) {
-                if (!wait_bar(B, &B.o_full, m)) break;
+                if (!wait_bar(B, &B.o_full[m & 1], m >> 1)) break;
                 fence_after_sync();
                 const Gate* gt = gate(m);
                 const int live = gt->live, flags = gt->flags;
@@ -463,25 +495,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                 for (int b = 0; b < 4; ++b) {
                     float x1[16], x2[16];
-                    tmem_ld16x2(tl + kColO1 + 16 * b, tl + kColO2 + 16 * b, x1, x2);
+                    tmem_ld16x2(tl + kColO1 + 128 * (m & 1) + 16 * b, tl + kColO2 + 128 * (m & 1) + 16 * b, x1, x2);
+                    uint32_t y[8];
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
                         const float4 e = *reinterpret_cast<const float4*>(&gt->e[16 * b + j]);
                         const float2 a = __ffma2_rn(make_float2(e.x, e.y), make_float2(x2[j], x2[j + 1]), make_float2(x1[j], x1[j + 1]));
                         const float2 c = __ffma2_rn(make_float2(e.z, e.w), make_float2(x2[j + 2], x2[j + 3]), make_float2(x1[j + 2], x1[j + 3]));
-                        x1[j] = a.x, x1[j + 1] = a.y, x1[j + 2] = c.x, x1[j + 3] = c.y;
+                        y[j / 2] = pack_bf16(a.x, a.y);
+                        y[j / 2 + 1] = pack_bf16(c.x, c.y);
                     }
                     if (b == 3) {
                         fence_before_sync();
-                        arrive(&B.o_free);
+                        arrive(&B.o_free[m & 1]);
                     }
-                    if (live == C) {
+                    unsigned short* to = reinterpret_cast<unsigned short*>(dst);
+                    if (live >= 16 * b + 16) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) dst[j * step] = __float2bfloat16_rn(x1[j]);
+                        for (int j = 0; j < 8; ++j) {
+                            to[0] = (unsigned short)y[j];
+                            to[step] = (unsigned short)(y[j] >> 16);
+                            to += 2 * step;
+                        }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (16 * b + j < live) dst[j * step] = __float2bfloat16_rn(x1[j]);
+                        for (int j = 0; j < 8; ++j) {
+                            if (16 * b + 2 * j < live) to[0] = (unsigned short)y[j];
+                            if (16 * b + 2 * j + 1 < live) to[step] = (unsigned short)(y[j] >> 16);
+                            to += 2 * step;
+                        }
                     }
                     dst += 16 * step;
                 }
@@ -495,19 +537,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // ---- decayed scores ----
                 const int wq = warp & 1, i = 32 * wq + lane, jb0 = warp == 25 ? 2 : 0;
                 const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
+#pragma unroll 1
                 for (int m = 0; work; ++m) {
                     if (!wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
                     fence_after_sync();
                     const Gate* gt = gate(m);
                     const int flags = gt->flags;
                     const float ci = gt->c2[i];
-                    uint8_t* row = sm + L::ps + (m & 1) * 2 * L::kP + i * 128;
-                    // this buffer's last product is that of chunk m - 2
-                    if (m > 1 && !wait_bar(B, &B.empty[(m - 2) % L::kStages], (m - 2) / L::kStages)) break;
+                    uint8_t* row = sm + L::ps + (m & 1) * L::kP + i * 128;
+                    // this buffer's last products are those of chunk m - 2
+                    if (m > 1 && !wait_bar(B, &B.pv_done[(m - 2) % 5], (m - 2) / 5)) break;
+                    if (warp == 20)  // rows 0 .. 31: nothing in columns 32 .. 63
+#pragma unroll
+                        for (int q = 4; q < 8; ++q) *reinterpret_cast<uint4*>(row + ((q ^ (i & 7)) << 4)) = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
                     for (int jb = jb0; jb < jb0 + 2; ++jb) {  // 16 columns at a time
                         float x[16];
-                        tmem_ld16(tl + kColP + 64 * (m & 1) + 16 * jb, x);
+                        tmem_ld16(tl + kColP + 16 * jb, x);
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
                             const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[16 * jb + j]);
@@ -520,16 +566,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 a = make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]), r = below2(a);
-                                hi[e] = upper2(a);
-                                lo[e] = pack_bf16(r.x, r.y);
-                            }
-                            const uint32_t o = ((2 * jb + q) ^ (i & 7)) << 4;
-                            *reinterpret_cast<uint4*>(row + o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4*>(row + L::kP + o) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            const float* y = x + 8 * q;
+                            *reinterpret_cast<uint4*>(row + (((2 * jb + q) ^ (i & 7)) << 4)) = make_uint4(
+                                pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
                         }
                     }
                     fence_before_sync();
@@ -546,33 +585,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!loads) it = find_item<kStateOnly>(p, finder, idx / p.HV);
             while (ok && it.n < p.N) {
                 const int h = idx % p.HV, hq = h / p.rep, len = it.t1 - it.t0, nch = len > C ? (len + C - 1) / C : 1;
-                const size_t mat = (size_t)kDim * kDim, wsi = (size_t)(it.ws + it.s) * p.HV + h;
+                const int wsi = (it.ws + it.s) * p.HV + h, number = it.n * p.HV + h;
                 const float* src = nullptr;
-                float *dst = nullptr, *decay = nullptr;
-                if (kStateOnly) {
-                    dst = p.ws_state + (wsi + p.HV) * mat;
-                    decay = p.ws_decay + wsi + p.HV;
-                } else {
+                if (!kStateOnly) {
                     if (it.s > 0 || (it.nseg > 1 && p.first_from_ws))
-                        src = p.ws_state + wsi * mat;
+                        src = p.ws_state + (size_t)wsi * kDim * kDim;
                     else if (p.state != nullptr)
-                        src = p.state + ((size_t)it.n * p.HV + h) * mat;
-                    if (it.s == it.nseg - 1) dst = p.new_state + ((size_t)it.n * p.HV + h) * mat;
-                    if (loads && src != nullptr && lane == 0)
-                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
+                        src = p.state + (size_t)number * kDim * kDim;
                 }
                 idx += gridDim.x;
                 if (loads) {
+                    if (src != nullptr && lane == 0)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
+#pragma unroll 1
                     for (int c = 0; c < nch; ++c, ++m) {
                         const int st = m % L::kStages;
                         if (m >= L::kStages && !wait_bar(B, &B.empty[st], m / L::kStages - 1)) {
                             ok = false;
                             break;
                         }
-                        const int t = it.t0 + c * C;
                         if (lane == 0) {
-                            mbar_arrive_expect_tx(&B.full[st], L::kStage);
                             const uint32_t d = sb + st * L::kStage;
+                            const int t = it.t0 + c * C;
+                            mbar_arrive_expect_tx(&B.full[st], L::kStage);
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
                                 if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
@@ -597,8 +632,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float n0, n1;
                 ask(0, n0, n1);
                 const Item next = find_item<kStateOnly>(p, finder, idx / p.HV);
+#pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++m) {
-                    const int st = m % L::kStages;
                     const float g0 = clamp_log_decay(n0), g1 = clamp_log_decay(n1);
                     if (c + 1 < nch) ask(c + 1, n0, n1);
                     float pre = g0 + g1, suf = g0 + g1;  // inclusive sums up to and from this lane
@@ -615,7 +650,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float2 e = make_float2(p.scale * expf(c0), p.scale * expf(pre));
                     const float2 w = make_float2(expf(behind + g1), expf(behind));
                     const float all = expf(suf);
-                    if (m >= L::kStages && !wait_bar(B, &B.empty[st], m / L::kStages - 1)) {
+                    // the stage is free, so the products of chunk m - 3 are done, and before them the last reader of
+                    // gate slot m - 5 was
+                    if (m >= L::kStages && !wait_bar(B, &B.empty[m % L::kStages], m / L::kStages - 1)) {
                         ok = false;
                         break;
                     }
@@ -628,19 +665,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         gt->flags = (c == 0 ? kFirst : 0) | (c == nch - 1 ? kLast : 0) |
                                     (c == nch - 1 && next.n >= p.N ? kFinal : 0);
                         gt->t = it.t0 + c * C, gt->live = min(C, len - c * C);
-                        gt->src = src, gt->dst = dst, gt->decay = decay, gt->h = h;
+                        gt->h = h, gt->src = src, gt->out = kStateOnly ? wsi + p.HV : it.s == it.nseg - 1 ? number : -1;
                     }
                     __syncwarp();
-                    if (lane == 0) arrive(&B.full[st]);
+                    if (lane == 0) arrive(&B.full[m % L::kStages]);
                 }
                 it = next;
             }
             if (loads && !ok && lane == 0)  // given up: copies in flight land before the CTA ends
-                for (int k = m > L::kStages ? m - L::kStages : 0; k < m; ++k) {
-                    // (their gates may be missing: only the bytes are waited for, as long as they can take)
-                    const long long t0 = clock64();
-                    while (!mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && clock64() - t0 < (1ll << 24)) {}
-                }
+                // (their gates may be missing: only the bytes are waited for, as long as they can take)
+#pragma unroll 1
+                for (int k = m > L::kStages ? m - L::kStages : 0; k < m; ++k)
+                    for (const int t0 = (int)clock(); !mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && (int)clock() - t0 < 1 << 24;) {}
         } else if (warp == 23) {
             // ---- products, issued by one elected thread ----
             constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
@@ -649,14 +685,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t dkw = desc_mnmaj(su + L::kw, C, 0), dps = desc_kmaj(su + L::ps, C, 0);
             const uint64_t dq0 = desc_kmaj(su, C, 0), dk0 = desc_kmaj(su + L::oK, C, 0), dv0 = desc_mnmaj(su + L::oV, C, 0);
             const uint64_t dk0w = desc_mnmaj(su + L::oK, C, 0);  // k as U's operand
-            auto scores = [&](int m) {
+            auto scores = [&](int m, int st) {
                 if (elect_one()) {
-                    const uint64_t dq = desc_add(dq0, (m % L::kStages) * L::kStage), dk = desc_add(dk0, (m % L::kStages) * L::kStage);
+                    const uint64_t dq = desc_add(dq0, st * L::kStage), dk = desc_add(dk0, st * L::kStage);
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tu + kColP + 64 * (m & 1), desc_add(dq, x * (kTile / 2) + 32 * ks),
+                            mma_f16(tu + kColP, desc_add(dq, x * (kTile / 2) + 32 * ks),
                                     desc_add(dk, x * (kTile / 2) + 32 * ks), id_qk, (x | ks) > 0);
                     mma_commit(&B.qk_full[m & 1]);
                 }
@@ -666,18 +702,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!kStateOnly && ok) {
                 ok = wait_bar(B, &B.full[0], 0);
                 fence_after_sync();
-                if (ok) scores(0);
+                if (ok) scores(0, 0);
             }
+#pragma unroll 1
             for (int m = 0; ok; ++m) {
                 const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
                 const uint64_t dv = desc_add(dv0, st * L::kStage), dk = desc_add(dk0w, st * L::kStage);
-                bool final;
+                bool final, last = false;
                 if (!kStateOnly) {
-                    final = gate(m)->flags & kFinal;
+                    final = gate(m)->flags & kFinal, last = gate(m)->flags & kLast;
                     if (!final) {
                         if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
+                        if (!wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;  // and read: P's columns are free
                         fence_after_sync();
-                        scores(m + 1);
+                        scores(m + 1, (m + 1) % L::kStages);
                     }
                 }
                 if (!wait_bar(B, &B.kw_ready[ub], kStateOnly ? m >> 1 : m)) break;
@@ -701,47 +739,60 @@ __global__ void __launch_bounds__(kThreads, 1)
                     continue;
                 }
                 if (!wait_bar(B, &B.s_ready, m)) break;
-                if (m > 0 && !wait_bar(B, &B.o_free, m - 1)) break;
+                if (m > 1 && !wait_bar(B, &B.o_free[m & 1], (m >> 1) - 1)) break;
                 fence_after_sync();
                 if (elect_one()) {
                     const uint64_t dq = desc_add(dq0, st * L::kStage);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)  // terms and halves of K: columns kColSHi + 64 * term + 32 * half
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
-                            mma_f16_ts(tu + kColO2, tu + kColSHi + 32 * x + 8 * ks,
-                                       desc_add(dq, (x & 1) * (kTile / 2) + 32 * ks), id_qs, (x | ks) > 0);
+                            mma_f16_ts(tu + kColO2 + 128 * (m & 1), tu + kColS + 32 * x + 8 * ks, desc_add(dq, x * (kTile / 2) + 32 * ks), id_qs,
+                                       (x | ks) > 0);
                     mma_commit(&B.s_free);
                 }
                 __syncwarp();
-                if (!wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;
+                if (final && !wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;
                 fence_after_sync();
                 if (elect_one()) {
-                    const uint64_t dp = desc_add(dps, (m & 1) * 2 * L::kP);
+                    const uint64_t dp = desc_add(dps, (m & 1) * L::kP);
 #pragma unroll
-                    for (int term = 1; term >= 0; --term)
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tu + kColO1, desc_add(dv, koff_mnmaj(16 * ks)),
-                                    desc_add(dp, term * L::kP + koff_kmaj(C, 16 * ks)), id_pv, term < 1 || ks > 0);
-                    mma_commit(&B.o_full);
-                    mma_commit(&B.empty[st]);
+                    for (int ks = 0; ks < 4; ++ks)
+                        mma_f16(tu + kColO1 + 128 * (m & 1), desc_add(dv, koff_mnmaj(16 * ks)), desc_add(dp, koff_kmaj(C, 16 * ks)), id_pv, ks > 0);
+                    mma_commit(&B.o_full[m & 1]);
+                    mma_commit(&B.pv_done[m % 5]);
+                    if (!last) mma_commit(&B.empty[st]);  // a last chunk's stage takes the state out first
                 }
                 __syncwarp();
                 if (final) break;
             }
             if (B.abort && elect_one()) {  // products in flight end before the tensor memory is given back
                 mma_commit(&B.drain);
-                const long long t0 = clock64();
-                while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitBudget) {}
+                for (const int t0 = (int)clock(); !mbar_try_wait(&B.drain, 0) && (int)clock() - t0 < 1 << 30;) {}
             }
             __syncwarp();
         }
     }
+    if (!kStateOnly && warp == 26 && lane == 0)
+        // ---- finished states on their way out ----
+        for (int i = 0; work; ++i) {
+            if (!wait_one(B, &B.st_full, i)) break;
+            const int out = B.st_out, m = B.st_m, final = B.st_final, st = m % L::kStages;
+            if (out >= 0) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    tma_store(&m_new, sb + (x == 3 ? L::spare : st * L::kStage + x * kBox), 32 * x, out);
+                bulk_wait_read0();
+            }
+            arrive(&B.empty[st]);
+            arrive(&B.st_free);
+            if (final) break;
+        }
     __syncwarp();
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
+    if (tid == 0 && B.abort) atomicOr(&g_device_status, kDevStatTimeout);
     if (warp == 23) tmem_dealloc(tm, kStateOnly ? 256 : 512);
 }
 
@@ -754,6 +805,7 @@ __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillP
     // the sequence's place in the workspace: the segments of those before it
     if (threadIdx.x < 32) {
         int ws = 0;
+#pragma unroll 1
         for (int i = threadIdx.x; i < n; i += 32) {
             int t0, len;
             const int k = n_segments(p, i, t0, len);
@@ -776,6 +828,7 @@ __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillP
                        : make_float4(0.f, 0.f, 0.f, 0.f);
     if (p.first_from_ws) *reinterpret_cast<float4*>(w) = s;
     float4 u = *reinterpret_cast<const float4*>(w + step);
+#pragma unroll 2
     for (int i = 1; i < nseg; ++i) {
         float4 next = u;
         if (i + 1 < nseg) next = *reinterpret_cast<const float4*>(w + (i + 1) * step);
@@ -814,6 +867,18 @@ static bool encode(CUtensorMap* map, const void* x, int heads, int T) {
     const cuuint64_t strides[2] = {(cuuint64_t)kDim * 2, (cuuint64_t)heads * kDim * 2};
     const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)C}, estr[3] = {1u, 1u, 1u};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// [states, 128, 128] fp32 in boxes of 32 columns x 128 rows, 128-byte swizzle.
+static bool encode_states(CUtensorMap* map, const void* x, long long states) {
+    const EncodeFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)kDim, (cuuint64_t)kDim, (cuuint64_t)states};
+    const cuuint64_t strides[2] = {(cuuint64_t)kDim * 4, (cuuint64_t)kDim * kDim * 4};
+    const cuuint32_t box[3] = {32u, (cuuint32_t)kDim, 1u}, estr[3] = {1u, 1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(x), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -920,15 +985,17 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
             e = cudaMemcpyAsync(new_state, state, bytes, cudaMemcpyDeviceToDevice, st);
         return e == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
     }
-    CUtensorMap mq{}, mk{}, mv{};
-    if (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T)) return GDN_ERR_CUDA;
+    CUtensorMap mq{}, mk{}, mv{}, mn{};
+    if (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T) ||
+        (N > 0 && !encode_states(&mn, new_state, (long long)N * HV)))
+        return GDN_ERR_CUDA;
     if (!set_attributes()) return GDN_ERR_CUDA;
     if (ws_slots > 0) {
         const int inner = T / seg * HV;
-        decay_prefill_kernel<true><<<inner < kSms ? inner : kSms, kThreads, Lay<true>::total, st>>>(p, mq, mk, mv);
+        decay_prefill_kernel<true><<<inner < kSms ? inner : kSms, kThreads, Lay<true>::total, st>>>(p, mq, mk, mv, mn);
         decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p);
     }
     const int items = slots * HV;
-    decay_prefill_kernel<false><<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, Lay<false>::total, st>>>(p, mq, mk, mv);
+    decay_prefill_kernel<false><<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, Lay<false>::total, st>>>(p, mq, mk, mv, mn);
     return gdn_launch_status();
 }
