@@ -242,14 +242,17 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t upper2(float2 x) {
     return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
 }
-// What is left of two floats behind those bits (exact).
-__device__ __forceinline__ float2 below2(float2 x) {
-    const float a = __uint_as_float((__float_as_uint(x.x) & 0xffff0000u) ^ 0x80000000u);
-    const float b = __uint_as_float((__float_as_uint(x.y) & 0xffff0000u) ^ 0x80000000u);
-    return __fadd2_rn(x, make_float2(a, b));
+// y minus the lower / upper bf16 of t, exactly rounded once (exact where t holds y's
+// leading bits): one mixed-precision fma on the FMA pipe, where masking t out
+// and subtracting it would be an integer operation on the busier ALU pipe.
+__device__ __forceinline__ float2 minus_bf16(float2 y, uint32_t t) {
+    float2 d;
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xbf80;\n\t"
+        "fma.rn.f32.bf16 %0, l, m, %3;\n\tfma.rn.f32.bf16 %1, h, m, %4;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "r"(t), "f"(y.x), "f"(y.y));
+    return d;
 }
-
-__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 template <int kN>
 __device__ __forceinline__ void more_registers() {
@@ -441,25 +444,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = x; i < 2 * C * 8; i += 256)
                     if ((i >> 3 & (C - 1)) >= live)
                         *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
+            uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
+            uint8_t* kw = sm + L::kw + (kStateOnly ? (m & 1) * 2 * kTile : 0) + 16 * x;
+            const int row = x >> 3;  // and row + 32, in two halves of K
+            uint4 k[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const uint4*>(ks + 4096 * i);
+            const float w[2] = {gt->w[row], gt->w[row + 32]};
+            if (live < C) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (row + 32 * (i & 1) >= live) k[i] = make_uint4(0, 0, 0, 0);
+            }
             // the lower terms' buffer is free after the last product with it, k's place after its scores
             if (m >= L::kBuf && !wait_bar(B, &B.u_full[kStateOnly ? m & 1 : 0], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
             if (!kStateOnly && !wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
-            uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
-            uint8_t* kw = sm + L::kw + (kStateOnly ? (m & 1) * 2 * kTile : 0) + 16 * x;
-#pragma unroll 2
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = (32 * i + (x >> 3)) & (C - 1);
-                const uint4 r = *reinterpret_cast<const uint4*>(ks + 4096 * i);
-                const uint32_t in[4] = {r.x, r.y, r.z, r.w};
-                const float w = gt->w[row];
+                const uint32_t in[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
                 uint32_t t0[4], t1[4], t2[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float2 y = __fmul2_rn(make_float2(w, w), widen2(row < live ? in[e] : 0u));
+                    float2 y = __fmul2_rn(make_float2(w[i & 1], w[i & 1]), widen2(in[e]));
                     t0[e] = upper2(y);
-                    y = below2(y);
+                    y = minus_bf16(y, t0[e]);
                     t1[e] = upper2(y);
-                    t2[e] = upper2(below2(y));
+                    t2[e] = upper2(minus_bf16(y, t1[e]));
                 }
                 *reinterpret_cast<uint4*>(ks + 4096 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
                 *reinterpret_cast<uint4*>(kw + 4096 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
