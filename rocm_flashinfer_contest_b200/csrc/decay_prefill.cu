@@ -129,7 +129,7 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 //   warps 16..19      outputs: one v each thread, written 32 v (64 bytes) at a time
 //   warps 20, 21, 25  decayed scores: one row i each thread, 32 columns j
 //   warp  22          TMA loads
-//   warp  23          one thread that issues the products
+//   warps 23, 27      one thread each that issues the products
 //   warp  24          gates, and what the chunk belongs to
 //   warp  26          finished states on their way out
 // (a warp reads the 32 tensor-memory lanes of its number modulo 4, hence 25).
@@ -176,8 +176,8 @@ struct Gate {
 static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
-    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full[2], u_free[2], p_ready[2], kw_ready[2], s_ready,
-        s_free, o_full[2], o_free[2], st_full, st_free, drain;
+    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full[2], u_free[2], p_read, p_ready[2], kw_ready[2], s_ready,
+        s_free, o_full[2], o_free[2], st_full, st_free, drain[2];
     uint32_t tmem;
     volatile int abort;
     int none;
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             B.abort = 0;
 #pragma unroll
-            for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 1);
+            for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], kStateOnly ? 1 : 2);
 #pragma unroll
             for (int i = 0; i < 5; ++i) mbar_init(&B.pv_done[i], 1);
 #pragma unroll
@@ -293,11 +293,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_init(&B.p_ready[i], 96), mbar_init(&B.kw_ready[i], 256);
                 mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
             }
+            mbar_init(&B.p_read, 96);
             mbar_init(&B.s_ready, 256);
             mbar_init(&B.s_free, 1);
             mbar_init(&B.st_full, 256);
             mbar_init(&B.st_free, 1);
-            mbar_init(&B.drain, 1);
+            mbar_init(&B.drain[0], 1), mbar_init(&B.drain[1], 1);
             fence_mbar_init();
         }
         __syncwarp();
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp < 22 || warp == 25) {
             if (!kStateOnly) {
                 // ---- decayed scores ----
-                const int wq = warp & 1, i = 32 * wq + lane, jb0 = warp == 25 ? 2 : 0;
+                const int wq = warp & 1, i = 32 * wq + lane, jb = warp == 25 ? 1 : 0;
                 const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
 #pragma unroll 1
                 for (int m = 0; work; ++m) {
@@ -555,31 +556,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int flags = gt->flags;
                     const float ci = gt->c2[i];
                     uint8_t* row = sm + L::ps + (m & 1) * L::kP + i * 128;
+                    float x[32];
+                    tmem_ld32(tl + kColP + 32 * jb, x);
+                    fence_before_sync();
+                    arrive(&B.p_read);  // the next chunk's scores may follow
                     // this buffer's last products are those of chunk m - 2
                     if (m > 1 && !wait_bar(B, &B.pv_done[(m - 2) % 5], (m - 2) / 5)) break;
                     if (warp == 20)  // rows 0 .. 31: nothing in columns 32 .. 63
 #pragma unroll
                         for (int q = 4; q < 8; ++q) *reinterpret_cast<uint4*>(row + ((q ^ (i & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-#pragma unroll 1
-                    for (int jb = jb0; jb < jb0 + 2; ++jb) {  // 16 columns at a time
-                        float x[16];
-                        tmem_ld16(tl + kColP + 16 * jb, x);
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4) {
-                            const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[16 * jb + j]);
-                            const float2 a = __fmul2_rn(make_float2(p.scale * ex2(ci - cj.x), p.scale * ex2(ci - cj.y)), make_float2(x[j], x[j + 1]));
-                            const float2 c = __fmul2_rn(make_float2(p.scale * ex2(ci - cj.z), p.scale * ex2(ci - cj.w)), make_float2(x[j + 2], x[j + 3]));
-                            x[j] = 16 * jb + j <= i ? a.x : 0.f;
-                            x[j + 1] = 16 * jb + j + 1 <= i ? a.y : 0.f;
-                            x[j + 2] = 16 * jb + j + 2 <= i ? c.x : 0.f;
-                            x[j + 3] = 16 * jb + j + 3 <= i ? c.y : 0.f;
-                        }
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[32 * jb + j]);
+                        const float2 a = __fmul2_rn(make_float2(ex2(ci - cj.x), ex2(ci - cj.y)), make_float2(x[j], x[j + 1]));
+                        const float2 c = __fmul2_rn(make_float2(ex2(ci - cj.z), ex2(ci - cj.w)), make_float2(x[j + 2], x[j + 3]));
+                        x[j] = a.x, x[j + 1] = a.y, x[j + 2] = c.x, x[j + 3] = c.y;
+                    }
+                    if (warp != 21)  // the blocks on the diagonal
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const float* y = x + 8 * q;
-                            *reinterpret_cast<uint4*>(row + (((2 * jb + q) ^ (i & 7)) << 4)) = make_uint4(
-                                pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+                        for (int j = 0; j < 32; ++j) x[j] = j <= lane ? x[j] : 0.f;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t t[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 z = __fmul2_rn(make_float2(p.scale, p.scale), make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]));
+                            t[e] = pack_bf16(z.x, z.y);
                         }
+                        *reinterpret_cast<uint4*>(row + (((4 * jb + q) ^ (i & 7)) << 4)) = make_uint4(t[0], t[1], t[2], t[3]);
                     }
                     fence_before_sync();
                     fence_proxy_async_smem();
@@ -687,100 +691,112 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                 for (int k = m > L::kStages ? m - L::kStages : 0; k < m; ++k)
                     for (const int t0 = (int)clock(); !mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && (int)clock() - t0 < 1 << 24;) {}
-        } else if (warp == 23) {
-            // ---- products, issued by one elected thread ----
+        } else if (warp == 23 || (!kStateOnly && warp == 27)) {
+            // ---- products, each warp's issued by one elected thread: warp 23 the scores and U, warp 27 the outputs ----
             constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
                                id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
             const uint32_t tu = __shfl_sync(0xffffffffu, tm, 0), su = __shfl_sync(0xffffffffu, sb, 0);
-            const uint64_t dkw = desc_mnmaj(su + L::kw, C, 0), dps = desc_kmaj(su + L::ps, C, 0);
-            const uint64_t dq0 = desc_kmaj(su, C, 0), dk0 = desc_kmaj(su + L::oK, C, 0), dv0 = desc_mnmaj(su + L::oV, C, 0);
-            const uint64_t dk0w = desc_mnmaj(su + L::oK, C, 0);  // k as U's operand
-            auto scores = [&](int m, int st) {
-                if (elect_one()) {
-                    const uint64_t dq = desc_add(dq0, st * L::kStage), dk = desc_add(dk0, st * L::kStage);
+            const uint64_t dv0 = desc_mnmaj(su + L::oV, C, 0), dq0 = desc_kmaj(su, C, 0);
+            if (warp == 23) {
+                const uint64_t dkw = desc_mnmaj(su + L::kw, C, 0);
+                const uint64_t dk0 = desc_kmaj(su + L::oK, C, 0), dk0w = desc_mnmaj(su + L::oK, C, 0);  // k of the scores, of U
+                auto scores = [&](int st) {
+                    if (elect_one()) {
+                        const uint64_t dq = desc_add(dq0, st * L::kStage), dk = desc_add(dk0, st * L::kStage);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
+                        for (int x = 0; x < 2; ++x)
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tu + kColP, desc_add(dq, x * (kTile / 2) + 32 * ks),
-                                    desc_add(dk, x * (kTile / 2) + 32 * ks), id_qk, (x | ks) > 0);
-                    mma_commit(&B.qk_full[m & 1]);
-                }
-                __syncwarp();
-            };
-            bool ok = work;
-            if (!kStateOnly && ok) {
-                ok = wait_bar(B, &B.full[0], 0);
-                fence_after_sync();
-                if (ok) scores(0, 0);
-            }
-#pragma unroll 1
-            for (int m = 0; ok; ++m) {
-                const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
-                const uint64_t dv = desc_add(dv0, st * L::kStage), dk = desc_add(dk0w, st * L::kStage);
-                bool final, last = false;
-                if (!kStateOnly) {
-                    final = gate(m)->flags & kFinal, last = gate(m)->flags & kLast;
-                    if (!final) {
-                        if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
-                        if (!wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;  // and read: P's columns are free
-                        fence_after_sync();
-                        scores(m + 1, (m + 1) % L::kStages);
+                            for (int ks = 0; ks < 4; ++ks)
+                                mma_f16(tu + kColP, desc_add(dq, x * (kTile / 2) + 32 * ks),
+                                        desc_add(dk, x * (kTile / 2) + 32 * ks), id_qk, (x | ks) > 0);
+                    }
+                };
+                bool ok = work;
+                if (!kStateOnly && ok) {
+                    ok = wait_bar(B, &B.full[0], 0);
+                    fence_after_sync();
+                    if (ok) {
+                        scores(0);
+                        if (elect_one()) mma_commit(&B.qk_full[0]);
+                        __syncwarp();
                     }
                 }
-                if (!wait_bar(B, &B.kw_ready[ub], kStateOnly ? m >> 1 : m)) break;
-                if (kStateOnly) final = gate(m)->flags & kFinal;
-                if (m >= L::kBuf && !wait_bar(B, &B.u_free[ub], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
-                fence_after_sync();
-                if (elect_one()) {
+#pragma unroll 1
+                for (int m = 0; ok; ++m) {
+                    const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
+                    const uint64_t dv = desc_add(dv0, st * L::kStage), dk = desc_add(dk0w, st * L::kStage);
+                    bool final;
+                    if (!kStateOnly) {
+                        final = gate(m)->flags & kFinal;
+                        if (!final) {
+                            if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
+                            if (!wait_bar(B, &B.p_read, m)) break;  // P's columns are free
+                            fence_after_sync();
+                            scores((m + 1) % L::kStages);
+                            if (elect_one()) mma_commit(&B.qk_full[(m + 1) & 1]);
+                            __syncwarp();
+                        }
+                    }
+                    if (!wait_bar(B, &B.kw_ready[ub], kStateOnly ? m >> 1 : m)) break;
+                    if (kStateOnly) final = gate(m)->flags & kFinal;
+                    if (m >= L::kBuf && !wait_bar(B, &B.u_free[ub], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
+                    fence_after_sync();
+                    if (elect_one()) {
 #pragma unroll
-                    for (int term = 2; term >= 0; --term)  // small terms first
+                        for (int term = 2; term >= 0; --term)  // small terms first
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tu + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
-                                    desc_add(term ? desc_add(dkw, (ub * 2 + term - 1) * kTile) : dk, koff_mnmaj(16 * ks)), id_u,
-                                    term < 2 || ks > 0);
-                    mma_commit(&B.u_full[ub]);
-                    if (kStateOnly) mma_commit(&B.empty[st]);
-                }
-                __syncwarp();
-                if (kStateOnly) {
+                            for (int ks = 0; ks < 4; ++ks)
+                                mma_f16(tu + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
+                                        desc_add(term ? desc_add(dkw, (ub * 2 + term - 1) * kTile) : dk, koff_mnmaj(16 * ks)),
+                                        id_u, term < 2 || ks > 0);
+                        mma_commit(&B.u_full[ub]);
+                        mma_commit(&B.empty[st]);
+                    }
+                    __syncwarp();
                     if (final) break;
-                    continue;
                 }
-                if (!wait_bar(B, &B.s_ready, m)) break;
-                if (m > 1 && !wait_bar(B, &B.o_free[m & 1], (m >> 1) - 1)) break;
-                fence_after_sync();
-                if (elect_one()) {
-                    const uint64_t dq = desc_add(dq0, st * L::kStage);
+            } else {
+                const uint64_t dps = desc_kmaj(su + L::ps, C, 0);
+#pragma unroll 1
+                for (int m = 0; work; ++m) {
+                    const int st = m % L::kStages;
+                    const uint64_t dv = desc_add(dv0, st * L::kStage);
+                    if (!wait_bar(B, &B.s_ready, m)) break;
+                    if (m > 1 && !wait_bar(B, &B.o_free[m & 1], (m >> 1) - 1)) break;
+                    fence_after_sync();
+                    if (elect_one()) {
+                        const uint64_t dq = desc_add(dq0, st * L::kStage);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks)
+                                mma_f16_ts(tu + kColO2 + 128 * (m & 1), tu + kColS + 32 * x + 8 * ks,
+                                           desc_add(dq, x * (kTile / 2) + 32 * ks), id_qs, (x | ks) > 0);
+                        mma_commit(&B.s_free);
+                    }
+                    __syncwarp();
+                    const int flags = gate(m)->flags;
+                    if (!wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;
+                    fence_after_sync();
+                    if (elect_one()) {
+                        const uint64_t dp = desc_add(dps, (m & 1) * L::kP);
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
-                            mma_f16_ts(tu + kColO2 + 128 * (m & 1), tu + kColS + 32 * x + 8 * ks, desc_add(dq, x * (kTile / 2) + 32 * ks), id_qs,
-                                       (x | ks) > 0);
-                    mma_commit(&B.s_free);
+                            mma_f16(tu + kColO1 + 128 * (m & 1), desc_add(dv, koff_mnmaj(16 * ks)),
+                                    desc_add(dp, koff_kmaj(C, 16 * ks)), id_pv, ks > 0);
+                        mma_commit(&B.o_full[m & 1]);
+                        mma_commit(&B.pv_done[m % 5]);
+                        if (!(flags & kLast)) mma_commit(&B.empty[st]);  // a last chunk's stage takes the state out first
+                    }
+                    __syncwarp();
+                    if (flags & kFinal) break;
                 }
-                __syncwarp();
-                if (final && !wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;
-                fence_after_sync();
-                if (elect_one()) {
-                    const uint64_t dp = desc_add(dps, (m & 1) * L::kP);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        mma_f16(tu + kColO1 + 128 * (m & 1), desc_add(dv, koff_mnmaj(16 * ks)), desc_add(dp, koff_kmaj(C, 16 * ks)), id_pv, ks > 0);
-                    mma_commit(&B.o_full[m & 1]);
-                    mma_commit(&B.pv_done[m % 5]);
-                    if (!last) mma_commit(&B.empty[st]);  // a last chunk's stage takes the state out first
-                }
-                __syncwarp();
-                if (final) break;
             }
             if (B.abort && elect_one()) {  // products in flight end before the tensor memory is given back
-                mma_commit(&B.drain);
-                for (const int t0 = (int)clock(); !mbar_try_wait(&B.drain, 0) && (int)clock() - t0 < 1 << 30;) {}
+                uint64_t* drain = &B.drain[warp == 27];
+                mma_commit(drain);
+                for (const int t0 = (int)clock(); !mbar_try_wait(drain, 0) && (int)clock() - t0 < 1 << 30;) {}
             }
-            __syncwarp();
         }
     }
     if (!kStateOnly && warp == 26 && lane == 0)
