@@ -126,7 +126,7 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 // chunk goes through all of its warps:
 //   warps  0..7       state: half a row of S each thread, fp32, in registers
 //   warps  8..15      w_j k_j in three bf16 terms
-//   warps 16..19      outputs: one v each thread, written 32 v (64 bytes) at a time
+//   warps 16..19      outputs: 32 v each warp, turned on the way to shared memory, rows sent by TMA
 //   warps 20, 21, 25  decayed scores: one row i each thread, 32 columns j
 //   warp  22          TMA loads
 //   warps 23, 27      one thread each that issues the products
@@ -151,8 +151,8 @@ struct Lay {
     static constexpr uint32_t kw = kStages * kStage;  // the scaled k's two lower terms (the first takes k's own place)
     static constexpr uint32_t ps = kw + kBuf * 2 * kTile;  // two buffers of P
     static constexpr uint32_t kP = C * C * 2;
-    static constexpr uint32_t spare = ps + (kStateOnly ? 0 : 2 * kP);  // the last columns of a state on its way out
-    static constexpr uint32_t turn = spare + (kStateOnly ? 0 : 16384);  // 1 KiB for each state warp
+    static constexpr uint32_t os = ps + (kStateOnly ? 0 : 2 * kP);  // a chunk's outputs, [token][v]
+    static constexpr uint32_t turn = os + (kStateOnly ? 0 : kTile);  // 1 KiB for each state warp
     static constexpr uint32_t gates = turn + 8 * 1024;
     static constexpr uint32_t bars = gates + kGates * 832;
     static constexpr uint32_t total = bars + 320;
@@ -176,7 +176,7 @@ struct Gate {
 static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
-    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full[2], u_free[2], p_read, p_ready[2], kw_ready[2], s_ready,
+    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full[2], u_free[2], p_read, p_ready[2], p_free[2], kw_ready[2], s_ready,
         s_free, o_full[2], o_free[2], st_full, st_free, drain[2];
     uint32_t tmem;
     volatile int abort;
@@ -216,11 +216,11 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
         : "memory");
 }
 
-// 32 columns of all 128 rows of one state ([states, 128, 128] fp32), 128-byte swizzle.
+// 32 columns of a state, 128-byte swizzle, sent in two boxes of 64 rows.
 constexpr uint32_t kBox = 128 * 32 * 4;
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int number) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(0),
-                 "r"(number), "r"(src)
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(src)
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -230,6 +230,24 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t x;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
     return x != 0;
+}
+
+// 16 lanes x 32 columns of two accumulators in the fragment layout: x[4 n + 2 r + i]
+// is lane lane / 4 + 8 r, column 8 n + 2 (lane % 4) + i.
+__device__ __forceinline__ void tmem_ld_frag2(uint32_t ta, uint32_t tb, float (&a)[16], float (&b)[16]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(ta), "r"(tb)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a[i] = __uint_as_float(r[i]), b[i] = __uint_as_float(r[16 + i]);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -254,6 +272,8 @@ __device__ __forceinline__ float2 minus_bf16(float2 y, uint32_t t) {
     return d;
 }
 
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
 template <int kN>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kN));
@@ -270,7 +290,7 @@ template <bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     decay_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mq,
                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                         const __grid_constant__ CUtensorMap m_new) {
+                         const __grid_constant__ CUtensorMap m_new, const __grid_constant__ CUtensorMap m_out) {
     using L = Lay<kStateOnly>;
     extern __shared__ __align__(1024) uint8_t sm[];
     Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
@@ -290,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&B.qk_full[i], 1), mbar_init(&B.o_full[i], 1), mbar_init(&B.o_free[i], 128);
-                mbar_init(&B.p_ready[i], 96), mbar_init(&B.kw_ready[i], 256);
+                mbar_init(&B.p_ready[i], 96), mbar_init(&B.p_free[i], 1), mbar_init(&B.kw_ready[i], 256);
                 mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
             }
             mbar_init(&B.p_read, 96);
@@ -343,6 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                              : make_float4(0.f, 0.f, 0.f, 0.f);
                         s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
                     }
+                    // (the turning space may still hold a part of the last state, on its way out)
+                    if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
 #pragma unroll
                     for (int b = 0; b < 8; ++b) {
                         float* y = s + 8 * b;
@@ -409,18 +431,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (tid == 0) p.ws_decay[out] = prod;
             }
             if (!kStateOnly && first) {
-                // the state leaves by way of its last chunk's stage (48 KiB, free after that chunk's last products)
-                // and 16 KiB beside it; the store warp sends it on and gives the stage back
+                // the state leaves by way of its last chunk's stage (48 KiB), its buffer of P and the turning
+                // space (8 KiB each), free after that chunk's last products; the store warp sends it on
+                // and gives them back
                 if (!wait_bar(B, &B.pv_done[m % 5], m / 5)) break;
-                if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
                 ++stored;
                 if (out >= 0) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        uint8_t* row = sm + (half && x ? L::spare : (m % L::kStages) * L::kStage + (2 * half + x) * kBox) + v * 128;
+                        const uint32_t box = half && x ? (v < 64 ? L::ps + (m & 1) * L::kP : L::turn - 64 * 128)
+                                                       : (m % L::kStages) * L::kStage + (2 * half + x) * kBox;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<float4*>(row + ((i ^ (v & 7)) << 4)) =
+                            *reinterpret_cast<float4*>(sm + box + v * 128 + ((i ^ (v & 7)) << 4)) =
                                 make_float4(s[32 * x + 4 * i], s[32 * x + 4 * i + 1], s[32 * x + 4 * i + 2], s[32 * x + 4 * i + 3]);
                     }
                     fence_proxy_async_smem();
@@ -501,42 +524,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait_bar(B, &B.o_full[m & 1], m >> 1)) break;
                 fence_after_sync();
                 const Gate* gt = gate(m);
-                const int live = gt->live, flags = gt->flags;
-                __nv_bfloat16* dst = p.out + ((size_t)gt->t * p.HV + gt->h) * kDim + 32 * wq + lane;
+                const int live = gt->live, flags = gt->flags, t = gt->t, h = gt->h;
+                if (tid == 512) bulk_wait_read0();  // the last chunk's rows have left
+                bar_sync(1, 128);
+                // 16 v x 32 tokens at a time, in the fragment layout of 8 x 8 matrices, which stmatrix turns
+                // into 8 tokens x 8 v: 16 bytes of a token's row, at their place under the 128-byte swizzle
 #pragma unroll 1
                 for (int b = 0; b < 4; ++b) {
+                    const uint32_t at = tl + ((uint32_t)(16 * (b & 1)) << 16) + kColO1 + 128 * (m & 1) + 32 * (b >> 1);
                     float x1[16], x2[16];
-                    tmem_ld16x2(tl + kColO1 + 128 * (m & 1) + 16 * b, tl + kColO2 + 128 * (m & 1) + 16 * b, x1, x2);
-                    uint32_t y[8];
+                    tmem_ld_frag2(at, at + (kColO2 - kColO1), x1, x2);
+                    uint32_t y[8];  // tokens 8 n + 2 (lane % 4) + {0, 1}; v lane / 4 and 8 on
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const float4 e = *reinterpret_cast<const float4*>(&gt->e[16 * b + j]);
-                        const float2 a = __ffma2_rn(make_float2(e.x, e.y), make_float2(x2[j], x2[j + 1]), make_float2(x1[j], x1[j + 1]));
-                        const float2 c = __ffma2_rn(make_float2(e.z, e.w), make_float2(x2[j + 2], x2[j + 3]), make_float2(x1[j + 2], x1[j + 3]));
-                        y[j / 2] = pack_bf16(a.x, a.y);
-                        y[j / 2 + 1] = pack_bf16(c.x, c.y);
-                    }
-                    if (b == 3) {
-                        fence_before_sync();
-                        arrive(&B.o_free[m & 1]);
-                    }
-                    unsigned short* to = reinterpret_cast<unsigned short*>(dst);
-                    if (live >= 16 * b + 16) {
+                    for (int n = 0; n < 4; ++n) {
+                        const float2 e = *reinterpret_cast<const float2*>(&gt->e[32 * (b >> 1) + 8 * n + 2 * (lane & 3)]);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            to[0] = (unsigned short)y[j];
-                            to[step] = (unsigned short)(y[j] >> 16);
-                            to += 2 * step;
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (16 * b + 2 * j < live) to[0] = (unsigned short)y[j];
-                            if (16 * b + 2 * j + 1 < live) to[step] = (unsigned short)(y[j] >> 16);
-                            to += 2 * step;
+                        for (int r = 0; r < 2; ++r) {
+                            const float2 z = __ffma2_rn(e, make_float2(x2[4 * n + 2 * r], x2[4 * n + 2 * r + 1]),
+                                                        make_float2(x1[4 * n + 2 * r], x1[4 * n + 2 * r + 1]));
+                            y[2 * n + r] = pack_bf16(z.x, z.y);
                         }
                     }
-                    dst += 16 * step;
+                    // matrices of a store: tokens 8 n, v 0 and 8; tokens 8 (n + 1), v 0 and 8.  This lane's address:
+                    // token lane % 8 of matrix lane / 8
+                    const int chunk = (4 * wq + 2 * (b & 1) + (lane >> 3 & 1)) & 7;
+#pragma unroll
+                    for (int n = 0; n < 4; n += 2) {
+                        const int t8 = 32 * (b >> 1) + 8 * (n + (lane >> 4)) + (lane & 7);
+                        const uint32_t to = sb + L::os + (wq >> 1) * (kTile / 2) + t8 * 128 + ((chunk ^ (lane & 7)) << 4);
+                        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to),
+                                     "r"(y[2 * n]), "r"(y[2 * n + 1]), "r"(y[2 * n + 2]), "r"(y[2 * n + 3])
+                                     : "memory");
+                    }
+                }
+                fence_before_sync();
+                arrive(&B.o_free[m & 1]);
+                fence_proxy_async_smem();
+                bar_sync(1, 128);
+                if (live == C) {
+                    if (tid == 512) {
+                        tma_store(&m_out, sb + L::os, 0, h, t);
+                        tma_store(&m_out, sb + L::os + kTile / 2, 64, h, t);
+                    }
+                } else {  // the segment ends in this chunk: its rows only
+#pragma unroll 1
+                    for (int i = tid - 512; i < live * 16; i += 128) {
+                        const int r = i >> 4, x = i & 15;
+                        *reinterpret_cast<uint4*>(p.out + ((size_t)(t + r) * p.HV + h) * kDim + 8 * x) =
+                            *reinterpret_cast<const uint4*>(sm + L::os + (x >> 3) * (kTile / 2) + r * 128 + (((x & 7) ^ (r & 7)) << 4));
+                    }
                 }
                 if (flags & kFinal) break;
             }
@@ -561,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fence_before_sync();
                     arrive(&B.p_read);  // the next chunk's scores may follow
                     // this buffer's last products are those of chunk m - 2
-                    if (m > 1 && !wait_bar(B, &B.pv_done[(m - 2) % 5], (m - 2) / 5)) break;
+                    if (m > 1 && !wait_bar(B, &B.p_free[m & 1], (m >> 1) - 1)) break;
                     if (warp == 20)  // rows 0 .. 31: nothing in columns 32 .. 63
 #pragma unroll
                         for (int q = 4; q < 8; ++q) *reinterpret_cast<uint4*>(row + ((q ^ (i & 7)) << 4)) = make_uint4(0, 0, 0, 0);
@@ -786,7 +822,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     desc_add(dp, koff_kmaj(C, 16 * ks)), id_pv, ks > 0);
                         mma_commit(&B.o_full[m & 1]);
                         mma_commit(&B.pv_done[m % 5]);
-                        if (!(flags & kLast)) mma_commit(&B.empty[st]);  // a last chunk's stage takes the state out first
+                        if (!(flags & kLast)) {  // a last chunk's buffers take the state out first
+                            mma_commit(&B.empty[st]);
+                            mma_commit(&B.p_free[m & 1]);
+                        }
                     }
                     __syncwarp();
                     if (flags & kFinal) break;
@@ -806,11 +845,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int out = B.st_out, m = B.st_m, final = B.st_final, st = m % L::kStages;
             if (out >= 0) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    tma_store(&m_new, sb + (x == 3 ? L::spare : st * L::kStage + x * kBox), 32 * x, out);
+                for (int x = 0; x < 8; ++x)
+                    tma_store(&m_new, sb + (x == 7 ? L::turn : x == 6 ? L::ps + (m & 1) * L::kP : st * L::kStage + x * (kBox / 2)),
+                              32 * (x >> 1), 64 * (x & 1), out);
                 bulk_wait_read0();
             }
             arrive(&B.empty[st]);
+            arrive(&B.p_free[m & 1]);
             arrive(&B.st_free);
             if (final) break;
         }
@@ -897,13 +938,13 @@ static bool encode(CUtensorMap* map, const void* x, int heads, int T) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// [states, 128, 128] fp32 in boxes of 32 columns x 128 rows, 128-byte swizzle.
+// [states, 128, 128] fp32 in boxes of 32 columns x 64 rows, 128-byte swizzle.
 static bool encode_states(CUtensorMap* map, const void* x, long long states) {
     const EncodeFn fn = encode_fn();
     if (fn == nullptr) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)kDim, (cuuint64_t)kDim, (cuuint64_t)states};
     const cuuint64_t strides[2] = {(cuuint64_t)kDim * 4, (cuuint64_t)kDim * kDim * 4};
-    const cuuint32_t box[3] = {32u, (cuuint32_t)kDim, 1u}, estr[3] = {1u, 1u, 1u};
+    const cuuint32_t box[3] = {32u, 64u, 1u}, estr[3] = {1u, 1u, 1u};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(x), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1011,17 +1052,17 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
             e = cudaMemcpyAsync(new_state, state, bytes, cudaMemcpyDeviceToDevice, st);
         return e == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
     }
-    CUtensorMap mq{}, mk{}, mv{}, mn{};
-    if (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T) ||
+    CUtensorMap mq{}, mk{}, mv{}, mn{}, mo{};
+    if (!encode(&mq, q, H, T) || !encode(&mo, out, HV, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T) ||
         (N > 0 && !encode_states(&mn, new_state, (long long)N * HV)))
         return GDN_ERR_CUDA;
     if (!set_attributes()) return GDN_ERR_CUDA;
     if (ws_slots > 0) {
         const int inner = T / seg * HV;
-        decay_prefill_kernel<true><<<inner < kSms ? inner : kSms, kThreads, Lay<true>::total, st>>>(p, mq, mk, mv, mn);
+        decay_prefill_kernel<true><<<inner < kSms ? inner : kSms, kThreads, Lay<true>::total, st>>>(p, mq, mk, mv, mn, mo);
         decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p);
     }
     const int items = slots * HV;
-    decay_prefill_kernel<false><<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, Lay<false>::total, st>>>(p, mq, mk, mv, mn);
+    decay_prefill_kernel<false><<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, Lay<false>::total, st>>>(p, mq, mk, mv, mn, mo);
     return gdn_launch_status();
 }
