@@ -17,7 +17,8 @@
  * current device; nothing is allocated, the host never waits, argument errors
  * are reported before anything is launched.  K == V == 128, H >= 1,
  * HV % H == 0.  scale == 0 means 1/sqrt(K).  q, k, v, out, states, pools and
- * workspaces 16-byte aligned, log_decay 4 bytes, index arrays their own size.
+ * workspaces 16-byte aligned (the prefill's states and workspace 32),
+ * log_decay 4 bytes, index arrays their own size.
  * The reference project has no counterpart of these operators.
  */
 #ifndef GDN_DECAY_B200_H_
@@ -46,7 +47,7 @@ extern "C" {
  * The products run on 64-token chunks, so a value of v that is not finite
  * spoils the outputs of its whole chunk, those of earlier tokens too.
  *
- * workspace: device memory, 16-byte aligned, at least
+ * workspace: device memory, 32-byte aligned, at least
  * gdn_decay_prefill_workspace_bytes(N, T, HV) bytes (which may be 0; the
  * workspace may then be NULL); contents on entry do not matter.  Calls whose
  * work overlaps on the GPU need a workspace each.

@@ -68,11 +68,11 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
-def require16(t, name: str, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """``require`` for a read-only operand of a kernel that loads 16 bytes at a
-    time: a view that starts off a 16-byte boundary is copied."""
+def require16(t, name: str, dtype: torch.dtype, device: torch.device, align: int = 16) -> torch.Tensor:
+    """``require`` for a read-only operand of a kernel that loads ``align`` bytes
+    at a time: a view that starts off such a boundary is copied."""
     t = require(t, name, dtype, device)
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.data_ptr() % align == 0 else t.clone()
 
 
 def require_out(t, name: str, dtype: torch.dtype, shape, device: torch.device) -> torch.Tensor:

@@ -6,12 +6,16 @@
 //   o_i = scale * ( e^{c_i} S q_i  +  sum_{j <= i} e^{c_i - c_j} (q_i . k_j) v_j )
 //   S'  = e^{c_63} S + sum_j v_j (w_j k_j)^T,     w_j = e^{c_63 - c_j}
 //
-// One CTA walks the chunks of one segment (up to seg_len tokens of one
-// sequence) of one v-head.  Long sequences are cut into segments so that about
-// 148 CTAs have work: a first launch sums every segment's own contribution to
-// the state (the same kernel without queries, kStateOnly), a second turns these
-// into the state before each segment, and the third does everything.  A call
-// whose T fits one segment launches the third only.
+// A CTA walks the chunks of segments: up to seg_len tokens of one sequence, for
+// one v-head.  Long sequences are cut into segments so that 148 CTAs have work,
+// and these run in two launches of the same kernel: the first takes every
+// segment that another one follows, a sequence's first segment from its state
+// (and is done with it), the others from a zero state, for what they add to the
+// state (their outputs are dropped); a small kernel turns that into the state
+// before each segment; the second launch takes the segments that are not a
+// sequence's first.  With n segments the work is 2 (n - 1) / n of one pass, on
+// n - 1 times as many CTAs.  Sequences of one segment run in the second launch,
+// which is the only one of a call whose T fits a segment.
 //
 // Products, all on tcgen05 with fp32 accumulators in tensor memory and every
 // operand in the layout in which it arrives (token-major tiles from TMA):
@@ -51,11 +55,12 @@ struct PrefillParams {
     const void* cu;
     __nv_bfloat16* out;
     float* new_state;
-    float* ws_state;  // [ws slots][HV][V][K]: the state before a segment (of its predecessor, after the first launch)
-    float* ws_decay;  // [ws slots][HV]: e^(sum of a segment's log decays), at its successor's place
+    float* ws_state;  // [ws slots][HV][V][K]: the state before a segment (after the first launch: what its
+                      // predecessor adds to it)
+    float* ws_decay;  // [ws slots][HV]: e^(sum of the predecessor's log decays)
     float scale;
     int cu64, per_token, N, T, HV, rep, seg_len, ws_slots;
-    int first_from_ws;  // new_state is state: the first of several segments reads the copy in ws_state
+    int first;  // the first of the two launches
 };
 
 __device__ __forceinline__ int cu_at(const void* cu, int is64, int i, int T) {
@@ -63,9 +68,9 @@ __device__ __forceinline__ int cu_at(const void* cu, int is64, int i, int T) {
     return (int)(x < 0 ? 0 : x > T ? T : x);
 }
 
-// Segments in order of their sequences, found by one warp that asks for
-// ascending numbers: it keeps the block of 32 sequences where it last looked
-// and what came before it.
+// Segments of a launch in order of their sequences, found by one warp that asks
+// for ascending numbers: it keeps the block of 32 sequences where it last
+// looked and what came before it.
 struct Finder {
     int base = 0, before = 0, ws = 0;
 };
@@ -83,10 +88,9 @@ __device__ __forceinline__ int n_segments(const PrefillParams& p, int n, int& t0
     return len > p.seg_len ? (len + p.seg_len - 1) / p.seg_len : 1;
 }
 
-// The slot-th segment (kInner: of those that another one follows); n = N: there
-// is none.  Malformed cu_seqlens can make sequences overlap; segments whose
-// workspace slots would lie past the end are then left out.
-template <bool kInner>
+// The launch's segment number `slot`; n = N: there is none.  Malformed
+// cu_seqlens can make sequences overlap; segments whose workspace slots would
+// lie past the end are then left out.
 __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int slot) {
     const int lane = threadIdx.x & 31;
     Item it{p.N, 0, 0, 0, 0, 0};
@@ -94,7 +98,7 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
     for (; f.base < p.N; f.base += 32) {
         int t0 = 0, len = 0, nseg = 0;
         if (f.base + lane < p.N) nseg = n_segments(p, f.base + lane, t0, len);
-        const int cnt = kInner ? (nseg > 1 ? nseg - 1 : 0) : nseg, wcnt = nseg > 1 ? nseg : 0;
+        const int wcnt = nseg > 1 ? nseg : 0, cnt = nseg > 1 ? nseg - 1 : p.first ? 0 : nseg;
         int cs = cnt, wsum = wcnt;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -105,8 +109,8 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
         if (who) {
             const int src = __ffs(who) - 1;
             it.n = f.base + src;
-            it.s = slot - (f.before + __shfl_sync(0xffffffffu, cs - cnt, src));
             it.nseg = __shfl_sync(0xffffffffu, nseg, src);
+            it.s = slot - (f.before + __shfl_sync(0xffffffffu, cs - cnt, src)) + (!p.first && it.nseg > 1);
             it.ws = f.ws + __shfl_sync(0xffffffffu, wsum - wcnt, src);
             t0 = __shfl_sync(0xffffffffu, t0, src), len = __shfl_sync(0xffffffffu, len, src);
             it.t0 = t0 + it.s * p.seg_len;
@@ -141,23 +145,21 @@ constexpr int kThreads = 28 * 32;
 constexpr int kRegsState = 112, kRegsScale = 48, kRegsOut = 72, kRegsRest = 56;
 static_assert(256 * (kRegsState + kRegsScale) + 128 * (kRegsOut + 2 * kRegsRest) <= kThreads * 72, "register split");
 
-template <bool kStateOnly>
-struct Lay {
+// Shared memory, in bytes from its start.
+struct L {
     static constexpr int kStages = 3;
-    static constexpr int kGates = kStages + 2;       // gates outlive their tiles (read by the state and output warps)
-    static constexpr int kBuf = kStateOnly ? 2 : 1;  // buffers of U and of the scaled k's lower terms
-    static constexpr uint32_t kStage = (kStateOnly ? 2 : 3) * kTile;
-    static constexpr uint32_t oK = kStateOnly ? 0 : kTile, oV = oK + kTile;  // inside a stage; q at 0
+    static constexpr int kGates = kStages + 2;  // gates outlive their tiles (read by the state and output warps)
+    static constexpr uint32_t kStage = 3 * kTile, oK = kTile, oV = 2 * kTile;  // a stage: q, k, v
     static constexpr uint32_t kw = kStages * kStage;  // the scaled k's two lower terms (the first takes k's own place)
-    static constexpr uint32_t ps = kw + kBuf * 2 * kTile;  // two buffers of P
+    static constexpr uint32_t ps = kw + 2 * kTile;    // two buffers of P
     static constexpr uint32_t kP = C * C * 2;
-    static constexpr uint32_t os = ps + (kStateOnly ? 0 : 2 * kP);  // a chunk's outputs, [token][v]
-    static constexpr uint32_t turn = os + (kStateOnly ? 0 : kTile);  // 1 KiB for each state warp
-    static constexpr uint32_t gates = turn + 8 * 1024;
+    static constexpr uint32_t os = ps + 2 * kP;       // a chunk's outputs, [token][v]
+    static constexpr uint32_t tail = os + kTile;      // the last piece of a state on its way out
+    static constexpr uint32_t gates = tail + 8 * 1024;
     static constexpr uint32_t bars = gates + kGates * 832;
     static constexpr uint32_t total = bars + 320;
 };
-static_assert(Lay<false>::total <= 227 * 1024 && Lay<true>::total <= 227 * 1024, "shared memory");
+static_assert(L::total <= 227 * 1024, "shared memory");
 
 enum : int { kFirst = 1, kLast = 2, kFinal = 4 };
 
@@ -169,15 +171,18 @@ struct Gate {
     float a;      // e^{c_63}
     int flags;    // first / last chunk of its segment, last chunk of this CTA
     int t, live;  // first token; tokens of the segment from there on, at most 64
+    int rows;     // rows of output to write: live, or none
     int h;
     const float* src;  // first chunk: the state before it (null: zero)
-    int out;       // last chunk: the state's number in new_state (-1: it goes nowhere), kStateOnly: in the workspace
+    int out;           // last chunk: where the state after it goes: a number in the workspace (first launch) or in
+                       // new_state, or nowhere (-1)
+    int decay;         // last chunk: the number in the workspace where the segment's decay goes, or -1
 };
 static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
-    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full[2], u_free[2], p_read, p_ready[2], p_free[2], kw_ready[2], s_ready,
-        s_free, o_full[2], o_free[2], st_full, st_free, drain[2];
+    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full, u_free, p_read, p_ready[2], p_free[2], kw_ready, s_ready, s_free,
+        o_full[2], o_free[2], st_full, st_free, drain[2];
     uint32_t tmem;
     volatile int abort;
     int none;
@@ -286,12 +291,10 @@ __device__ __forceinline__ void fewer_registers() {
 // Tensor-memory columns
 constexpr uint32_t kColU = 0, kColS = 128, kColP = 192, kColO1 = 256, kColO2 = 320;  // (O: a second buffer 128 on)
 
-template <bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, 1)
     decay_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mq,
                          const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                         const __grid_constant__ CUtensorMap m_new, const __grid_constant__ CUtensorMap m_out) {
-    using L = Lay<kStateOnly>;
+                         const __grid_constant__ CUtensorMap m_state, const __grid_constant__ CUtensorMap m_out) {
     extern __shared__ __align__(1024) uint8_t sm[];
     Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -300,33 +303,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     Finder finder;
     Item it{p.N, 0, 0, 0, 0, 0};
-    if (warp == 22) {
-        if (lane == 0) {
-            B.abort = 0;
+    if (warp == 22 || warp == 24) it = find_item(p, finder, blockIdx.x / p.HV);
+    if (tid == 22 * 32) {
+        B.abort = 0;
+        B.none = it.n >= p.N;
 #pragma unroll
-            for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], kStateOnly ? 1 : 2);
+        for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 2);
 #pragma unroll
-            for (int i = 0; i < 5; ++i) mbar_init(&B.pv_done[i], 1);
+        for (int i = 0; i < 5; ++i) mbar_init(&B.pv_done[i], 1);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                mbar_init(&B.qk_full[i], 1), mbar_init(&B.o_full[i], 1), mbar_init(&B.o_free[i], 128);
-                mbar_init(&B.p_ready[i], 96), mbar_init(&B.p_free[i], 1), mbar_init(&B.kw_ready[i], 256);
-                mbar_init(&B.u_full[i], 1), mbar_init(&B.u_free[i], 256);
-            }
-            mbar_init(&B.p_read, 96);
-            mbar_init(&B.s_ready, 256);
-            mbar_init(&B.s_free, 1);
-            mbar_init(&B.st_full, 256);
-            mbar_init(&B.st_free, 1);
-            mbar_init(&B.drain[0], 1), mbar_init(&B.drain[1], 1);
-            fence_mbar_init();
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&B.qk_full[i], 1), mbar_init(&B.o_full[i], 1), mbar_init(&B.o_free[i], 128);
+            mbar_init(&B.p_ready[i], 96), mbar_init(&B.p_free[i], 1), mbar_init(&B.drain[i], 1);
         }
-        __syncwarp();
-        it = find_item<kStateOnly>(p, finder, blockIdx.x / p.HV);
-        if (lane == 0) B.none = it.n >= p.N;
+        mbar_init(&B.kw_ready, 256), mbar_init(&B.u_full, 1), mbar_init(&B.u_free, 256);
+        mbar_init(&B.p_read, 96), mbar_init(&B.s_ready, 256), mbar_init(&B.s_free, 1);
+        mbar_init(&B.st_full, 256), mbar_init(&B.st_free, 1);
+        fence_mbar_init();
     }
     if (warp == 23) {
-        tmem_alloc(&B.tmem, kStateOnly ? 256 : 512);
+        tmem_alloc(&B.tmem, 512);
         tmem_relinquish();
     }
     fence_before_sync();
@@ -340,12 +336,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         more_registers<kRegsState>();
         const int half = warp >> 2, v0 = 32 * (warp & 3), v = v0 + lane;
         const uint32_t tl = tm + ((uint32_t)v0 << 16);
-        // rows v0 .. v0 + 31 are turned in shared memory by 8 columns at a time, so that two lanes
-        // read or write 32 bytes of one row; 16-byte place x of row r holds columns of x ^ (r >> 2 & 1)
-        uint8_t* by_row = sm + L::turn + 1024 * warp + lane * 32;
-        uint8_t* by_pair = sm + L::turn + 1024 * warp + (lane >> 1) * 32 + (((lane ^ lane >> 3) & 1) << 4);
-        const int sw = (lane >> 2 & 1) << 4;
-        const int off = (v0 + (lane >> 1)) * kDim + 64 * half + 4 * (lane & 1);
         float s[64];
         float prod = 1.f;
         bool first = true;
@@ -353,60 +343,46 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int m = 0; work; ++m) {
             const Gate* gt = gate(m);
-            if (!kStateOnly) {
-                if (first) {
-                    if (!wait_bar(B, &B.full[m % L::kStages], m / L::kStages)) break;
-                    const float* src = gt->src;
+            if (first) {
+                if (!wait_bar(B, &B.full[m % L::kStages], m / L::kStages)) break;
+                prod = 1.f;
+                const float* src = gt->src;
+                if (src != nullptr) {
+                    src += v * kDim + 64 * half;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 x = src ? __ldcs(reinterpret_cast<const float4*>(src + off + (i & 1) * 16 * kDim + 8 * (i >> 1)))
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
-                        s[4 * i] = x.x, s[4 * i + 1] = x.y, s[4 * i + 2] = x.z, s[4 * i + 3] = x.w;
-                    }
-                    // (the turning space may still hold a part of the last state, on its way out)
-                    if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
+                    for (int i = 0; i < 8; ++i)
+                        asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                                     : "=f"(s[8 * i]), "=f"(s[8 * i + 1]), "=f"(s[8 * i + 2]), "=f"(s[8 * i + 3]),
+                                       "=f"(s[8 * i + 4]), "=f"(s[8 * i + 5]), "=f"(s[8 * i + 6]), "=f"(s[8 * i + 7])
+                                     : "l"(src + 8 * i)
+                                     : "memory");
+                } else {
 #pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        float* y = s + 8 * b;
-                        __syncwarp();
-                        *reinterpret_cast<float4*>(by_pair) = make_float4(y[0], y[1], y[2], y[3]);
-                        *reinterpret_cast<float4*>(by_pair + 512) = make_float4(y[4], y[5], y[6], y[7]);
-                        __syncwarp();
-                        const float4 x0 = *reinterpret_cast<const float4*>(by_row + sw);
-                        const float4 x1 = *reinterpret_cast<const float4*>(by_row + (sw ^ 16));
-                        y[0] = x0.x, y[1] = x0.y, y[2] = x0.z, y[3] = x0.w;
-                        y[4] = x1.x, y[5] = x1.y, y[6] = x1.z, y[7] = x1.w;
-                    }
+                    for (int i = 0; i < 64; ++i) s[i] = 0.f;
                 }
-                // S's terms are free once the products with them are done
-                if (m > 0 && !wait_bar(B, &B.s_free, m - 1)) break;
-                fence_after_sync();
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t x[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] = pack_bf16(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]);
-                    tmem_st16_u32_nowait(tl + kColS + 32 * half + 16 * i, x);
-                }
-                tmem_wait_st();
-                fence_before_sync();
-                arrive(&B.s_ready);
             }
-            const int ub = kStateOnly ? m & 1 : 0;
-            if (!wait_bar(B, &B.u_full[ub], kStateOnly ? m >> 1 : m)) break;
+            // S's operand is free once the products with it are done
+            if (m > 0 && !wait_bar(B, &B.s_free, m - 1)) break;
+            fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t x[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = pack_bf16(s[32 * i + 2 * j], s[32 * i + 2 * j + 1]);
+                tmem_st16_u32_nowait(tl + kColS + 32 * half + 16 * i, x);
+            }
+            tmem_wait_st();
+            fence_before_sync();
+            arrive(&B.s_ready);
+            if (!wait_bar(B, &B.u_full, m)) break;
             fence_after_sync();
             const float a = gt->a;
-            const int flags = gt->flags, out = gt->out;
-            if (kStateOnly && first) {
-                prod = 1.f;
-#pragma unroll
-                for (int i = 0; i < 64; ++i) s[i] = 0.f;
-            }
+            const int flags = gt->flags, out = gt->out, decay = gt->decay;
             prod *= a;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float x[16];
-                tmem_ld16(tl + kColU + 128 * ub + 64 * half + 16 * i, x);
+                tmem_ld16(tl + kColU + 64 * half + 16 * i, x);
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) {
                     const float2 y = __ffma2_rn(make_float2(a, a), make_float2(s[16 * i + j], s[16 * i + j + 1]), make_float2(x[j], x[j + 1]));
@@ -414,32 +390,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             fence_before_sync();
-            arrive(&B.u_free[ub]);
+            arrive(&B.u_free);
             first = flags & kLast;
-            if (kStateOnly && first) {
-                float* dst = p.ws_state + (size_t)out * kDim * kDim + off;
-#pragma unroll
-                for (int b = 0; b < 8; ++b) {
-                    const float* y = s + 8 * b;
-                    __syncwarp();
-                    *reinterpret_cast<float4*>(by_row + sw) = make_float4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<float4*>(by_row + (sw ^ 16)) = make_float4(y[4], y[5], y[6], y[7]);
-                    __syncwarp();
-                    *reinterpret_cast<float4*>(dst + 8 * b) = *reinterpret_cast<const float4*>(by_pair);
-                    *reinterpret_cast<float4*>(dst + 16 * kDim + 8 * b) = *reinterpret_cast<const float4*>(by_pair + 512);
-                }
-                if (tid == 0) p.ws_decay[out] = prod;
-            }
-            if (!kStateOnly && first) {
-                // the state leaves by way of its last chunk's stage (48 KiB), its buffer of P and the turning
-                // space (8 KiB each), free after that chunk's last products; the store warp sends it on
-                // and gives them back
+            if (first) {
+                // the state leaves by way of its last chunk's stage (48 KiB) and buffer of P (8 KiB), free after
+                // that chunk's last products, and 8 KiB beside them; the store warp sends it on and gives
+                // them back
                 if (!wait_bar(B, &B.pv_done[m % 5], m / 5)) break;
+                if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
                 ++stored;
                 if (out >= 0) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const uint32_t box = half && x ? (v < 64 ? L::ps + (m & 1) * L::kP : L::turn - 64 * 128)
+                        const uint32_t box = half && x ? (v < 64 ? L::ps + (m & 1) * L::kP : L::tail - 64 * 128)
                                                        : (m % L::kStages) * L::kStage + (2 * half + x) * kBox;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
@@ -448,7 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     fence_proxy_async_smem();
                 }
-                if (tid == 0) B.st_out = out, B.st_m = m, B.st_final = flags & kFinal;
+                if (tid == 0) {
+                    B.st_out = out, B.st_m = m, B.st_final = flags & kFinal;
+                    if (decay >= 0) p.ws_decay[decay] = prod;
+                }
                 arrive(&B.st_full);
             }
             if (flags & kFinal) break;
@@ -469,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if ((i >> 3 & (C - 1)) >= live)
                         *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
             uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
-            uint8_t* kw = sm + L::kw + (kStateOnly ? (m & 1) * 2 * kTile : 0) + 16 * x;
+            uint8_t* kw = sm + L::kw + 16 * x;
             const int row = x >> 3;  // and row + 32, in two halves of K
             uint4 k[4];
 #pragma unroll
@@ -481,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (row + 32 * (i & 1) >= live) k[i] = make_uint4(0, 0, 0, 0);
             }
             // the lower terms' buffer is free after the last product with it, k's place after its scores
-            if (m >= L::kBuf && !wait_bar(B, &B.u_full[kStateOnly ? m & 1 : 0], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
-            if (!kStateOnly && !wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
+            if (m > 0 && !wait_bar(B, &B.u_full, m - 1)) break;
+            if (!wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t in[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
@@ -500,17 +466,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 *reinterpret_cast<uint4*>(kw + kTile + 4096 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
             }
             fence_proxy_async_smem();
-            arrive(&B.kw_ready[kStateOnly ? m & 1 : 0]);
+            arrive(&B.kw_ready);
             if (flags & kFinal) break;
         }
     } else if (warp < 20) {
         fewer_registers<kRegsOut>();
-        if (!kStateOnly) {
+        {
             // ---- outputs ----
             const int wq = warp - 16;
             const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
             const size_t step = (size_t)p.HV * kDim;
-            {  // tokens of no sequence: zeros
+            if (!p.first) {  // tokens of no sequence: zeros
                 const int c0 = cu_at(p.cu, p.cu64, 0, p.T), c1 = max(c0, cu_at(p.cu, p.cu64, p.N, p.T));
                 const int rows = c0 + p.T - c1;  // a row is HV * 16 pieces of 16 bytes
 #pragma unroll 1
@@ -524,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait_bar(B, &B.o_full[m & 1], m >> 1)) break;
                 fence_after_sync();
                 const Gate* gt = gate(m);
-                const int live = gt->live, flags = gt->flags, t = gt->t, h = gt->h;
+                const int rows = gt->rows, flags = gt->flags, t = gt->t, h = gt->h;
                 if (tid == 512) bulk_wait_read0();  // the last chunk's rows have left
                 bar_sync(1, 128);
                 // 16 v x 32 tokens at a time, in the fragment layout of 8 x 8 matrices, which stmatrix turns
@@ -561,14 +527,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 arrive(&B.o_free[m & 1]);
                 fence_proxy_async_smem();
                 bar_sync(1, 128);
-                if (live == C) {
+                if (rows == C) {
                     if (tid == 512) {
                         tma_store(&m_out, sb + L::os, 0, h, t);
                         tma_store(&m_out, sb + L::os + kTile / 2, 64, h, t);
                     }
                 } else {  // the segment ends in this chunk: its rows only
 #pragma unroll 1
-                    for (int i = tid - 512; i < live * 16; i += 128) {
+                    for (int i = tid - 512; i < rows * 16; i += 128) {
                         const int r = i >> 4, x = i & 15;
                         *reinterpret_cast<uint4*>(p.out + ((size_t)(t + r) * p.HV + h) * kDim + 8 * x) =
                             *reinterpret_cast<const uint4*>(sm + L::os + (x >> 3) * (kTile / 2) + r * 128 + (((x & 7) ^ (r & 7)) << 4));
@@ -580,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         fewer_registers<kRegsRest>();
         if (warp < 22 || warp == 25) {
-            if (!kStateOnly) {
+            {
                 // ---- decayed scores ----
                 const int wq = warp & 1, i = 32 * wq + lane, jb = warp == 25 ? 1 : 0;
                 const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
@@ -632,21 +598,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool loads = warp == 22;
             int m = 0, idx = blockIdx.x;
             bool ok = work;
-            if (!loads) it = find_item<kStateOnly>(p, finder, idx / p.HV);
+            auto source = [&](const Item& it, int h) -> const float* {  // the state a segment starts from
+                const size_t mat = (size_t)kDim * kDim;
+                if (it.s > 0) return p.first ? nullptr : p.ws_state + ((size_t)(it.ws + it.s) * p.HV + h) * mat;
+                return p.state ? p.state + ((size_t)it.n * p.HV + h) * mat : nullptr;
+            };
             while (ok && it.n < p.N) {
                 const int h = idx % p.HV, hq = h / p.rep, len = it.t1 - it.t0, nch = len > C ? (len + C - 1) / C : 1;
-                const int wsi = (it.ws + it.s) * p.HV + h, number = it.n * p.HV + h;
-                const float* src = nullptr;
-                if (!kStateOnly) {
-                    if (it.s > 0 || (it.nseg > 1 && p.first_from_ws))
-                        src = p.ws_state + (size_t)wsi * kDim * kDim;
-                    else if (p.state != nullptr)
-                        src = p.state + (size_t)number * kDim * kDim;
-                }
                 idx += gridDim.x;
+                const Item next = find_item(p, finder, idx / p.HV);
                 if (loads) {
-                    if (src != nullptr && lane == 0)
-                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
+                    if (lane == 0 && next.n < p.N) {  // the next segment's state: into L2
+                        const float* src = source(next, idx % p.HV);
+                        if (src != nullptr) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
+                    }
 #pragma unroll 1
                     for (int c = 0; c < nch; ++c, ++m) {
                         const int st = m % L::kStages;
@@ -660,16 +625,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mbar_arrive_expect_tx(&B.full[st], L::kStage);
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
-                                if (!kStateOnly) tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
+                                tma_box(d + x * (kTile / 2), &mq, 64 * x, hq, t, &B.full[st]);
                                 tma_box(d + L::oK + x * (kTile / 2), &mk, 64 * x, hq, t, &B.full[st]);
                                 tma_box(d + L::oV + x * (kTile / 2), &mv, 64 * x, h, t, &B.full[st]);
                             }
                         }
                         __syncwarp();
                     }
-                    it = find_item<kStateOnly>(p, finder, idx / p.HV);
+                    it = next;
                     continue;
                 }
+                const bool last = it.s == it.nseg - 1;
+                const int after = (it.ws + it.s + 1) * p.HV + h;  // the next segment's number in the workspace
+                const float* src = source(it, h);
+                const int out = p.first ? after : last ? it.n * p.HV + h : -1, decay = p.first && it.s > 0 ? after : -1;
                 // lane l has tokens 2 l and 2 l + 1 of a chunk; a chunk's log decays are asked for one chunk ahead
                 const float* gl = p.log_decay + (p.per_token ? (size_t)(it.t0 + 2 * lane) * p.HV + h : h);
                 const size_t one = p.per_token ? p.HV : 0;
@@ -681,7 +650,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 float n0, n1;
                 ask(0, n0, n1);
-                const Item next = find_item<kStateOnly>(p, finder, idx / p.HV);
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++m) {
                     const float g0 = clamp_log_decay(n0), g1 = clamp_log_decay(n1);
@@ -715,7 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         gt->flags = (c == 0 ? kFirst : 0) | (c == nch - 1 ? kLast : 0) |
                                     (c == nch - 1 && next.n >= p.N ? kFinal : 0);
                         gt->t = it.t0 + c * C, gt->live = min(C, len - c * C);
-                        gt->h = h, gt->src = src, gt->out = kStateOnly ? wsi + p.HV : it.s == it.nseg - 1 ? number : -1;
+                        gt->rows = p.first && it.s > 0 ? 0 : gt->live;
+                        gt->h = h, gt->src = src, gt->out = out, gt->decay = decay;
                     }
                     __syncwarp();
                     if (lane == 0) arrive(&B.full[m % L::kStages]);
@@ -727,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                 for (int k = m > L::kStages ? m - L::kStages : 0; k < m; ++k)
                     for (const int t0 = (int)clock(); !mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && (int)clock() - t0 < 1 << 24;) {}
-        } else if (warp == 23 || (!kStateOnly && warp == 27)) {
+        } else if (warp == 23 || warp == 27) {
             // ---- products, each warp's issued by one elected thread: warp 23 the scores and U, warp 27 the outputs ----
             constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
                                id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
@@ -748,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 };
                 bool ok = work;
-                if (!kStateOnly && ok) {
+                if (ok) {
                     ok = wait_bar(B, &B.full[0], 0);
                     fence_after_sync();
                     if (ok) {
@@ -759,33 +728,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll 1
                 for (int m = 0; ok; ++m) {
-                    const int st = m % L::kStages, ub = kStateOnly ? m & 1 : 0;
+                    const int st = m % L::kStages;
                     const uint64_t dv = desc_add(dv0, st * L::kStage), dk = desc_add(dk0w, st * L::kStage);
-                    bool final;
-                    if (!kStateOnly) {
-                        final = gate(m)->flags & kFinal;
-                        if (!final) {
-                            if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
-                            if (!wait_bar(B, &B.p_read, m)) break;  // P's columns are free
-                            fence_after_sync();
-                            scores((m + 1) % L::kStages);
-                            if (elect_one()) mma_commit(&B.qk_full[(m + 1) & 1]);
-                            __syncwarp();
-                        }
+                    const bool final = gate(m)->flags & kFinal;
+                    if (!final) {
+                        if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
+                        if (!wait_bar(B, &B.p_read, m)) break;  // P's columns are free
+                        fence_after_sync();
+                        scores((m + 1) % L::kStages);
+                        if (elect_one()) mma_commit(&B.qk_full[(m + 1) & 1]);
+                        __syncwarp();
                     }
-                    if (!wait_bar(B, &B.kw_ready[ub], kStateOnly ? m >> 1 : m)) break;
-                    if (kStateOnly) final = gate(m)->flags & kFinal;
-                    if (m >= L::kBuf && !wait_bar(B, &B.u_free[ub], kStateOnly ? (m >> 1) - 1 : m - 1)) break;
+                    if (!wait_bar(B, &B.kw_ready, m)) break;
+                    if (m > 0 && !wait_bar(B, &B.u_free, m - 1)) break;
                     fence_after_sync();
                     if (elect_one()) {
 #pragma unroll
                         for (int term = 2; term >= 0; --term)  // small terms first
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks)
-                                mma_f16(tu + kColU + 128 * ub, desc_add(dv, koff_mnmaj(16 * ks)),
-                                        desc_add(term ? desc_add(dkw, (ub * 2 + term - 1) * kTile) : dk, koff_mnmaj(16 * ks)),
-                                        id_u, term < 2 || ks > 0);
-                        mma_commit(&B.u_full[ub]);
+                                mma_f16(tu + kColU, desc_add(dv, koff_mnmaj(16 * ks)),
+                                        desc_add(term ? desc_add(dkw, (term - 1) * kTile) : dk, koff_mnmaj(16 * ks)), id_u,
+                                        term < 2 || ks > 0);
+                        mma_commit(&B.u_full);
                         mma_commit(&B.empty[st]);
                     }
                     __syncwarp();
@@ -838,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
-    if (!kStateOnly && warp == 26 && lane == 0)
+    if (warp == 26 && lane == 0)
         // ---- finished states on their way out ----
         for (int i = 0; work; ++i) {
             if (!wait_one(B, &B.st_full, i)) break;
@@ -846,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (out >= 0) {
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
-                    tma_store(&m_new, sb + (x == 7 ? L::turn : x == 6 ? L::ps + (m & 1) * L::kP : st * L::kStage + x * (kBox / 2)),
+                    tma_store(&m_state, sb + (x == 7 ? L::tail : x == 6 ? L::ps + (m & 1) * L::kP : st * L::kStage + x * (kBox / 2)),
                               32 * (x >> 1), 64 * (x & 1), out);
                 bulk_wait_read0();
             }
@@ -860,12 +825,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after_sync();
     if (tid == 0 && B.abort) atomicOr(&g_device_status, kDevStatTimeout);
-    if (warp == 23) tmem_dealloc(tm, kStateOnly ? 256 : 512);
+    if (warp == 23) tmem_dealloc(tm, 512);
 }
 
-// The state before every segment of the sequences that have several: ws[0] = S,
-// ws[s + 1] = decay[s + 1] ws[s] + ws[s + 1].  1,024 elements of one sequence's
-// v-head per CTA.
+// The state before every segment of the sequences that have several: slot 1 holds
+// the state after the first segment already, ws[i] = decay[i] ws[i - 1] + ws[i]
+// from slot 2 on.  1,024 elements of one sequence's v-head per CTA.
 __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillParams p) {
     const int part = blockIdx.x & 15, nh = blockIdx.x >> 4, n = nh / p.HV, h = nh % p.HV;
     __shared__ int s_nseg, s_ws;
@@ -888,18 +853,16 @@ __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillP
     }
     __syncthreads();
     const int nseg = s_nseg, ws = s_ws;
-    if (nseg < 2 || ws + nseg > p.ws_slots) return;
+    if (nseg < 3 || ws + nseg > p.ws_slots) return;
     const size_t at = (size_t)part * 1024 + 4 * threadIdx.x, step = (size_t)p.HV * kDim * kDim;
-    float* w = p.ws_state + ((size_t)ws * p.HV + h) * kDim * kDim + at;
-    float4 s = p.state ? *reinterpret_cast<const float4*>(p.state + (size_t)nh * kDim * kDim + at)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.first_from_ws) *reinterpret_cast<float4*>(w) = s;
-    float4 u = *reinterpret_cast<const float4*>(w + step);
+    float* w = p.ws_state + ((size_t)(ws + 1) * p.HV + h) * kDim * kDim + at;
+    const float* d = p.ws_decay + (size_t)(ws + 1) * p.HV + h;
+    float4 s = *reinterpret_cast<const float4*>(w), u = *reinterpret_cast<const float4*>(w + step);
 #pragma unroll 2
-    for (int i = 1; i < nseg; ++i) {
+    for (int i = 1; i < nseg - 1; ++i) {
         float4 next = u;
-        if (i + 1 < nseg) next = *reinterpret_cast<const float4*>(w + (i + 1) * step);
-        const float a = p.ws_decay[(size_t)(ws + i) * p.HV + h];
+        if (i + 1 < nseg - 1) next = *reinterpret_cast<const float4*>(w + (i + 1) * step);
+        const float a = d[i * p.HV];
         s = make_float4(fmaf(a, s.x, u.x), fmaf(a, s.y, u.y), fmaf(a, s.z, u.z), fmaf(a, s.w, u.w));
         *reinterpret_cast<float4*>(w + i * step) = s;
         u = next;
@@ -950,17 +913,15 @@ static bool encode_states(CUtensorMap* map, const void* x, long long states) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Kernel attributes, once per device (again after a failure).
-static bool set_attributes() {
+// The kernel's attribute, once per device (again after a failure).
+static bool set_attribute() {
     static std::atomic<unsigned long long> done{0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return false;
     const unsigned long long bit = 1ull << (dev & 63);
     if (dev < 64 && (done.load() & bit)) return true;
-    if (cudaFuncSetAttribute(decay_prefill_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)Lay<true>::total) != cudaSuccess ||
-        cudaFuncSetAttribute(decay_prefill_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)Lay<false>::total) != cudaSuccess) {
+    if (cudaFuncSetAttribute(decay_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::total) !=
+        cudaSuccess) {
         cudaGetLastError();
         return false;
     }
@@ -968,9 +929,11 @@ static bool set_attributes() {
     return true;
 }
 
-// Tokens of a segment: T over as many as give 148 CTAs one each, at least 256.
+// Tokens of a segment, at least 256: with P = 148 / HV CTAs for each v-head, T
+// over P + 1 segments gives both launches P of them.  (HV > 74: whole sequences,
+// as two launches of one CTA a head would gain nothing.)
 static int segment_tokens(int T, int HV) {
-    const int parts = HV < kSms ? kSms / HV : 1;
+    const int parts = HV <= kSms / 2 ? kSms / HV + 1 : 1;
     const int x = T / parts + (T % parts != 0), r = x > 1 << 30 ? 1 << 30 : (x + C - 1) / C * C;
     return r < 256 ? 256 : r;
 }
@@ -1018,12 +981,12 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
     if (!cu_seqlens || (T > 0 && (!q || !k || !v || !out)) || !log_decay || (N > 0 && !new_state))
         return GDN_ERR_INVALID;
     if (!gdn_aligned(q, 16) || !gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(out, 16) ||
-        !gdn_aligned(state, 16) || !gdn_aligned(new_state, 16) || !gdn_aligned(log_decay, 4) ||
+        !gdn_aligned(state, 32) || !gdn_aligned(new_state, 32) || !gdn_aligned(log_decay, 4) ||
         !gdn_aligned(cu_seqlens, cu_seqlens_is_int64 ? 8 : 4))
         return GDN_ERR_ALIGN;
     const size_t need = gdn_decay_prefill_workspace_bytes(N, T, HV);
     if (need && (!workspace || workspace_bytes < need)) return GDN_ERR_INVALID;
-    if (need && !gdn_aligned(workspace, 16)) return GDN_ERR_ALIGN;
+    if (need && !gdn_aligned(workspace, 32)) return GDN_ERR_ALIGN;
     PrefillParams p;
     p.state = state;
     p.log_decay = log_decay;
@@ -1041,7 +1004,7 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
     p.rep = HV / H;
     p.seg_len = seg;
     p.ws_slots = ws_slots;
-    p.first_from_ws = state != nullptr && state == new_state;
+    p.first = 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (T == 0) {  // every sequence keeps its state
         const size_t bytes = (size_t)N * HV * gdn::kDim * gdn::kDim * sizeof(float);
@@ -1052,17 +1015,20 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
             e = cudaMemcpyAsync(new_state, state, bytes, cudaMemcpyDeviceToDevice, st);
         return e == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
     }
-    CUtensorMap mq{}, mk{}, mv{}, mn{}, mo{};
-    if (!encode(&mq, q, H, T) || !encode(&mo, out, HV, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T) ||
-        (N > 0 && !encode_states(&mn, new_state, (long long)N * HV)))
+    CUtensorMap mq{}, mk{}, mv{}, mn{}, mo{}, mw{};
+    if (!encode(&mq, q, H, T) || !encode(&mk, k, H, T) || !encode(&mv, v, HV, T) || !encode(&mo, out, HV, T) ||
+        (N > 0 && !encode_states(&mn, new_state, (long long)N * HV)) ||
+        (ws_slots > 0 && !encode_states(&mw, workspace, (long long)ws_slots * HV)))
         return GDN_ERR_CUDA;
-    if (!set_attributes()) return GDN_ERR_CUDA;
+    if (!set_attribute()) return GDN_ERR_CUDA;
     if (ws_slots > 0) {
-        const int inner = T / seg * HV;
-        decay_prefill_kernel<true><<<inner < kSms ? inner : kSms, kThreads, Lay<true>::total, st>>>(p, mq, mk, mv, mn, mo);
+        const int items = T / seg * HV;  // at most: segments that another one follows
+        p.first = 1;
+        decay_prefill_kernel<<<items < kSms ? items : kSms, kThreads, L::total, st>>>(p, mq, mk, mv, mw, mo);
         decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p);
+        p.first = 0;
     }
     const int items = slots * HV;
-    decay_prefill_kernel<false><<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, Lay<false>::total, st>>>(p, mq, mk, mv, mn, mo);
+    decay_prefill_kernel<<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, L::total, st>>>(p, mq, mk, mv, mn, mo);
     return gdn_launch_status();
 }

@@ -45,7 +45,7 @@ def _inputs(q, k, v, state, log_decay, cu_seqlens):
         raise ValueError("cu_seqlens must be a 1-d tensor of N + 1 offsets")
     N = cu_seqlens.numel() - 1
     if state is not None:
-        state = C.require16(state, "state", torch.float32, dev)
+        state = C.require16(state, "state", torch.float32, dev, 32)
         if tuple(state.shape) != (N, HV, V, K):
             raise ValueError(f"state must be {(N, HV, V, K)}, got {tuple(state.shape)}")
     return dev, (q, k, v, state, g, cu_seqlens.contiguous()), per_token, (T, N, H, HV, K, V)
