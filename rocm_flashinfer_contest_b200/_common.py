@@ -1,7 +1,6 @@
 """Argument handling shared by the decode and prefill ``run`` shims."""
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -58,14 +57,19 @@ def ptr(t) -> int:
 
 # ---- the decay operators and the state cache ----
 
-_no_guard = contextlib.nullcontext()
+# A call's host time is a good part of a small step, so the checks ask ready()
+# first: one short test that nearly always passes, before the functions that say
+# what is wrong or copy what can be copied.
+
+_Tensor = torch.Tensor
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def on_device(device: torch.device):
-    """Makes ``device`` current for a launch where it is not already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _no_guard
-    return torch.cuda.device(device)
+def ready(t, dtype: torch.dtype, device: torch.device) -> bool:
+    """Whether a kernel can take ``t`` as it is: its type and device, contiguous,
+    on a 32-byte boundary."""
+    return isinstance(t, _Tensor) and t.dtype is dtype and t.device == device and t.is_contiguous() \
+        and not t.data_ptr() & 31
 
 
 def require16(t, name: str, dtype: torch.dtype, device: torch.device, align: int = 16) -> torch.Tensor:

@@ -830,30 +830,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // The state before every segment of the sequences that have several: slot 1 holds
 // the state after the first segment already, ws[i] = decay[i] ws[i - 1] + ws[i]
-// from slot 2 on.  1,024 elements of one sequence's v-head per CTA.
+// from slot 2 on.  1,024 elements of one v-head of one such sequence per CTA; the
+// j-th of them is found by going through the lengths.
 __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillParams p) {
-    const int part = blockIdx.x & 15, nh = blockIdx.x >> 4, n = nh / p.HV, h = nh % p.HV;
-    __shared__ int s_nseg, s_ws;
-    // the sequence's place in the workspace: the segments of those before it
-    if (threadIdx.x < 32) {
-        int ws = 0;
+    const int part = blockIdx.x & 15, j = (blockIdx.x >> 4) / p.HV, h = (blockIdx.x >> 4) % p.HV, lane = threadIdx.x & 31;
+    int nseg = 0, ws = 0, before = 0;
+    bool found = false;
 #pragma unroll 1
-        for (int i = threadIdx.x; i < n; i += 32) {
-            int t0, len;
-            const int k = n_segments(p, i, t0, len);
-            ws += k > 1 ? k : 0;
-        }
+    for (int base = 0; base < p.N && !found; base += 32) {
+        int t0, len, k = 0;
+        if (base + lane < p.N) k = n_segments(p, base + lane, t0, len);
+        const int mine = k > 1 ? k : 0;
+        int wsum = mine;
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) ws += __shfl_xor_sync(0xffffffffu, ws, d);
-        if (threadIdx.x == 0) {
-            int t0, len;
-            s_nseg = n_segments(p, n, t0, len);
-            s_ws = ws;
+        for (int d = 1; d < 32; d *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, wsum, d);
+            if (lane >= d) wsum += x;
+        }
+        const unsigned long3 = __ballot_sync(0xffffffffu, k > 2);
+        const unsigned who = __ballot_sync(0xffffffffu, k > 2 && before + __popc(long3 & ((1u << lane) - 1)) == j);
+        if (who) {
+            const int src = __ffs(who) - 1;
+            nseg = __shfl_sync(0xffffffffu, k, src);
+            ws += __shfl_sync(0xffffffffu, wsum - mine, src);
+            found = true;
+        } else {
+            ws += __shfl_sync(0xffffffffu, wsum, 31);
+            before += __popc(long3);
         }
     }
-    __syncthreads();
-    const int nseg = s_nseg, ws = s_ws;
-    if (nseg < 3 || ws + nseg > p.ws_slots) return;
+    if (!found || ws + nseg > p.ws_slots) return;
     const size_t at = (size_t)part * 1024 + 4 * threadIdx.x, step = (size_t)p.HV * kDim * kDim;
     float* w = p.ws_state + ((size_t)(ws + 1) * p.HV + h) * kDim * kDim + at;
     const float* d = p.ws_decay + (size_t)(ws + 1) * p.HV + h;
@@ -1025,7 +1031,9 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         const int items = T / seg * HV;  // at most: segments that another one follows
         p.first = 1;
         decay_prefill_kernel<<<items < kSms ? items : kSms, kThreads, L::total, st>>>(p, mq, mk, mv, mw, mo);
-        decay_prefill_carry_kernel<<<(unsigned)((long long)N * HV * 16), 256, 0, st>>>(p);
+        // at most T / (2 seg) sequences have more than two segments (any number, if they overlap: the first are taken)
+        const int longs = T / 2 / seg;
+        if (longs > 0) decay_prefill_carry_kernel<<<longs * HV * 16, 256, 0, st>>>(p);
         p.first = 0;
     }
     const int items = slots * HV;

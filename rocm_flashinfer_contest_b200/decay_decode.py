@@ -33,69 +33,86 @@ from . import _common as C
 from ._lib import check, lib
 
 
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
 def _inputs(q, k, v, log_decay):
     dev = C.cuda_device_of(q)
-    bf = torch.bfloat16
-    q, k, v = C.require16(q, "q", bf, dev), C.require16(k, "k", bf, dev), C.require16(v, "v", bf, dev)
-    if q.dim() != 4 or q.shape[1] != 1:
-        raise ValueError(f"q must be [B, 1, H, K], got {tuple(q.shape)}")
-    B = q.shape[0]
-    H, HV, K, V = C.require_heads(q, k, v, (B, 1))
+    ready = C.ready
+    if not ready(q, _BF16, dev):
+        q = C.require16(q, "q", _BF16, dev)
+    if not ready(k, _BF16, dev):
+        k = C.require16(k, "k", _BF16, dev)
+    if not ready(v, _BF16, dev):
+        v = C.require16(v, "v", _BF16, dev)
+    qs, vs = q.shape, v.shape
+    if len(qs) != 4 or qs[1] != 1:
+        raise ValueError(f"q must be [B, 1, H, K], got {tuple(qs)}")
+    B, _, H, K = qs
+    if k.shape != qs or len(vs) != 4 or vs[:2] != qs[:2] or H < 1 or vs[2] < 1:
+        C.require_heads(q, k, v, (B, 1))
+    _, _, HV, V = vs
+    if ready(log_decay, _F32, dev) and log_decay.shape == (HV,):
+        return dev, q, k, v, log_decay, 0, B, H, HV, K, V
     g, per_token = C.require_log_decay(log_decay, (B, 1), HV, dev)
-    return dev, (q, k, v, g), per_token, (B, H, HV, K, V)
+    return dev, q, k, v, g, per_token, B, H, HV, K, V
 
 
-def _launch(dev, tensors, per_token, dims, scale, pool_in, pool_out, idx, out_idx, output):
-    q, k, v, g = tensors
-    B, H, HV, K, V = dims
-    with C.on_device(dev):
-        st = lib().gdn_decay_decode_fwd(
-            C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(pool_in), C.ptr(pool_out), int(pool_out.dtype == torch.bfloat16),
-            C.ptr(idx), C.ptr(out_idx), int(idx is not None and idx.dtype == torch.int64), C.ptr(g), per_token,
-            C.normalize_scale(scale, K), B, H, HV, K, V, pool_out.shape[0], C.ptr(output), C.stream_handle(dev))
-    check("gdn_decay_decode_fwd", st)
+def _launch(inputs, scale, pool_in, pool_out, idx, out_idx, output):
+    dev, q, k, v, g, per_token, B, H, HV, K, V = inputs
+    if dev.index != C.current_device():
+        with torch.cuda.device(dev):
+            return _launch(inputs, scale, pool_in, pool_out, idx, out_idx, output)
+    st = lib().gdn_decay_decode_fwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if pool_in is None else pool_in.data_ptr(), pool_out.data_ptr(),
+        pool_out.dtype is _BF16, 0 if idx is None else idx.data_ptr(), 0 if out_idx is None else out_idx.data_ptr(),
+        idx is not None and idx.dtype is torch.int64, g.data_ptr(), per_token, C.normalize_scale(scale, K),
+        B, H, HV, K, V, pool_out.shape[0], output.data_ptr(), C.stream_handle(dev))
+    if st:
+        check("gdn_decay_decode_fwd", st)
 
 
-def _run_checked(dev, tensors, per_token, dims, state, scale, output, new_state):
-    B, H, HV, K, V = dims
+def _state(state, inputs):
+    dev, _, _, _, _, _, B, _, HV, K, V = inputs
     if state is not None:
-        state = C.require16(state, "state", torch.float32, dev)
+        state = C.require16(state, "state", _F32, dev)
         if tuple(state.shape) != (B, HV, V, K):
             raise ValueError(f"state must be {(B, HV, V, K)}, got {tuple(state.shape)}")
-    _launch(dev, tensors, per_token, dims, scale, state, new_state, None, None, output)
-    return output, new_state
+    return state
 
 
 def run_into(q, k, v, state, log_decay, scale, output, new_state):
     """Destination-passing form of ``run`` (``new_state`` may be ``state``)."""
-    dev, tensors, per_token, dims = _inputs(q, k, v, log_decay)
-    B, H, HV, K, V = dims
-    C.require_out(output, "output", torch.bfloat16, (B, 1, HV, V), dev)
-    C.require_out(new_state, "new_state", torch.float32, (B, HV, V, K), dev)
-    return _run_checked(dev, tensors, per_token, dims, state, scale, output, new_state)
+    inputs = _inputs(q, k, v, log_decay)
+    dev, _, _, _, _, _, B, H, HV, K, V = inputs
+    C.require_out(output, "output", _BF16, (B, 1, HV, V), dev)
+    C.require_out(new_state, "new_state", _F32, (B, HV, V, K), dev)
+    _launch(inputs, scale, _state(state, inputs), new_state, None, None, output)
+    return output, new_state
 
 
 def run(q, k, v, state, log_decay, scale):
     """See the module docstring."""
-    dev, tensors, per_token, dims = _inputs(q, k, v, log_decay)
-    B, H, HV, K, V = dims
-    output = torch.empty((B, 1, HV, V), dtype=torch.bfloat16, device=dev)
-    new_state = torch.empty((B, HV, V, K), dtype=torch.float32, device=dev)
-    return _run_checked(dev, tensors, per_token, dims, state, scale, output, new_state)
+    inputs = _inputs(q, k, v, log_decay)
+    dev, q, k, v, _, _, B, H, HV, K, V = inputs
+    output = torch.empty_like(v)
+    new_state = torch.empty((B, HV, V, K), dtype=_F32, device=dev)
+    _launch(inputs, scale, _state(state, inputs), new_state, None, None, output)
+    return output, new_state
 
 
 def run_pool(q, k, v, initial_state, initial_state_indices, log_decay, scale=None, output=None,
              output_state_indices=None):
     """See the module docstring."""
-    dev, tensors, per_token, dims = _inputs(q, k, v, log_decay)
-    B, H, HV, K, V = dims
-    pool = C.require_pool(initial_state, HV, V, K, dev)
+    inputs = _inputs(q, k, v, log_decay)
+    dev, q, k, v, _, _, B, H, HV, K, V = inputs
+    C.require_pool(initial_state, HV, V, K, dev)
     idx = C.require_indices(initial_state_indices, B, dev, "initial_state_indices")
     out_idx = None if output_state_indices is None else \
         C.require_indices(output_state_indices, B, dev, "output_state_indices", like=idx)
     if output is None:
-        output = torch.empty((B, 1, HV, V), dtype=torch.bfloat16, device=dev)
+        output = torch.empty_like(v)
     else:
-        C.require_out(output, "output", torch.bfloat16, (B, 1, HV, V), dev)
-    _launch(dev, tensors, per_token, dims, scale, pool, pool, idx, out_idx, output)
+        C.require_out(output, "output", _BF16, (B, 1, HV, V), dev)
+    _launch(inputs, scale, initial_state, initial_state, idx, out_idx, output)
     return output, initial_state

@@ -28,56 +28,76 @@ from . import _common as C
 from ._lib import check, lib
 
 
+_BF16, _F32 = torch.bfloat16, torch.float32
+_MIN_SEGMENT = 256  # calls of up to this many tokens need no workspace
+
+
 def _inputs(q, k, v, state, log_decay, cu_seqlens):
     dev = C.cuda_device_of(q)
-    bf = torch.bfloat16
-    q, k, v = C.require16(q, "q", bf, dev), C.require16(k, "k", bf, dev), C.require16(v, "v", bf, dev)
-    if q.dim() != 3:
-        raise ValueError(f"q must be [T, H, K], got {tuple(q.shape)}")
-    T = q.shape[0]
-    H, HV, K, V = C.require_heads(q, k, v, (T,))
-    g, per_token = C.require_log_decay(log_decay, (T,), HV, dev)
+    ready = C.ready
+    if not ready(q, _BF16, dev):
+        q = C.require16(q, "q", _BF16, dev)
+    if not ready(k, _BF16, dev):
+        k = C.require16(k, "k", _BF16, dev)
+    if not ready(v, _BF16, dev):
+        v = C.require16(v, "v", _BF16, dev)
+    qs, vs = q.shape, v.shape
+    if len(qs) != 3:
+        raise ValueError(f"q must be [T, H, K], got {tuple(qs)}")
+    T, H, K = qs
+    if k.shape != qs or len(vs) != 3 or vs[0] != T or H < 1 or vs[1] < 1:
+        C.require_heads(q, k, v, (T,))
+    _, HV, V = vs
+    if ready(log_decay, _F32, dev) and log_decay.shape == (T, HV):
+        g, per_token = log_decay, 1
+    else:
+        g, per_token = C.require_log_decay(log_decay, (T,), HV, dev)
     if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise TypeError("cu_seqlens must be an int32 or int64 tensor")
     if cu_seqlens.device != dev:
         raise ValueError(f"cu_seqlens is on {cu_seqlens.device}, expected {dev}")
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be a 1-d tensor of N + 1 offsets")
-    N = cu_seqlens.numel() - 1
+    N = cu_seqlens.shape[0] - 1
     if state is not None:
-        state = C.require16(state, "state", torch.float32, dev, 32)
-        if tuple(state.shape) != (N, HV, V, K):
+        if not ready(state, _F32, dev):
+            state = C.require16(state, "state", _F32, dev, 32)
+        if state.shape != (N, HV, V, K):
             raise ValueError(f"state must be {(N, HV, V, K)}, got {tuple(state.shape)}")
-    return dev, (q, k, v, state, g, cu_seqlens.contiguous()), per_token, (T, N, H, HV, K, V)
+    return dev, q, k, v, state, g, per_token, cu_seqlens.contiguous(), T, N, H, HV, K, V
 
 
-def _run_checked(dev, tensors, per_token, dims, scale, output, new_state):
-    q, k, v, state, g, cu = tensors
-    T, N, H, HV, K, V = dims
-    with C.on_device(dev):
-        nbytes = lib().gdn_decay_prefill_workspace_bytes(N, T, HV)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        st = lib().gdn_decay_prefill_fwd(
-            C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(state), C.ptr(g), per_token, C.ptr(cu),
-            int(cu.dtype == torch.int64), N, T, C.normalize_scale(scale, K), H, HV, K, V, C.ptr(output),
-            C.ptr(new_state), C.ptr(ws), nbytes, C.stream_handle(dev))
-    check("gdn_decay_prefill_fwd", st)
-    return output, new_state
+def _launch(inputs, scale, output, new_state):
+    dev, q, k, v, state, g, per_token, cu, T, N, H, HV, K, V = inputs
+    if dev.index != C.current_device():
+        with torch.cuda.device(dev):
+            return _launch(inputs, scale, output, new_state)
+    L = lib()
+    nbytes = L.gdn_decay_prefill_workspace_bytes(N, T, HV) if T > _MIN_SEGMENT else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    st = L.gdn_decay_prefill_fwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if state is None else state.data_ptr(), g.data_ptr(), per_token,
+        cu.data_ptr(), cu.dtype is torch.int64, N, T, C.normalize_scale(scale, K), H, HV, K, V, output.data_ptr(),
+        new_state.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes, C.stream_handle(dev))
+    if st:
+        check("gdn_decay_prefill_fwd", st)
 
 
 def run_into(q, k, v, state, log_decay, cu_seqlens, scale, output, new_state):
     """Destination-passing form of ``run`` (``new_state`` may be ``state``)."""
-    dev, tensors, per_token, dims = _inputs(q, k, v, state, log_decay, cu_seqlens)
-    T, N, H, HV, K, V = dims
-    C.require_out(output, "output", torch.bfloat16, (T, HV, V), dev)
-    C.require_out(new_state, "new_state", torch.float32, (N, HV, V, K), dev)
-    return _run_checked(dev, tensors, per_token, dims, scale, output, new_state)
+    inputs = _inputs(q, k, v, state, log_decay, cu_seqlens)
+    dev, _, _, _, _, _, _, _, T, N, H, HV, K, V = inputs
+    C.require_out(output, "output", _BF16, (T, HV, V), dev)
+    C.require_out(new_state, "new_state", _F32, (N, HV, V, K), dev)
+    _launch(inputs, scale, output, new_state)
+    return output, new_state
 
 
 def run(q, k, v, state, log_decay, cu_seqlens, scale):
     """See the module docstring."""
-    dev, tensors, per_token, dims = _inputs(q, k, v, state, log_decay, cu_seqlens)
-    T, N, H, HV, K, V = dims
-    output = torch.empty((T, HV, V), dtype=torch.bfloat16, device=dev)
-    new_state = torch.empty((N, HV, V, K), dtype=torch.float32, device=dev)
-    return _run_checked(dev, tensors, per_token, dims, scale, output, new_state)
+    inputs = _inputs(q, k, v, state, log_decay, cu_seqlens)
+    dev, _, _, v, state, _, _, _, T, N, H, HV, K, V = inputs
+    output = torch.empty_like(v)
+    new_state = torch.empty((N, HV, V, K), dtype=_F32, device=dev)
+    _launch(inputs, scale, output, new_state)
+    return output, new_state

@@ -40,61 +40,88 @@ from ._lib import check, lib
 MAX_NODES = 64  # GDN_DECAY_TREE_MAX (include/gdn_decay_b200.h)
 
 
+_BF16, _F32 = torch.bfloat16, torch.float32
+
+
 def _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay):
     dev = C.cuda_device_of(k)
-    bf = torch.bfloat16
-    k, v = C.require16(k, "k", bf, dev), C.require16(v, "v", bf, dev)
-    if q is not None:
-        q = C.require16(q, "q", bf, dev)
-    if k.dim() != 4:
-        raise ValueError(f"k must be [B, T, H, K], got {tuple(k.shape)}")
-    B, T = k.shape[:2]
-    H, HV, K, V = C.require_heads(q, k, v, (B, T))
+    ready = C.ready
+    if q is not None and not ready(q, _BF16, dev):
+        q = C.require16(q, "q", _BF16, dev)
+    if not ready(k, _BF16, dev):
+        k = C.require16(k, "k", _BF16, dev)
+    if not ready(v, _BF16, dev):
+        v = C.require16(v, "v", _BF16, dev)
+    ks, vs = k.shape, v.shape
+    if len(ks) != 4:
+        raise ValueError(f"k must be [B, T, H, K], got {tuple(ks)}")
+    B, T, H, K = ks
+    if (q is not None and q.shape != ks) or len(vs) != 4 or vs[:2] != ks[:2] or H < 1 or vs[2] < 1:
+        C.require_heads(q, k, v, (B, T))
+    _, _, HV, V = vs
     if T > MAX_NODES:
         raise ValueError(f"a tree has at most {MAX_NODES} nodes, got {T}")
-    g, per_token = C.require_log_decay(log_decay, (B, T), HV, dev)
-    pool = C.require_pool(initial_state, HV, V, K, dev)
+    if ready(log_decay, _F32, dev) and log_decay.shape == (HV,):
+        g, per_token = log_decay, 0
+    else:
+        g, per_token = C.require_log_decay(log_decay, (B, T), HV, dev)
+    C.require_pool(initial_state, HV, V, K, dev)
     idx = C.require_indices(initial_state_indices, B, dev, "initial_state_indices")
-    parents = C.require(parents, "parents", torch.int32, dev)
-    if tuple(parents.shape) != (B, T):
+    if not ready(parents, torch.int32, dev):
+        parents = C.require(parents, "parents", torch.int32, dev)
+    if parents.shape != (B, T):
         raise ValueError(f"parents must be {(B, T)}, got {tuple(parents.shape)}")
-    return dev, (q, k, v, pool, idx, parents, g), per_token, (B, T, H, HV, K, V)
+    return dev, q, k, v, initial_state, idx, parents, g, per_token, B, T, H, HV, K, V
 
 
 def run(q, k, v, initial_state, initial_state_indices, parents, log_decay, scale=None, output=None):
     """See the module docstring."""
     if q is None:
         raise TypeError("q must be a torch.Tensor, got NoneType")
-    dev, tensors, per_token, dims = _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay)
-    q, k, v, pool, idx, parents, g = tensors
-    B, T, H, HV, K, V = dims
+    inputs = _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay)
     if output is None:
-        output = torch.empty((B, T, HV, V), dtype=torch.bfloat16, device=dev)
+        output = torch.empty_like(inputs[3])
     else:
-        C.require_out(output, "output", torch.bfloat16, (B, T, HV, V), dev)
-    with C.on_device(dev):
-        st = lib().gdn_decay_verify_fwd(
-            C.ptr(q), C.ptr(k), C.ptr(v), C.ptr(pool), int(pool.dtype == torch.bfloat16), C.ptr(idx),
-            int(idx.dtype == torch.int64), C.ptr(parents), C.ptr(g), per_token, C.normalize_scale(scale, K),
-            B, T, H, HV, K, V, pool.shape[0], C.ptr(output), C.stream_handle(dev))
-    check("gdn_decay_verify_fwd", st)
+        C.require_out(output, "output", _BF16, inputs[3].shape, inputs[0])
+    return _run(inputs, scale, output)
+
+
+def _run(inputs, scale, output):
+    dev, q, k, v, pool, idx, parents, g, per_token, B, T, H, HV, K, V = inputs
+    if dev.index != C.current_device():
+        with torch.cuda.device(dev):
+            return _run(inputs, scale, output)
+    st = lib().gdn_decay_verify_fwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), pool.data_ptr(), pool.dtype is _BF16, idx.data_ptr(),
+        idx.dtype is torch.int64, parents.data_ptr(), g.data_ptr(), per_token, C.normalize_scale(scale, K),
+        B, T, H, HV, K, V, pool.shape[0], output.data_ptr(), C.stream_handle(dev))
+    if st:
+        check("gdn_decay_verify_fwd", st)
     return output
 
 
 def commit(k, v, initial_state, initial_state_indices, parents, accepted, log_decay, output_state_indices=None):
     """See the module docstring."""
-    dev, tensors, per_token, dims = _inputs(None, k, v, initial_state, initial_state_indices, parents, log_decay)
-    _, k, v, pool, idx, parents, g = tensors
-    B, T, H, HV, K, V = dims
-    accepted = C.require(accepted, "accepted", torch.int32, dev)
-    if tuple(accepted.shape) != (B,):
+    inputs = _inputs(None, k, v, initial_state, initial_state_indices, parents, log_decay)
+    dev, idx, B = inputs[0], inputs[5], inputs[9]
+    if not C.ready(accepted, torch.int32, dev):
+        accepted = C.require(accepted, "accepted", torch.int32, dev)
+    if accepted.shape != (B,):
         raise ValueError(f"accepted must be {(B,)}, got {tuple(accepted.shape)}")
     out_idx = None if output_state_indices is None else \
         C.require_indices(output_state_indices, B, dev, "output_state_indices", like=idx)
-    with C.on_device(dev):
-        st = lib().gdn_decay_commit(
-            C.ptr(k), C.ptr(v), C.ptr(pool), int(pool.dtype == torch.bfloat16), C.ptr(idx), C.ptr(out_idx),
-            int(idx.dtype == torch.int64), C.ptr(parents), C.ptr(accepted), C.ptr(g), per_token,
-            B, T, H, HV, K, V, pool.shape[0], C.stream_handle(dev))
-    check("gdn_decay_commit", st)
+    _commit(inputs, accepted, out_idx)
     return initial_state
+
+
+def _commit(inputs, accepted, out_idx):
+    dev, _, k, v, pool, idx, parents, g, per_token, B, T, H, HV, K, V = inputs
+    if dev.index != C.current_device():
+        with torch.cuda.device(dev):
+            return _commit(inputs, accepted, out_idx)
+    st = lib().gdn_decay_commit(
+        k.data_ptr(), v.data_ptr(), pool.data_ptr(), pool.dtype is _BF16, idx.data_ptr(),
+        0 if out_idx is None else out_idx.data_ptr(), idx.dtype is torch.int64, parents.data_ptr(),
+        accepted.data_ptr(), g.data_ptr(), per_token, B, T, H, HV, K, V, pool.shape[0], C.stream_handle(dev))
+    if st:
+        check("gdn_decay_commit", st)

@@ -24,6 +24,8 @@ pool's device, no host synchronisation.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _common as C
@@ -51,46 +53,61 @@ def _check(pool, slots, codes, exponents, cache_slots):
         raise TypeError(f"pool must be fp32 or bf16, got {pool.dtype}")
     if not isinstance(codes, torch.Tensor) or codes.dtype not in _CODES:
         raise TypeError("codes must be an int8 or float8_e4m3fn tensor")
-    if pool.dim() < 2 or pool.shape[-1] % GROUP != 0 or not pool.is_contiguous():
-        raise ValueError(f"pool must be contiguous [slots, ..., a multiple of {GROUP}], got {tuple(pool.shape)}")
-    shape = tuple(pool.shape[1:])
-    if codes.dim() != pool.dim() or tuple(codes.shape[1:]) != shape or not codes.is_contiguous() \
-            or codes.device != dev:
-        raise ValueError(f"codes must be contiguous [slots, {', '.join(map(str, shape))}] on {dev}, "
-                         f"got {tuple(codes.shape)} on {codes.device}")
-    C.require_out(exponents, "exponents", torch.uint8, (codes.shape[0], *shape[:-1], shape[-1] // GROUP), dev)
+    shape, cshape = pool.shape, codes.shape
+    if len(shape) < 2 or shape[-1] % GROUP != 0 or not pool.is_contiguous():
+        raise ValueError(f"pool must be contiguous [slots, ..., a multiple of {GROUP}], got {tuple(shape)}")
+    if cshape[1:] != shape[1:] or not codes.is_contiguous() or codes.device != dev:
+        raise ValueError(f"codes must be contiguous [slots, {', '.join(map(str, shape[1:]))}] on {dev}, "
+                         f"got {tuple(cshape)} on {codes.device}")
+    want = (cshape[0], *shape[1:-1], shape[-1] // GROUP)
+    if not (isinstance(exponents, torch.Tensor) and exponents.dtype is torch.uint8 and exponents.shape == want
+            and exponents.is_contiguous() and exponents.device == dev):
+        C.require_out(exponents, "exponents", torch.uint8, want, dev)
     if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
         raise ValueError("slots must be a 1-d int32/int64 tensor")
-    B = slots.numel()
+    B = slots.shape[0]
     slots = C.require_indices(slots, B, dev, "slots")
     cache_slots = C.require_indices(cache_slots, B, dev, "cache_slots", like=slots)
-    elems = 1
-    for n in shape:
-        elems *= n
-    return dev, slots, cache_slots, B, elems
+    return dev, pool, slots, codes, exponents, cache_slots, B, math.prod(shape[1:])
 
 
 def store(pool, slots, codes, exponents, cache_slots):
     """See the module docstring; returns ``(codes, exponents)``."""
-    dev, slots, cache_slots, B, elems = _check(pool, slots, codes, exponents, cache_slots)
-    if elems:
-        with C.on_device(dev):
-            st = lib().gdn_state_cache_store(
-                C.ptr(pool), int(pool.dtype == torch.bfloat16), C.ptr(slots), C.ptr(cache_slots),
-                int(slots.dtype == torch.int64), C.ptr(codes), int(codes.dtype == torch.float8_e4m3fn),
-                C.ptr(exponents), B, elems, pool.shape[0], codes.shape[0], C.stream_handle(dev))
-        check("gdn_state_cache_store", st)
+    _store(_check(pool, slots, codes, exponents, cache_slots))
     return codes, exponents
+
+
+def _store(args):
+    dev, pool, slots, codes, exponents, cache_slots, B, elems = args
+    if not elems:
+        return
+    if dev.index != C.current_device():
+        with torch.cuda.device(dev):
+            return _store(args)
+    st = lib().gdn_state_cache_store(
+        pool.data_ptr(), pool.dtype is torch.bfloat16, slots.data_ptr(), cache_slots.data_ptr(),
+        slots.dtype is torch.int64, codes.data_ptr(), codes.dtype is torch.float8_e4m3fn,
+        exponents.data_ptr(), B, elems, pool.shape[0], codes.shape[0], C.stream_handle(dev))
+    if st:
+        check("gdn_state_cache_store", st)
 
 
 def load(codes, exponents, cache_slots, pool, slots):
     """See the module docstring; returns ``pool``."""
-    dev, slots, cache_slots, B, elems = _check(pool, slots, codes, exponents, cache_slots)
-    if elems:
-        with C.on_device(dev):
-            st = lib().gdn_state_cache_load(
-                C.ptr(codes), int(codes.dtype == torch.float8_e4m3fn), C.ptr(exponents), C.ptr(cache_slots),
-                C.ptr(slots), int(slots.dtype == torch.int64), C.ptr(pool), int(pool.dtype == torch.bfloat16),
-                B, elems, pool.shape[0], codes.shape[0], C.stream_handle(dev))
-        check("gdn_state_cache_load", st)
+    _load(_check(pool, slots, codes, exponents, cache_slots))
     return pool
+
+
+def _load(args):
+    dev, pool, slots, codes, exponents, cache_slots, B, elems = args
+    if not elems:
+        return
+    if dev.index != C.current_device():
+        with torch.cuda.device(dev):
+            return _load(args)
+    st = lib().gdn_state_cache_load(
+        codes.data_ptr(), codes.dtype is torch.float8_e4m3fn, exponents.data_ptr(), cache_slots.data_ptr(),
+        slots.data_ptr(), slots.dtype is torch.int64, pool.data_ptr(), pool.dtype is torch.bfloat16,
+        B, elems, pool.shape[0], codes.shape[0], C.stream_handle(dev))
+    if st:
+        check("gdn_state_cache_load", st)
