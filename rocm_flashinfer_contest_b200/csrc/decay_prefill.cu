@@ -606,12 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             while (ok && it.n < p.N) {
                 const int h = idx % p.HV, hq = h / p.rep, len = it.t1 - it.t0, nch = len > C ? (len + C - 1) / C : 1;
                 idx += gridDim.x;
-                const Item next = find_item(p, finder, idx / p.HV);
                 if (loads) {
-                    if (lane == 0 && next.n < p.N) {  // the next segment's state: into L2
-                        const float* src = source(next, idx % p.HV);
-                        if (src != nullptr) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
-                    }
+                    Item next;
 #pragma unroll 1
                     for (int c = 0; c < nch; ++c, ++m) {
                         const int st = m % L::kStages;
@@ -631,6 +627,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                         __syncwarp();
+                        if (c == 0) {
+                            next = find_item(p, finder, idx / p.HV);
+                            if (lane == 0 && next.n < p.N) {  // the next segment's state: into L2
+                                const float* src = source(next, idx % p.HV);
+                                if (src != nullptr)
+                                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(65536) : "memory");
+                            }
+                        }
                     }
                     it = next;
                     continue;
@@ -650,6 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 float n0, n1;
                 ask(0, n0, n1);
+                const Item next = find_item(p, finder, idx / p.HV);
 #pragma unroll 1
                 for (int c = 0; c < nch; ++c, ++m) {
                     const float g0 = clamp_log_decay(n0), g1 = clamp_log_decay(n1);
