@@ -60,6 +60,22 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
+// The upper halves of two floats, packed: their first 8 significant bits.
+__device__ __forceinline__ uint32_t upper2(float2 x) {
+    return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+}
+// y minus the lower / upper bf16 of t, exactly rounded once (exact where t holds y's
+// leading bits): one mixed-precision fma on the FMA pipe, where masking t out
+// and subtracting it would be an integer operation on the busier ALU pipe.
+__device__ __forceinline__ float2 minus_bf16(float2 y, uint32_t t) {
+    float2 d;
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xbf80;\n\t"
+        "fma.rn.f32.bf16 %0, l, m, %3;\n\tfma.rn.f32.bf16 %1, h, m, %4;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "r"(t), "f"(y.x), "f"(y.y));
+    return d;
+}
+
 template <>
 struct StateRow<true> {
     using Raw = uint4;

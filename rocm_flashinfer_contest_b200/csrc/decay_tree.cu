@@ -5,7 +5,13 @@
 // (node t included) and j <= t meaning "j is on node t's path":
 //   o_t = scale * ( e^{c_t} S q_t + sum_{j <= t} e^{c_t - c_j} (q_t . k_j) v_j )
 //   S'  = e^{c_a} S + sum_{j <= a} e^{c_a - c_j} v_j k_j^T      (a: accepted)
+#include <cuda.h>
+
+#include <atomic>
+#include <mutex>
+
 #include "decay_common.cuh"
+#include "umma.cuh"
 
 namespace gdn {
 namespace decay {
@@ -13,16 +19,20 @@ namespace decay {
 constexpr int kTreeMax = GDN_DECAY_TREE_MAX;
 
 // ---------------------------------------------------------------------------
-// Verification: one CTA per entry and v-head, 8 warps of 16 state rows each.
+// Verification: persistent CTAs of 8 warps, one entry's v-head after the other,
+// two CTAs per SM up to 32 nodes.
 //
-// The state (64 KiB in fp32) is the traffic: it is read once, straight into
-// the A fragments of warp-level matrix products, o^T[v, t] = S[v, :] . q_t,
-// and q, k, v of the tree (3 T KiB / 4) come through shared memory.  At T = 64 the
-// products are 4.7 M multiply-adds a state (two for each of S q's, S being
-// split as below), about as long on the warp-level tensor path as the state's
-// 64 KiB take from HBM; below that HBM bounds the kernel.  tcgen05 would need
-// the state staged in shared or tensor memory first and a 512-column CTA per
-// SM, for products of at most 64 columns.
+// The state (64 KiB in fp32) is the traffic.  It is read once, by TMA into shared
+// memory while the CTA works on the item before it; a thread then turns half a
+// row into bf16 terms in tensor memory, where they are the A operand of
+// o^T[v, t] = S[v, :] . q_t on tcgen05, and the next state may come.  q, k and v of
+// the tree (3 T / 4 KiB) come through shared memory, asked for as soon as the last
+// item's products are done.  The scores and their product with v are small
+// (T x T x 128) and cut by the paths: warp-level products, which run beside the
+// tcgen05 ones.
+// (64 entries, 32 v-heads, 32 nodes: VERIFY_US.  With S q on warp-level products
+// too, 54 us: two terms of a state times 32 tokens kept that path, an eighth of
+// tcgen05's rate, busy for 3,700 cycles a state, as long as its bytes take.)
 //
 // Precision: q, k, v are bf16 as given.  An fp32 state is split into two bf16
 // terms (hi + lo, off by at most 2^-17 of it) and the decayed scores P likewise,
@@ -39,19 +49,25 @@ struct VerifyParams {
     const __nv_bfloat16* q;
     const __nv_bfloat16* k;
     const __nv_bfloat16* v;
-    const void* pool;
     const void* indices;
     const int* parents;
     const float* log_decay;
     __nv_bfloat16* out;
     float scale;
-    int idx64, per_token, T, Tp, H, HV, rep, pool_size;  // Tp: T rounded up to 16
+    int idx64, per_token, T, Tp, H, HV, rep, pool_size, items;  // Tp: T rounded up to 16; items: entries * HV
 };
 
-constexpr int kQS = 144, kVS = 136, kPS = 72;  // row strides in bf16 elements
+constexpr int kQS = 144, kVS = 136, kPS = 72;  // row strides in bf16 elements of k, of v and the outputs, of P
 
-__host__ __device__ constexpr size_t verify_smem(int Tp) {
-    return (size_t)Tp * 2 * (2 * kQS + kVS + 2 * kPS);
+// tensor-memory columns: S's two terms, o^T
+constexpr uint32_t kTmHi = 0, kTmLo = 64, kTmO = 128;
+
+// Shared memory: the next state in boxes of 128 rows x 128 bytes (128-byte swizzle),
+// then q (a K-major operand, same swizzle), k, v, outputs and the two terms of P.
+constexpr uint32_t kStateBox = 128 * 128;
+__host__ __device__ constexpr uint32_t state_bytes(bool bf16) { return bf16 ? 2 * kStateBox : 4 * kStateBox; }
+__host__ __device__ constexpr size_t verify_smem(int Tp, bool bf16) {
+    return state_bytes(bf16) + (size_t)Tp * 2 * (kDim + kQS + 2 * kVS + 2 * kPS);
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -68,217 +84,302 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
 
-// hi + lo split of a pair: hi = bf16(x), lo = bf16(x - hi).  A value that bf16
-// rounds to infinity, or that is not finite, keeps lo = 0 (inf - inf is NaN).
+// hi + lo split of a pair: hi = the first 8 bits, lo = the rest rounded to bf16.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    hi = pack_bf16(x, y);
-    const float2 h = widen2(hi);
-    const float rx = isinf(h.x) ? 0.f : x - h.x, ry = isinf(h.y) ? 0.f : y - h.y;
-    lo = pack_bf16(rx, ry);
+    hi = upper2(make_float2(x, y));
+    const float2 r = minus_bf16(make_float2(x, y), hi);
+    lo = pack_bf16(r.x, r.y);
+}
+
+// 16 lanes x 16 columns in the fragment layout of a 16 x 8 product's result, two of
+// them: a lane's rows lane / 4 and 8 on, columns 2 (lane % 4) + {0, 1} and 8 on.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t ta, float (&a)[4], float (&b)[4]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3]), "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3])
+        : "r"(ta)
+        : "memory");
 }
 
 template <bool kBf16>
-__global__ void __launch_bounds__(256, 2) decay_verify_kernel(const VerifyParams p) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+__global__ void __launch_bounds__(256, 2)
+    decay_verify_kernel(const VerifyParams p, const __grid_constant__ CUtensorMap m_pool) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ unsigned long long s_path[kTreeMax];  // bit j: j is on the node's path; 0: padding
     __shared__ float s_c[kTreeMax], s_e[kTreeMax];   // c_t and e^{c_t}
     __shared__ int s_up[kTreeMax];
+    __shared__ uint64_t s_full, s_done;
+    __shared__ uint32_t s_tmem;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-    const int b = blockIdx.x / p.HV, h = blockIdx.x % p.HV, hq = h / p.rep, T = p.T, Tp = p.Tp;
-    const size_t row_out = ((size_t)b * T * p.HV + h) * kDim;  // + t * HV * 128
-
-    const long long slot = slot_at(p.indices, p.idx64, b);
-    if (slot < 0 || slot >= p.pool_size) {
-        for (int i = tid; i < T * 16; i += 256)
-            *reinterpret_cast<uint4*>(p.out + row_out + (size_t)(i >> 4) * p.HV * kDim + 8 * (i & 15)) =
-                make_uint4(0, 0, 0, 0);
-        return;
-    }
-
-    // the state, first: rows g and g + 8 of this warp's 16, columns 16 ks + 4 c + {0..3}
-    const size_t srow = ((size_t)slot * p.HV + h) * kDim + 16 * warp + g;
-    float4 sf[kBf16 ? 1 : 8][2];
-    uint2 sb[kBf16 ? 8 : 1][2];
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const size_t at = (srow + 8 * r) * kDim + 16 * ks + 4 * c;
-            if (kBf16)
-                sb[ks][r] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p.pool) + at));
-            else
-                sf[ks][r] = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p.pool) + at));
-        }
-
-    __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(smem_raw);
-    __nv_bfloat16* ks_ = qs + Tp * kQS;
+    const int T = p.T, Tp = p.Tp, mt = Tp / 16;
+    const int quarter = warp & 3, half = warp >> 2;  // tensor-memory lanes; columns of S, and rows of o^T
+    const int rows = 32 * quarter + 16 * half;       // this warp's rows of o^T
+    uint8_t* qs = smem_raw + state_bytes(kBf16);
+    __nv_bfloat16* ks_ = reinterpret_cast<__nv_bfloat16*>(qs + Tp * 256);
     __nv_bfloat16* vs = ks_ + Tp * kQS;
-    __nv_bfloat16* ph = vs + Tp * kVS;
+    __nv_bfloat16* os = vs + Tp * kVS;
+    __nv_bfloat16* ph = os + Tp * kVS;
     __nv_bfloat16* pl = ph + Tp * kPS;
-    for (int i = tid; i < Tp * 16; i += 256) {
-        const int t = i >> 4, x = 8 * (i & 15);
-        if (t < T) {
-            const size_t qk = (((size_t)b * T + t) * p.H + hq) * kDim + x;
-            cp_async16(qs + t * kQS + x, p.q + qk);
+
+    auto slot_of = [&](int item) -> long long {  // -1: padding
+        const long long slot = slot_at(p.indices, p.idx64, item / p.HV);
+        return slot < 0 || slot >= p.pool_size ? -1 : slot;
+    };
+    // one thread asks for the state of an item; padding has none
+    auto ask_state = [&](int item) {
+        if (item >= p.items) return;
+        const long long slot = slot_of(item);
+        if (slot < 0) return;
+        const int number = (int)slot * p.HV + item % p.HV;
+        umma::mbar_arrive_expect_tx(&s_full, state_bytes(kBf16));
+#pragma unroll
+        for (int x = 0; x < (kBf16 ? 2 : 4); ++x)
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                    smem_addr(smem_raw) + x * kStateBox),
+                "l"(reinterpret_cast<uint64_t>(&m_pool)), "r"(x * (kBf16 ? 64 : 32)), "r"(0), "r"(number), "r"(smem_addr(&s_full))
+                : "memory");
+    };
+    // all threads ask for the tree's q, k and v, warp 0 for its parents and log decays (nodes lane, lane + 32)
+    int par[2];
+    float gg[2];
+    auto ask_tree = [&](int item) {
+        if (item >= p.items) return;
+        const int b = item / p.HV, h = item % p.HV, hq = h / p.rep;
+#pragma unroll 1
+        for (int i = tid; i < T * 16; i += 256) {
+            const int t = i >> 4, x = 8 * (i & 15);
+            const size_t qk = (((size_t)b * T + t) * p.H + hq) * kDim + x, vv = (((size_t)b * T + t) * p.HV + h) * kDim + x;
+            cp_async16(qs + umma::kmaj_off(t, x, Tp), p.q + qk);
             cp_async16(ks_ + t * kQS + x, p.k + qk);
-            cp_async16(vs + t * kVS + x, p.v + row_out + (size_t)t * p.HV * kDim + x);
-        } else {
-            *reinterpret_cast<uint4*>(qs + t * kQS + x) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(ks_ + t * kQS + x) = make_uint4(0, 0, 0, 0);
+            cp_async16(vs + t * kVS + x, p.v + vv);
         }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-
-    // Paths and their decays by pointer doubling: after r rounds a node knows the
-    // last 2^r nodes of its path; -1 ends a path, -2 marks padding.
-    if (warp == 0) {
-        unsigned long long m[2];
-        float cc[2];
-        int up[2];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (warp == 0)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = lane + 32 * i;
-            up[i] = -2, cc[i] = 0.f, m[i] = 0ull;
-            if (t < T) {
-                const int par = p.parents[(size_t)b * T + t];
-                up[i] = par < -1 || par >= t ? -2 : par;
-                cc[i] = clamp_log_decay(p.log_decay[p.per_token ? ((size_t)b * T + t) * p.HV + h : h]);
-                m[i] = 1ull << t;
-            }
-            s_up[t] = up[i], s_c[t] = cc[i], s_path[t] = m[i];
-        }
-        __syncwarp();
-        for (int hop = 1; hop < T; hop *= 2) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (up[i] >= 0) {
-                    const int u = up[i];
-                    cc[i] += s_c[u], m[i] |= s_path[u], up[i] = s_up[u];
+            for (int i = 0; i < 2; ++i) {
+                const int t = lane + 32 * i;
+                par[i] = -2, gg[i] = 0.f;
+                if (t < T) {
+                    par[i] = p.parents[(size_t)b * T + t];
+                    gg[i] = p.log_decay[p.per_token ? ((size_t)b * T + t) * p.HV + h : h];
                 }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 2; ++i) s_up[lane + 32 * i] = up[i], s_c[lane + 32 * i] = cc[i], s_path[lane + 32 * i] = m[i];
-            __syncwarp();
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (up[i] != -1) s_path[lane + 32 * i] = 0ull;
-            s_e[lane + 32 * i] = expf(cc[i]);
-        }
+            }
+    };
+
+    if (tid == 0) {
+        umma::mbar_init(&s_full, 1);
+        umma::mbar_init(&s_done, 1);
+        umma::fence_mbar_init();
+        ask_state(blockIdx.x);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (warp == 1) {
+        umma::tmem_alloc(&s_tmem, 256);
+        umma::tmem_relinquish();
+    }
+    // rows T .. Tp - 1 of q, k and v stay zero
+    for (int i = tid; i < (Tp - T) * 16; i += 256) {
+        const int t = T + (i >> 4), x = 8 * (i & 15);
+        *reinterpret_cast<uint4*>(qs + umma::kmaj_off(t, x, Tp)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(ks_ + t * kQS + x) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(vs + t * kVS + x) = make_uint4(0, 0, 0, 0);
+    }
+    ask_tree(blockIdx.x);
+    umma::fence_before_sync();
     __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tm = s_tmem;
+    uint32_t phase = 0;
+    bool lost = false;  // a wait has run out
 
-    // what padding nodes hold must not meet a zero weight as 0 * NaN
-    for (int i = tid; i < Tp * 16; i += 256)
-        if (s_path[i >> 4] == 0ull) *reinterpret_cast<uint4*>(vs + (i >> 4) * kVS + 8 * (i & 15)) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+        const int next = item + gridDim.x;
+        __nv_bfloat16* out = p.out + ((size_t)(item / p.HV) * T * p.HV + item % p.HV) * kDim;  // + t * HV * 128
+        const bool padding = slot_of(item) < 0;
 
-    // P[t, j] = e^{c_t - c_j} (q_t . k_j) on the paths, 0 elsewhere; nodes come after
-    // their parents, so 16 x 8 tiles with every j > t stay out (they are not read either)
-    const int mt = Tp / 16;
-    for (int tile = warp; tile < mt * (mt + 1); tile += 8) {
-        int m = 0, n = tile;  // row block m has 2 (m + 1) column tiles
-        while (n >= 2 * (m + 1)) n -= 2 * (m + 1), ++m;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-            const uint2 a0 = *reinterpret_cast<const uint2*>(qs + (16 * m + g) * kQS + 16 * ks + 4 * c);
-            const uint2 a1 = *reinterpret_cast<const uint2*>(qs + (16 * m + g + 8) * kQS + 16 * ks + 4 * c);
-            const uint2 bb = *reinterpret_cast<const uint2*>(ks_ + (8 * n + g) * kQS + 16 * ks + 4 * c);
-            const uint32_t a[4] = {a0.x, a1.x, a0.y, a1.y};
-            mma16816(acc, a, bb.x, bb.y);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int t = 16 * m + g + 8 * r, j = 8 * n + 2 * c;
-            const unsigned long long path = s_path[t];
-            const float x = path >> j & 1 ? acc[2 * r] * expf(s_c[t] - s_c[j]) : 0.f;
-            const float y = path >> (j + 1) & 1 ? acc[2 * r + 1] * expf(s_c[t] - s_c[j + 1]) : 0.f;
-            uint32_t hi, lo;
-            split2(x, y, hi, lo);
-            *reinterpret_cast<uint32_t*>(ph + t * kPS + j) = hi;
-            *reinterpret_cast<uint32_t*>(pl + t * kPS + j) = lo;
-        }
-    }
-    __syncthreads();
-
-    uint32_t shi[8][4], slo[kBf16 ? 1 : 8][4];
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
-        if (kBf16) {
-            shi[ks][0] = sb[ks][0].x, shi[ks][1] = sb[ks][1].x, shi[ks][2] = sb[ks][0].y, shi[ks][3] = sb[ks][1].y;
-        } else {
-            split2(sf[ks][0].x, sf[ks][0].y, shi[ks][0], slo[ks][0]);
-            split2(sf[ks][1].x, sf[ks][1].y, shi[ks][1], slo[ks][1]);
-            split2(sf[ks][0].z, sf[ks][0].w, shi[ks][2], slo[ks][2]);
-            split2(sf[ks][1].z, sf[ks][1].w, shi[ks][3], slo[ks][3]);
-        }
-    }
-    // o^T rows 16 warp + {g, g + 8}, columns 8 n + 2 c + {0, 1}, two column tiles at a time
-    float o[4][2][4];  // [pair of tiles][tile][fragment]
-    for (int np = 0; np < mt; ++np) {
-        float hi[2][4], lo[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) hi[i][e] = lo[i][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
+        // Paths and their decays by pointer doubling: after r rounds a node knows the
+        // last 2^r nodes of its path; -1 ends a path, -2 marks padding.
+        if (warp == 0) {
+            unsigned long long m[2];
+            float cc[2];
+            int up[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint2 bb = *reinterpret_cast<const uint2*>(qs + (16 * np + 8 * i + g) * kQS + 16 * ks + 4 * c);
-                mma16816(hi[i], shi[ks], bb.x, bb.y);
-                if (!kBf16) mma16816(lo[i], slo[ks], bb.x, bb.y);
+                const int t = lane + 32 * i;
+                up[i] = par[i] < -1 || par[i] >= t || padding ? -2 : par[i];
+                cc[i] = clamp_log_decay(gg[i]);
+                m[i] = t < T ? 1ull << t : 0ull;
+                s_up[t] = up[i], s_c[t] = cc[i], s_path[t] = m[i];
             }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float e0 = s_e[16 * np + 8 * i + 2 * c], e1 = s_e[16 * np + 8 * i + 2 * c + 1];
-            hi[i][0] = (hi[i][0] + lo[i][0]) * e0, hi[i][1] = (hi[i][1] + lo[i][1]) * e1;
-            hi[i][2] = (hi[i][2] + lo[i][2]) * e0, hi[i][3] = (hi[i][3] + lo[i][3]) * e1;
-        }
-        for (int js = 0; js <= np; ++js) {
-            uint32_t a[4];
-            const __nv_bfloat16* src =
-                vs + (16 * js + (lane >> 4) * 8 + (lane & 7)) * kVS + 16 * warp + (lane >> 3 & 1) * 8;
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                         : "r"(smem_addr(src)));
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int at = (16 * np + 8 * i + g) * kPS + 16 * js + 2 * c;
-                const uint32_t* h0 = reinterpret_cast<const uint32_t*>(ph + at);
-                const uint32_t* l0 = reinterpret_cast<const uint32_t*>(pl + at);
-                mma16816(hi[i], a, h0[0], h0[4]);
-                mma16816(hi[i], a, l0[0], l0[4]);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k == np)
+            __syncwarp();
+#pragma unroll 1
+            for (int hop = 1; hop < T; hop *= 2) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
+                    if (up[i] >= 0) {
+                        const int u = up[i];
+                        cc[i] += s_c[u], m[i] |= s_path[u], up[i] = s_up[u];
+                    }
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[k][i][e] = hi[i][e] * p.scale;
+                for (int i = 0; i < 2; ++i)
+                    s_up[lane + 32 * i] = up[i], s_c[lane + 32 * i] = cc[i], s_path[lane + 32 * i] = m[i];
+                __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (up[i] != -1) s_path[lane + 32 * i] = 0ull;
+                s_e[lane + 32 * i] = expf(cc[i]);
+            }
+        }
+        float acc[8][4];  // o^T rows `rows` + {g, g + 8}, tokens 8 n + 2 c + {0, 1}
+        if (!padding) {
+            // half of state row 32 quarter + lane, in bf16 terms, into tensor memory
+            lost = !umma::mbar_wait(&s_full, phase & 1u);
+            __syncwarp();
+            const uint32_t tl = tm + ((uint32_t)(32 * quarter) << 16);
+            const uint8_t* row = smem_raw + (32 * quarter + lane) * 128;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t hi[16], lo[16];
+                if (kBf16) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(row + half * kStateBox + (((4 * x + j) ^ (lane & 7)) << 4));
+                        hi[4 * j] = y.x, hi[4 * j + 1] = y.y, hi[4 * j + 2] = y.z, hi[4 * j + 3] = y.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 y = *reinterpret_cast<const float4*>(row + (2 * half + x) * kStateBox + ((j ^ (lane & 7)) << 4));
+                        split2(y.x, y.y, hi[2 * j], lo[2 * j]);
+                        split2(y.z, y.w, hi[2 * j + 1], lo[2 * j + 1]);
+                    }
+                    umma::tmem_st16_u32_nowait(tl + kTmLo + 32 * half + 16 * x, lo);
+                }
+                umma::tmem_st16_u32_nowait(tl + kTmHi + 32 * half + 16 * x, hi);
+            }
+            umma::tmem_wait_st();
+            umma::fence_before_sync();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        umma::fence_proxy_async_smem();  // q is read, and the state's place written, by the async proxy
+        if (__syncthreads_or(lost)) break;
+        if (tid == 0) ask_state(next);
+
+        if (!padding) {
+            if (warp == 1) {
+                umma::fence_after_sync();
+                if (lane == 0) {
+                    const uint32_t id = umma::idesc_f16(128, Tp, 1, 1, 0, 0);
+                    const uint64_t dq = umma::desc_kmaj(smem_addr(qs), Tp, 0);
+#pragma unroll
+                    for (int term = kBf16 ? 0 : 1; term >= 0; --term)  // the small one first
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks)
+                            umma::mma_f16_ts(tm + kTmO, tm + (term ? kTmLo : kTmHi) + 8 * ks,
+                                             umma::desc_add(dq, (ks >> 2) * Tp * 128 + (ks & 3) * 32), id, ks > 0 || (!kBf16 && term == 0));
+                    umma::mma_commit(&s_done);
+                }
+                __syncwarp();
+            }
+
+            // what padding nodes hold must not meet a zero weight as 0 * NaN
+            for (int i = tid; i < T * 16; i += 256)
+                if (s_path[i >> 4] == 0ull)
+                    *reinterpret_cast<uint4*>(vs + (i >> 4) * kVS + 8 * (i & 15)) = make_uint4(0, 0, 0, 0);
+
+            // P[t, j] = e^{c_t - c_j} (q_t . k_j) on the paths, 0 elsewhere; nodes come after their parents, so
+            // 16 x 8 tiles with every j > t stay out (they are not read either)
+#pragma unroll 1
+            for (int tile = warp; tile < mt * (mt + 1); tile += 8) {
+                int m = 0, n = tile;  // row block m has 2 (m + 1) column tiles
+                while (n >= 2 * (m + 1)) n -= 2 * (m + 1), ++m;
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    const uint2 a0 = *reinterpret_cast<const uint2*>(qs + umma::kmaj_off(16 * m + g, 16 * ks + 4 * c, Tp));
+                    const uint2 a1 = *reinterpret_cast<const uint2*>(qs + umma::kmaj_off(16 * m + g + 8, 16 * ks + 4 * c, Tp));
+                    const uint2 bb = *reinterpret_cast<const uint2*>(ks_ + (8 * n + g) * kQS + 16 * ks + 4 * c);
+                    const uint32_t a[4] = {a0.x, a1.x, a0.y, a1.y};
+                    mma16816(x, a, bb.x, bb.y);
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int t = 16 * m + g + 8 * r, j = 8 * n + 2 * c;
+                    const unsigned long long path = s_path[t];
+                    const float y = path >> j & 1 ? x[2 * r] * expf(s_c[t] - s_c[j]) : 0.f;
+                    const float z = path >> (j + 1) & 1 ? x[2 * r + 1] * expf(s_c[t] - s_c[j + 1]) : 0.f;
+                    uint32_t hi, low;
+                    split2(y, z, hi, low);
+                    *reinterpret_cast<uint32_t*>(ph + t * kPS + j) = hi;
+                    *reinterpret_cast<uint32_t*>(pl + t * kPS + j) = low;
+                }
+            }
+            lost = !umma::mbar_wait(&s_done, phase & 1u);
+            __syncwarp();
+            ++phase;
+            umma::fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < mt) {
+                    tmem_ld_frag(tm + ((uint32_t)rows << 16) + kTmO + 16 * i, acc[2 * i], acc[2 * i + 1]);
+#pragma unroll
+                    for (int n = 2 * i; n < 2 * i + 2; ++n) {
+                        const float2 e = *reinterpret_cast<const float2*>(&s_e[8 * n + 2 * c]);
+                        acc[n][0] *= e.x, acc[n][1] *= e.y, acc[n][2] *= e.x, acc[n][3] *= e.y;
+                    }
+                }
+            umma::fence_before_sync();
+        }
+        if (__syncthreads_or(lost)) break;
+        if (!padding) {
+#pragma unroll 1
+            for (int js = 0; js < mt; ++js) {
+                uint32_t a[4];
+                const __nv_bfloat16* src = vs + (16 * js + (lane >> 4) * 8 + (lane & 7)) * kVS + rows + (lane >> 3 & 1) * 8;
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                             : "r"(smem_addr(src)));
+#pragma unroll
+                for (int term = 0; term < 2; ++term)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+                        if (n < 2 * mt && n >= 2 * js) {
+                            const uint32_t* x = reinterpret_cast<const uint32_t*>((term ? ph : pl) + (8 * n + g) * kPS + 16 * js + 2 * c);
+                            mma16816(acc[n], a, x[0], x[4]);
+                        }
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (n < 2 * mt) {
+                    // turned by stmatrix: 8 tokens x 8 v, 16 bytes of a token's row each
+                    const uint32_t y0 = pack_bf16(p.scale * acc[n][0], p.scale * acc[n][1]);
+                    const uint32_t y1 = pack_bf16(p.scale * acc[n][2], p.scale * acc[n][3]);
+                    asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(
+                                     smem_addr(os + (8 * n + (lane & 7)) * kVS + rows + 8 * (lane >> 3 & 1))),
+                                 "r"(y0), "r"(y1)
+                                 : "memory");
+                }
+        }
+        __syncthreads();
+        ask_tree(next);
+        for (int i = tid; i < T * 16; i += 256) {
+            const int t = i >> 4, x = 8 * (i & 15);
+            uint4 val = *reinterpret_cast<const uint4*>(os + t * kVS + x);
+            if (s_path[t] == 0ull) val = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(out + (size_t)t * p.HV * kDim + x) = val;
+        }
+        __syncthreads();  // the paths are written for the next item
     }
-    // turned through shared memory (q's place) so that a token's row leaves in 16-byte stores
-    __syncthreads();
-#pragma unroll
-    for (int np = 0; np < 4; ++np)
-        if (np < mt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    qs[(16 * np + 8 * i + 2 * c + (e & 1)) * kVS + 16 * warp + g + 8 * (e >> 1)] =
-                        __float2bfloat16_rn(o[np][i][e]);
-    __syncthreads();
-    for (int i = tid; i < T * 16; i += 256) {
-        const int t = i >> 4, x = 8 * (i & 15);
-        uint4 val = *reinterpret_cast<const uint4*>(qs + t * kVS + x);
-        if (s_path[t] == 0ull) val = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(p.out + row_out + (size_t)t * p.HV * kDim + x) = val;
+    if (__syncthreads_or(lost) && tid == 0) {  // given up: what is in flight gets as long again to end before the CTA does
+        umma::mbar_wait(&s_full, phase & 1u);
+        umma::mbar_wait(&s_done, phase & 1u);
     }
+    __syncthreads();
+    if (warp == 1) umma::tmem_dealloc(tm, 256);
 }
 
 // ---------------------------------------------------------------------------
@@ -291,7 +392,8 @@ __global__ void __launch_bounds__(256, 2) decay_verify_kernel(const VerifyParams
 // its way, finds the path's decay (and whether it reaches the cached state); the
 // second adds the nodes, newest first, with the next node's k and v on their way.
 // (With one thread walking for the CTA and k and v staged in shared memory, two
-// barriers and the longer chain of waits made the 64-entry commit 57 us, not 45.)
+// barriers and the longer chain of waits made the 64-entry commit 57 us, not 48.5;
+// 72 registers, 7 CTAs an SM: 8 of 64 registers spill, 51 us.)
 // ---------------------------------------------------------------------------
 
 struct CommitParams {
@@ -307,7 +409,7 @@ struct CommitParams {
 };
 
 template <bool kBf16>
-__global__ void __launch_bounds__(128) decay_commit_kernel(const CommitParams p) {
+__global__ void __launch_bounds__(128, 7) decay_commit_kernel(const CommitParams p) {
     using Row = StateRow<kBf16>;
     constexpr int kRows = 32, kPasses = kRows / 16, kBlocks = kDim / kRows;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & 7;
@@ -347,15 +449,7 @@ __global__ void __launch_bounds__(128) decay_commit_kernel(const CommitParams p)
         const float x = __shfl_sync(0xffffffffu, g[0], t & 31), y = __shfl_sync(0xffffffffu, g[1], t & 31);
         return t < 32 ? x : y;
     };
-    float all = 0.f;
-    int end = some ? last : -2;
-    while (end >= 0) {
-        all += decay_of(end);
-        end = parent_of(end);
-    }
-    const bool path = some && end == -1;  // else padding lies on the path: nothing is accepted
-    if (!path && oslot == slot) return;
-
+    // the newest node's k and v come with the state
     uint2 kn[4];
     float vn[kPasses];
     auto fetch = [&](int t) {
@@ -365,7 +459,16 @@ __global__ void __launch_bounds__(128) decay_commit_kernel(const CommitParams p)
 #pragma unroll
         for (int ps = 0; ps < kPasses; ++ps) vn[ps] = bf16_to_f32(p.v[(((size_t)b * T + t) * p.HV + h) * kDim + row + 4 * ps]);
     };
-    if (path) fetch(last);
+    if (some) fetch(last);
+    float all = 0.f;
+    int end = some ? last : -2;
+    while (end >= 0) {
+        all += decay_of(end);
+        end = parent_of(end);
+    }
+    const bool path = some && end == -1;  // else padding lies on the path: nothing is accepted
+    if (!path && oslot == slot) return;
+
     const float a = path ? expf(all) : 1.f;
     float4 s[kPasses][4];
 #pragma unroll
@@ -407,21 +510,69 @@ static int check_tree(int state_bf16, int idx64, int per_token, int B, int T, in
     return GDN_OK;
 }
 
+// The driver's tensor-map encoder, looked up through the runtime once (no
+// link-time dependency on the driver library).
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn tree_encode_fn() {
+    static std::once_flag once;
+    static EncodeFn fn = nullptr;
+    std::call_once(once, []() {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(ptr);
+    });
+    return fn;
+}
+
 template <bool kBf16>
-static int launch_verify(const VerifyParams& p, int B, cudaStream_t st) {
-    const size_t smem = verify_smem(p.Tp);
-    // above 48 KiB with the kernel's static arrays: set on each such call, for the current device
-    if (smem > 40 * 1024 &&
-        cudaFuncSetAttribute(decay_verify_kernel<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)verify_smem(kTreeMax)) != cudaSuccess) {
-        cudaGetLastError();
+static int launch_verify(const VerifyParams& p, const void* pool, cudaStream_t st) {
+    // the pool, [states, 128, 128], in boxes of 128 rows x 128 bytes
+    const EncodeFn encode = tree_encode_fn();
+    if (encode == nullptr) return GDN_ERR_CUDA;
+    CUtensorMap map{};
+    const cuuint64_t el = kBf16 ? 2 : 4, n = (cuuint64_t)(p.pool_size > 0 ? p.pool_size : 1) * p.HV;
+    const cuuint64_t dims[3] = {(cuuint64_t)kDim, (cuuint64_t)kDim, n}, strides[2] = {kDim * el, kDim * kDim * el};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / el), (cuuint32_t)kDim, 1u}, estr[3] = {1u, 1u, 1u};
+    if (encode(&map, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(pool),
+               dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return GDN_ERR_CUDA;
+    const size_t smem = verify_smem(p.Tp, kBf16);
+    static std::atomic<unsigned long long> done{0};  // the kernel's attribute, once per device (again after a failure)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return GDN_ERR_CUDA;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev >= 64 || !(done.load() & bit)) {
+        if (cudaFuncSetAttribute(decay_verify_kernel<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)verify_smem(kTreeMax, kBf16)) != cudaSuccess) {
+            cudaGetLastError();
+            return GDN_ERR_CUDA;
+        }
+        if (dev < 64) done.fetch_or(bit);
     }
-    decay_verify_kernel<kBf16><<<(unsigned)(B * p.HV), 256, smem, st>>>(p);
+    const int per_sm = 2 * (smem + 4096) <= 227 * 1024 ? 2 : 1, most = per_sm * 148;
+    decay_verify_kernel<kBf16><<<p.items < most ? p.items : most, 256, smem, st>>>(p, map);
     return gdn_launch_status();
 }
 
+static int tree_status_bits(bool clear) {
+    unsigned int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(v)) != cudaSuccess) return -1;
+    if (clear && v) {
+        const unsigned int z = 0;
+        if (cudaMemcpyToSymbol(g_device_status, &z, sizeof(z)) != cudaSuccess) return -1;
+    }
+    return (int)v;
+}
+
 }  // namespace decay
+
+int decay_tree_status(bool clear) { return decay::tree_status_bits(clear); }
+
 }  // namespace gdn
 
 extern "C" int gdn_decay_verify_fwd(const void* q, const void* k, const void* v, const void* pool, int state_bf16,
@@ -431,6 +582,7 @@ extern "C" int gdn_decay_verify_fwd(const void* q, const void* k, const void* v,
     using namespace gdn::decay;
     const int bad = check_tree(state_bf16, indices_int64, decay_per_token, B, T, H, HV, K, V, pool_size);
     if (bad) return bad;
+    if ((long long)pool_size * HV > 0x7fffffffll) return GDN_ERR_UNSUPPORTED;  // state number
     if (B == 0 || T == 0) return GDN_OK;
     if (!q || !k || !v || !pool || !indices || !parents || !log_decay || !out) return GDN_ERR_INVALID;
     if (!gdn_aligned(q, 16) || !gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(out, 16) ||
@@ -441,7 +593,6 @@ extern "C" int gdn_decay_verify_fwd(const void* q, const void* k, const void* v,
     p.q = static_cast<const __nv_bfloat16*>(q);
     p.k = static_cast<const __nv_bfloat16*>(k);
     p.v = static_cast<const __nv_bfloat16*>(v);
-    p.pool = pool;
     p.indices = indices;
     p.parents = parents;
     p.log_decay = log_decay;
@@ -456,7 +607,8 @@ extern "C" int gdn_decay_verify_fwd(const void* q, const void* k, const void* v,
     p.rep = HV / H;
     p.pool_size = pool_size;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return state_bf16 ? launch_verify<true>(p, B, st) : launch_verify<false>(p, B, st);
+    p.items = B * HV;
+    return state_bf16 ? launch_verify<true>(p, pool, st) : launch_verify<false>(p, pool, st);
 }
 
 extern "C" int gdn_decay_commit(const void* k, const void* v, void* pool, int state_bf16, const void* indices,

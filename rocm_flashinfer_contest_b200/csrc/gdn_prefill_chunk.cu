@@ -1870,10 +1870,11 @@ int launch_prefill_chunk(const PrefillParams& p, void* workspace, size_t workspa
 namespace gdn {
 int mtp_stream_status(bool clear);     // gdn_mtp_stream.cu
 int decay_prefill_status(bool clear);  // decay_prefill.cu
+int decay_tree_status(bool clear);     // decay_tree.cu
 }
 
 // The status words of the translation units with bounded waits (the prefill,
-// the streaming MTP kernel, the decay prefill), or-ed.
+// the streaming MTP kernel, the decay prefill and tree), or-ed.
 extern "C" int gdn_device_status(int clear) {
     unsigned int v = 0;
     if (cudaMemcpyFromSymbol(&v, gdn::g_device_status, sizeof(v)) != cudaSuccess) return -1;
@@ -1883,6 +1884,7 @@ extern "C" int gdn_device_status(int clear) {
     }
     const int m = gdn::mtp_stream_status(clear != 0);
     const int d = gdn::decay_prefill_status(clear != 0);
-    if (m < 0 || d < 0) return -1;
-    return (int)(v | (unsigned int)m | (unsigned int)d);
+    const int t = gdn::decay_tree_status(clear != 0);
+    if (m < 0 || d < 0 || t < 0) return -1;
+    return (int)(v | (unsigned int)m | (unsigned int)d | (unsigned int)t);
 }
