@@ -60,6 +60,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
+// True in one lane of a converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t x;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+    return x != 0;
+}
+
 // The upper halves of two floats, packed: their first 8 significant bits.
 __device__ __forceinline__ uint32_t upper2(float2 x) {
     return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);

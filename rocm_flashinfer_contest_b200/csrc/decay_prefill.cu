@@ -230,13 +230,6 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// True in one lane of a converged warp, always the same.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t x;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
-    return x != 0;
-}
-
 // 16 lanes x 32 columns of two accumulators in the fragment layout: x[4 n + 2 r + i]
 // is lane lane / 4 + 8 r, column 8 n + 2 (lane % 4) + i.
 __device__ __forceinline__ void tmem_ld_frag2(uint32_t ta, uint32_t tb, float (&a)[16], float (&b)[16]) {

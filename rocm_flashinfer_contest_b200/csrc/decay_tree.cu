@@ -30,7 +30,7 @@ constexpr int kTreeMax = GDN_DECAY_TREE_MAX;
 // item's products are done.  The scores and their product with v are small
 // (T x T x 128) and cut by the paths: warp-level products, which run beside the
 // tcgen05 ones.
-// (64 entries, 32 v-heads, 32 nodes: VERIFY_US.  With S q on warp-level products
+// (64 entries, 32 v-heads, 32 nodes: 43 us.  With S q on warp-level products
 // too, 54 us: two terms of a state times 32 tokens kept that path, an eighth of
 // tcgen05's rate, busy for 3,700 cycles a state, as long as its bytes take.)
 //
@@ -107,11 +107,11 @@ __global__ void __launch_bounds__(256, 2)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ unsigned long long s_path[kTreeMax];  // bit j: j is on the node's path; 0: padding
     __shared__ float s_c[kTreeMax], s_e[kTreeMax];   // c_t and e^{c_t}
-    __shared__ int s_up[kTreeMax];
+    __shared__ int s_pad;  // some node is padding
     __shared__ uint64_t s_full, s_done;
     __shared__ uint32_t s_tmem;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int T = p.T, Tp = p.Tp, mt = Tp / 16;
     const int quarter = warp & 3, half = warp >> 2;  // tensor-memory lanes; columns of S, and rows of o^T
     const int rows = 32 * quarter + 16 * half;       // this warp's rows of o^T
@@ -199,8 +199,9 @@ __global__ void __launch_bounds__(256, 2)
         __nv_bfloat16* out = p.out + ((size_t)(item / p.HV) * T * p.HV + item % p.HV) * kDim;  // + t * HV * 128
         const bool padding = slot_of(item) < 0;
 
-        // Paths and their decays by pointer doubling: after r rounds a node knows the
-        // last 2^r nodes of its path; -1 ends a path, -2 marks padding.
+        // Paths and their decays by pointer doubling, a lane's two nodes in registers:
+        // after r rounds a node knows the last 2^r nodes of its path; -1 ends a path, -2
+        // marks padding.
         if (warp == 0) {
             unsigned long long m[2];
             float cc[2];
@@ -211,28 +212,40 @@ __global__ void __launch_bounds__(256, 2)
                 up[i] = par[i] < -1 || par[i] >= t || padding ? -2 : par[i];
                 cc[i] = clamp_log_decay(gg[i]);
                 m[i] = t < T ? 1ull << t : 0ull;
-                s_up[t] = up[i], s_c[t] = cc[i], s_path[t] = m[i];
             }
-            __syncwarp();
 #pragma unroll 1
             for (int hop = 1; hop < T; hop *= 2) {
+                unsigned long long mm[2];
+                float dc[2];
+                int uu[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (up[i] >= 0) {
-                        const int u = up[i];
-                        cc[i] += s_c[u], m[i] |= s_path[u], up[i] = s_up[u];
+                for (int i = 0; i < 2; ++i) {  // what node up[i] knows
+                    const int u = up[i] & 31;
+                    mm[i] = __shfl_sync(0xffffffffu, m[0], u);
+                    dc[i] = __shfl_sync(0xffffffffu, cc[0], u);
+                    uu[i] = __shfl_sync(0xffffffffu, up[0], u);
+                    if (T > 32) {
+                        const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], u);
+                        const float d1 = __shfl_sync(0xffffffffu, cc[1], u);
+                        const int u1 = __shfl_sync(0xffffffffu, up[1], u);
+                        if (up[i] >= 32) mm[i] = m1, dc[i] = d1, uu[i] = u1;
                     }
-                __syncwarp();
+                }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    s_up[lane + 32 * i] = up[i], s_c[lane + 32 * i] = cc[i], s_path[lane + 32 * i] = m[i];
-                __syncwarp();
+                    if (up[i] >= 0) cc[i] += dc[i], m[i] |= mm[i], up[i] = uu[i];
             }
+            bool pad = false;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (up[i] != -1) s_path[lane + 32 * i] = 0ull;
-                s_e[lane + 32 * i] = expf(cc[i]);
+                const int t = lane + 32 * i;
+                s_path[t] = up[i] == -1 ? m[i] : 0ull;
+                s_c[t] = cc[i];
+                s_e[t] = expf(cc[i]);
+                pad |= t < T && up[i] != -1;
             }
+            pad = __any_sync(0xffffffffu, pad);
+            if (lane == 0) s_pad = pad;
         }
         float acc[8][4];  // o^T rows `rows` + {g, g + 8}, tokens 8 n + 2 c + {0, 1}
         if (!padding) {
@@ -270,16 +283,16 @@ __global__ void __launch_bounds__(256, 2)
         if (tid == 0) ask_state(next);
 
         if (!padding) {
-            if (warp == 1) {
+            if (warp == 7) {  // the last to have a tile of scores
                 umma::fence_after_sync();
-                if (lane == 0) {
-                    const uint32_t id = umma::idesc_f16(128, Tp, 1, 1, 0, 0);
-                    const uint64_t dq = umma::desc_kmaj(smem_addr(qs), Tp, 0);
+                const uint32_t tu = __shfl_sync(0xffffffffu, tm, 0), id = umma::idesc_f16(128, Tp, 1, 1, 0, 0);
+                const uint64_t dq = umma::desc_kmaj(__shfl_sync(0xffffffffu, smem_addr(qs), 0), Tp, 0);
+                if (elect_one()) {
 #pragma unroll
                     for (int term = kBf16 ? 0 : 1; term >= 0; --term)  // the small one first
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks)
-                            umma::mma_f16_ts(tm + kTmO, tm + (term ? kTmLo : kTmHi) + 8 * ks,
+                            umma::mma_f16_ts(tu + kTmO, tu + (term ? kTmLo : kTmHi) + 8 * ks,
                                              umma::desc_add(dq, (ks >> 2) * Tp * 128 + (ks & 3) * 32), id, ks > 0 || (!kBf16 && term == 0));
                     umma::mma_commit(&s_done);
                 }
@@ -287,7 +300,7 @@ __global__ void __launch_bounds__(256, 2)
             }
 
             // what padding nodes hold must not meet a zero weight as 0 * NaN
-            for (int i = tid; i < T * 16; i += 256)
+            for (int i = tid; s_pad && i < T * 16; i += 256)
                 if (s_path[i >> 4] == 0ull)
                     *reinterpret_cast<uint4*>(vs + (i >> 4) * kVS + 8 * (i & 15)) = make_uint4(0, 0, 0, 0);
 
@@ -297,15 +310,17 @@ __global__ void __launch_bounds__(256, 2)
             for (int tile = warp; tile < mt * (mt + 1); tile += 8) {
                 int m = 0, n = tile;  // row block m has 2 (m + 1) column tiles
                 while (n >= 2 * (m + 1)) n -= 2 * (m + 1), ++m;
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, x2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
                     const uint2 a0 = *reinterpret_cast<const uint2*>(qs + umma::kmaj_off(16 * m + g, 16 * ks + 4 * c, Tp));
                     const uint2 a1 = *reinterpret_cast<const uint2*>(qs + umma::kmaj_off(16 * m + g + 8, 16 * ks + 4 * c, Tp));
                     const uint2 bb = *reinterpret_cast<const uint2*>(ks_ + (8 * n + g) * kQS + 16 * ks + 4 * c);
                     const uint32_t a[4] = {a0.x, a1.x, a0.y, a1.y};
-                    mma16816(x, a, bb.x, bb.y);
+                    mma16816(ks & 1 ? x2 : x, a, bb.x, bb.y);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] += x2[e];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int t = 16 * m + g + 8 * r, j = 8 * n + 2 * c;
