@@ -256,6 +256,12 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
+// The launches of a call overlap: one may start its CTAs once every CTA of the one
+// before it has started, and waits for that one's end and its writes where it
+// needs them.
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <int kN>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kN));
@@ -307,10 +313,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after_sync();
     const uint32_t tm = B.tmem;
     const bool work = B.none == 0;
+    let_next_launch_start();
 
     if (warp < 8) {
         // ---- state: row v of 128, half the columns, in registers ----
         more_registers<kRegsState>();
+        wait_for_last_launch();  // states
         const int half = warp >> 2, v0 = 32 * (warp & 3), v = v0 + lane;
         const uint32_t tl = tm + ((uint32_t)v0 << 16);
         float s[64];
@@ -450,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fewer_registers<kRegsOut>();
         {
             // ---- outputs ----
+            wait_for_last_launch();
             const int wq = warp - 16;
             const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
             const size_t step = (size_t)p.HV * kDim;
@@ -786,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     if (warp == 26 && lane == 0)
-        // ---- finished states on their way out ----
+        // ---- finished states on their way out (of the state warps, which have waited for the last launch) ----
         for (int i = 0; work; ++i) {
             if (!wait_one(B, &B.st_full, i)) break;
             const int out = B.st_out, m = B.st_m, final = B.st_final, st = m % L::kStages;
@@ -818,6 +827,7 @@ __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillP
     const int part = blockIdx.x & 15, j = (blockIdx.x >> 4) / p.HV, h = (blockIdx.x >> 4) % p.HV, lane = threadIdx.x & 31;
     int nseg = 0, ws = 0, before = 0;
     bool found = false;
+    let_next_launch_start();
 #pragma unroll 1
     for (int base = 0; base < p.N && !found; base += 32) {
         int t0, len, k = 0;
@@ -841,6 +851,7 @@ __global__ void __launch_bounds__(256) decay_prefill_carry_kernel(const PrefillP
             before += __popc(long3);
         }
     }
+    wait_for_last_launch();  // also where there is nothing to do: the next launch takes this one's end for both
     if (!found || ws + nseg > p.ws_slots) return;
     const size_t at = (size_t)part * 1024 + 4 * threadIdx.x, step = (size_t)p.HV * kDim * kDim;
     float* w = p.ws_state + ((size_t)(ws + 1) * p.HV + h) * kDim * kDim + at;
@@ -1009,16 +1020,34 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         (ws_slots > 0 && !encode_states(&mw, workspace, (long long)ws_slots * HV)))
         return GDN_ERR_CUDA;
     if (!set_attribute()) return GDN_ERR_CUDA;
+    // kernel after kernel, each but the first allowed to start before the one before it ends
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cudaError_t e = cudaSuccess;
     if (ws_slots > 0) {
-        const int items = T / seg * HV;  // at most: segments that another one follows
+        const int inner = T / seg * HV;  // at most: segments that another one follows
         p.first = 1;
-        decay_prefill_kernel<<<items < kSms ? items : kSms, kThreads, L::total, st>>>(p, mq, mk, mv, mw, mo);
+        cfg.gridDim = dim3(inner < kSms ? inner : kSms), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = L::total;
+        e = cudaLaunchKernelEx(&cfg, decay_prefill_kernel, p, mq, mk, mv, mw, mo);
+        cfg.numAttrs = 1;
         // at most T / (2 seg) sequences have more than two segments (any number, if they overlap: the first are taken)
         const int longs = T / 2 / seg;
-        if (longs > 0) decay_prefill_carry_kernel<<<longs * HV * 16, 256, 0, st>>>(p);
+        if (e == cudaSuccess && longs > 0) {
+            cfg.gridDim = dim3(longs * HV * 16), cfg.blockDim = dim3(256), cfg.dynamicSmemBytes = 0;
+            e = cudaLaunchKernelEx(&cfg, decay_prefill_carry_kernel, p);
+        }
         p.first = 0;
     }
     const int items = slots * HV;
-    decay_prefill_kernel<<<items < kSms ? (items > 0 ? items : 1) : kSms, kThreads, L::total, st>>>(p, mq, mk, mv, mn, mo);
+    cfg.gridDim = dim3(items < kSms ? (items > 0 ? items : 1) : kSms), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = L::total;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, decay_prefill_kernel, p, mq, mk, mv, mn, mo);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return GDN_ERR_CUDA;
+    }
     return gdn_launch_status();
 }
