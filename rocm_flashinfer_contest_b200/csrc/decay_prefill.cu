@@ -528,6 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (flags & kFinal) break;
             }
+            if (tid == 512) bulk_wait_read0();  // shared memory is read until then
         }
     } else {
         fewer_registers<kRegsRest>();
