@@ -139,6 +139,14 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 // (a warp reads the 32 tensor-memory lanes of its number modulo 4, hence 25).
 // ---------------------------------------------------------------------------
 
+// What follows a segment in its last chunk's v tile must not meet a zero weight as
+// 0 * NaN: rows from `live` on become zero.
+__device__ __forceinline__ void zero_rows(uint8_t* v, int live, int thread, int threads) {
+#pragma unroll 1
+    for (int i = thread; i < (C - live) * 16; i += threads)
+        *reinterpret_cast<uint4*>(v + (i >> 3 & 1) * (kTile / 2) + (live + (i >> 4)) * 128 + 16 * (i & 7)) = make_uint4(0, 0, 0, 0);
+}
+
 constexpr int kThreads = 28 * 32;
 // Registers per thread by warpgroup; 256 * (112 + 48) + 128 * (72 + 56 + 56) is
 // the 896 * 72 the CTA is launched with.
@@ -414,11 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!wait_bar(B, &B.full[st], m / L::kStages)) break;
             const Gate* gt = gate(m);
             const int live = gt->live, flags = gt->flags;
-            if (live < C)  // what follows the segment must not meet a zero weight as 0 * NaN
-#pragma unroll 1
-                for (int i = x; i < 2 * C * 8; i += 256)
-                    if ((i >> 3 & (C - 1)) >= live)
-                        *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oV + 16 * i) = make_uint4(0, 0, 0, 0);
+            if (live < C) zero_rows(sm + st * L::kStage + L::oV, live, x, 256);  // before U
             uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
             uint8_t* kw = sm + L::kw + 16 * x;
             const int row = x >> 3;  // and row + 32, in two halves of K
@@ -536,6 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             {
                 // ---- decayed scores ----
                 const int wq = warp & 1, i = 32 * wq + lane, jb = warp == 25 ? 1 : 0;
+                const int x96 = 32 * (warp == 25 ? 2 : wq) + lane;
                 const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
 #pragma unroll 1
                 for (int m = 0; work; ++m) {
@@ -544,6 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const Gate* gt = gate(m);
                     const int flags = gt->flags;
                     const float ci = gt->c2[i];
+                    // before P V, which does not wait for the other warps that do this, for U
+                    if (gt->live < C) zero_rows(sm + (m % L::kStages) * L::kStage + L::oV, gt->live, x96, 96);
                     uint8_t* row = sm + L::ps + (m & 1) * L::kP + i * 128;
                     float x[32];
                     tmem_ld32(tl + kColP + 32 * jb, x);
