@@ -985,12 +985,15 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
     const int seg = segment_tokens(T, HV), slots = T / seg + N, ws_slots = N > 0 ? workspace_slots(T, HV) : 0;
     if (((long long)slots + 1) * HV > (1ll << 26)) return GDN_ERR_UNSUPPORTED;  // grid index
     if (N == 0 && T == 0) return GDN_OK;
-    if (!cu_seqlens || (T > 0 && (!q || !k || !v || !out)) || !log_decay || (N > 0 && !new_state))
-        return GDN_ERR_INVALID;
+    if (!cu_seqlens || (T > 0 && (!q || !k || !v || !out || !log_decay)) || (N > 0 && !new_state)) return GDN_ERR_INVALID;
     if (!gdn_aligned(q, 16) || !gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(out, 16) ||
         !gdn_aligned(state, 32) || !gdn_aligned(new_state, 32) || !gdn_aligned(log_decay, 4) ||
         !gdn_aligned(cu_seqlens, cu_seqlens_is_int64 ? 8 : 4))
         return GDN_ERR_ALIGN;
+    // the states are one buffer or two that do not overlap
+    const size_t bytes = (size_t)N * HV * gdn::kDim * gdn::kDim * sizeof(float);
+    const uintptr_t si = (uintptr_t)state, so = (uintptr_t)new_state;
+    if (state && si != so && si < so + bytes && so < si + bytes) return GDN_ERR_INVALID;
     const size_t need = gdn_decay_prefill_workspace_bytes(N, T, HV);
     if (need && (!workspace || workspace_bytes < need)) return GDN_ERR_INVALID;
     if (need && !gdn_aligned(workspace, 32)) return GDN_ERR_ALIGN;
@@ -1014,7 +1017,6 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
     p.first = 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (T == 0) {  // every sequence keeps its state
-        const size_t bytes = (size_t)N * HV * gdn::kDim * gdn::kDim * sizeof(float);
         cudaError_t e = cudaSuccess;
         if (state == nullptr)
             e = cudaMemsetAsync(new_state, 0, bytes, st);

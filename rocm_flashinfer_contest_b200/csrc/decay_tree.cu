@@ -634,7 +634,7 @@ extern "C" int gdn_decay_commit(const void* k, const void* v, void* pool, int st
     const int bad = check_tree(state_bf16, indices_int64, decay_per_token, B, T, H, HV, K, V, pool_size);
     if (bad) return bad;
     if (B == 0) return GDN_OK;
-    if (!pool || !indices || !accepted || !log_decay || (T > 0 && (!k || !v || !parents))) return GDN_ERR_INVALID;
+    if (!pool || !indices || !accepted || (T > 0 && (!k || !v || !parents || !log_decay))) return GDN_ERR_INVALID;
     if (!gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(pool, 16) || !gdn_aligned(log_decay, 4) ||
         !gdn_aligned(parents, 4) || !gdn_aligned(accepted, 4) || !gdn_aligned(indices, indices_int64 ? 8 : 4) ||
         !gdn_aligned(out_indices, indices_int64 ? 8 : 4))

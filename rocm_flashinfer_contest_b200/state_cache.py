@@ -66,6 +66,8 @@ def _check(pool, slots, codes, exponents, cache_slots):
     if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
         raise ValueError("slots must be a 1-d int32/int64 tensor")
     B = slots.shape[0]
+    if max(B, shape[0], cshape[0]) >= 2 ** 31:
+        raise ValueError("fewer than 2^31 pairs and slots are needed")
     slots = C.require_indices(slots, B, dev, "slots")
     cache_slots = C.require_indices(cache_slots, B, dev, "cache_slots", like=slots)
     return dev, pool, slots, codes, exponents, cache_slots, B, math.prod(shape[1:])

@@ -16,7 +16,7 @@ def call(fn, defaults, over):
     return getattr(_lib.lib(), fn)(*d.values())
 
 
-PREFILL = dict(q=32, k=32, v=32, state=32, g=32, per=0, cu=32, cu64=0, N=1, T=64, scale=0.0, H=1, HV=2, K=128, V=128,
+PREFILL = dict(q=32, k=32, v=32, state=None, g=32, per=0, cu=32, cu64=0, N=1, T=64, scale=0.0, H=1, HV=2, K=128, V=128,
                out=32, new=64, ws=None, wsb=0, stream=None)
 
 
@@ -29,7 +29,8 @@ PREFILL = dict(q=32, k=32, v=32, state=32, g=32, per=0, cu=32, cu64=0, N=1, T=64
     (dict(T=4096), INV),                                   # needs a workspace
     (dict(T=4096, ws=64, wsb=1024), INV),                  # too small
     (dict(T=4096, ws=48, wsb=1 << 30), ALI),
-    (dict(N=0, T=0), OK),
+    (dict(state=64, new=96), INV), (dict(state=64 + 65536 * 2 - 32, new=64), INV),   # the states overlap
+    (dict(N=0, T=0), OK), (dict(N=0, T=0, g=None, q=None, k=None, v=None, out=None), OK),
 ])
 def test_prefill_refuses(over, code):
     assert call("gdn_decay_prefill_fwd", PREFILL, over) == code
@@ -166,3 +167,6 @@ def test_python_refuses_on_the_gpu():
             bad()
     with pytest.raises(TypeError):
         state_cache.load(codes.to(torch.int16), exps, idx, pool, idx)
+    many = idx[:1].expand(2 ** 31)
+    with pytest.raises(ValueError, match="2\\^31"):
+        state_cache.load(codes, exps, many, pool, many)

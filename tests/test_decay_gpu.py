@@ -177,6 +177,8 @@ def test_prefill_no_tokens_and_no_sequences():
     assert o.shape == (0, 2, 128) and torch.equal(s, st)
     o, s = decay_prefill.run(e, e, ev, None, g, cu, None)
     assert (s == 0).all()
+    o, s = decay_prefill.run(e, e, ev, st, g.expand(0, 2), cu, None)   # a decay for each of no tokens
+    assert torch.equal(s, st)
     q, v = rnd(gen, 9, 1, 128), rnd(gen, 9, 2, 128)
     o, s = decay_prefill.run(q, q, v, None, g, cu[:1], None)
     assert (o == 0).all() and s.shape[0] == 0
@@ -487,3 +489,67 @@ def test_graph_of_a_whole_step():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(pool, end) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_at_once_on_streams():
+    """Prefills (of several launches), trees and the delta rule's prefill on streams of their own give what each gives alone."""
+    from rocm_flashinfer_contest_b200 import decay_prefill, decay_tree, gdn_prefill
+    jobs = []
+    for seed in (1, 2):
+        q, k, v, st, g, cu = prefill_case([3000, 65, 0, 700], 2, 8, "token", seed)
+        jobs.append((decay_prefill.run, (q, k, v, st, g, torch.tensor(cu, device="cuda"), None)))
+    for bf16, T in ((False, 9), (True, 40)):
+        gen, pool, idx, q, k, v, g = pool_case(40, T, 2, 8, "token", T, bf16, 44)
+        jobs.append((decay_tree.run, (q, k, v, pool, idx, tree_parents(gen, 40, T, "mixed"), g)))
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = rnd(gen, 900, 4, 128), rnd(gen, 900, 4, 128, s=0.1), rnd(gen, 900, 8, 128)
+    a, b = rnd(gen, 900, 8), rnd(gen, 900, 8)
+    al, dt = rnd(gen, 8, dtype=torch.float32), rnd(gen, 8, dtype=torch.float32)
+    jobs.append((gdn_prefill.run, (q, k, v, None, al, a, dt, b, torch.tensor([0, 900], device="cuda"), None)))
+    flat = lambda x: x if isinstance(x, tuple) else (x,)  # noqa: E731
+    alone = [flat(f(*args)) for f, args in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for (f, args), stream in zip(jobs, streams):
+            with torch.cuda.stream(stream):
+                got.append(flat(f(*args)))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert all(torch.equal(y, z) for y, z in zip(x, alone[i % len(jobs)])), i
+
+
+def test_trees_without_nodes():
+    from rocm_flashinfer_contest_b200 import decay_tree
+    _, pool, idx, q, k, v, g = pool_case(3, 0, 1, 2, "token", 6, False, 6)
+    parents = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    assert decay_tree.run(q, k, v, pool, idx, parents, g).shape == (3, 0, 2, 128)
+    before = pool.clone()
+    dst = torch.tensor([i for i in range(6) if i not in idx.tolist()], device="cuda")
+    decay_tree.commit(k, v, pool, idx, parents, torch.tensor([-1, 0, 5], dtype=torch.int32, device="cuda"), g, dst)
+    assert torch.equal(pool[dst], before[idx]) and torch.equal(pool[idx], before[idx])
+
+
+def test_one_entry_of_many_heads_and_padding_around_it():
+    """A padded batch: one entry in use, first, in the middle or last; more v-heads than CTAs."""
+    from rocm_flashinfer_contest_b200 import decay_decode, decay_tree
+    gen, pool, idx, q, k, v, g = pool_case(3, 2, 1, 200, "token", 8, True, 4)
+    parents = torch.tensor([[-1, 0]] * 3, dtype=torch.int32, device="cuda")
+    full = decay_tree.run(q, k, v, pool, idx, parents, g)
+    one = lambda x: x[:, :1].contiguous()  # noqa: E731
+    end = pool.clone()
+    step_full, _ = decay_decode.run_pool(one(q), one(k), one(v), end, idx, one(g))
+    for i in range(3):
+        some = torch.full_like(idx, -1)
+        some[i] = idx[i]
+        q2, k2, v2, g2 = (torch.where((some < 0).view(-1, *[1] * (x.dim() - 1)), float("nan"), x) for x in (q, k, v, g))
+        o = decay_tree.run(q2, k2, v2, pool, some, parents, g2)
+        mine = pool.clone()
+        d, _ = decay_decode.run_pool(one(q2), one(k2), one(v2), mine, some, one(g2))
+        rest = [j for j in range(3) if j != i]
+        assert torch.equal(o[i], full[i]) and (o[rest] == 0).all()
+        assert torch.equal(d[i], step_full[i]) and (d[rest] == 0).all()
+        assert torch.equal(mine[idx[i]], end[idx[i]])
+        left = [s for s in range(4) if s != int(idx[i])]
+        assert torch.equal(mine[left], pool[left])
