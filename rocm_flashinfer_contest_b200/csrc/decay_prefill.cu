@@ -17,14 +17,16 @@
 // n - 1 times as many CTAs.  Sequences of one segment run in the second launch,
 // which is the only one of a call whose T fits a segment.
 //
-// Products, all on tcgen05 with fp32 accumulators in tensor memory and every
-// operand in the layout in which it arrives (token-major tiles from TMA):
-//   U   [v, k] = V^T (wK)       A: V tile (MN-major), B: scaled K (MN-major)
+// Products, all on tcgen05 with fp32 accumulators in tensor memory:
+//   U   [v, k] = (V w)^T K      A: in tensor memory, B: K tile (MN-major)
 //   P   [i, j] = Q K^T          rows 64..127 of the M = 128 tile are not used
 //   O2^T[v, i] = S Q^T          A: S (bf16) in tensor memory, B: Q tile
-//   O1^T[v, i] = V^T P^T        A: V tile (MN-major), B: decayed P (bf16)
+//   O1^T[v, i] = V^T P^T        A: V^T in tensor memory, B: decayed P (bf16)
+// Tiles arrive token-major by TMA.  V is turned once, by 8 x 8 matrices in
+// registers, and the weights w are put on it there: as an operand in tensor memory
+// it costs shared memory no bandwidth, and K's tile stays as it came.
 //
-// Precision: inputs are bf16.  wK is split into three bf16 terms of 8 bits each
+// Precision: inputs are bf16.  V w is split into three bf16 terms of 8 bits each
 // (exact), so the fp32 state loses nothing beside its accumulation: 8e-8 of it
 // measured, where two terms would give 3e-6.  S and P only meet the output, which
 // is rounded to bf16 itself; they are rounded to bf16 once each, one for each of
@@ -32,6 +34,19 @@
 // rounding alone (measured 0.0023 against 0.0017 of the output; second terms
 // bring it to 0.0017 and cost 12 more products and 1,000 more instructions a
 // chunk).
+//
+// Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 92 us (its 205 MB alone
+// take 31), a chunk every 2,400 cycles in each CTA, of
+// which the products keep the tensor pipe for 1,408 at its full rate.  Half of
+// them have N = 64 and do not reach it, and what lies between two chunks' U (its
+// sums into S, S to bf16, or V's turn) is a chain of waits of 100 cycles and more
+// each, which the pipe waits for.  61 prompts of 82 tokens, 32 v-heads: 107 us,
+// bound by states (64 KiB in and 64 KiB out a prompt and head) that a CTA reads
+// and writes one after the other.  Tried and not kept, at those two: K scaled
+// instead of V, in shared memory (97 and 117 us); that with its lower terms
+// double-buffered (104); V turned by the state warps (100 and 117) or by the output
+// warps (111 and 117); scaling unrolled (96 and 113); the next state by TMA (95 and
+// 120, from 96 and 118).
 #include <cuda.h>
 
 #include <atomic>
@@ -129,7 +144,7 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 // without a break (a segment without tokens is one chunk without tokens).  Each
 // chunk goes through all of its warps:
 //   warps  0..7       state: half a row of S each thread, fp32, in registers
-//   warps  8..15      w_j k_j in three bf16 terms
+//   warps  8..15      V^T, and V^T w in three bf16 terms: 32 v and 32 tokens each warp
 //   warps 16..19      outputs: 32 v each warp, turned on the way to shared memory, rows sent by TMA
 //   warps 20, 21, 25  decayed scores: one row i each thread, 32 columns j
 //   warp  22          TMA loads
@@ -139,18 +154,10 @@ __device__ __forceinline__ Item find_item(const PrefillParams& p, Finder& f, int
 // (a warp reads the 32 tensor-memory lanes of its number modulo 4, hence 25).
 // ---------------------------------------------------------------------------
 
-// What follows a segment in its last chunk's v tile must not meet a zero weight as
-// 0 * NaN: rows from `live` on become zero.
-__device__ __forceinline__ void zero_rows(uint8_t* v, int live, int thread, int threads) {
-#pragma unroll 1
-    for (int i = thread; i < (C - live) * 16; i += threads)
-        *reinterpret_cast<uint4*>(v + (i >> 3 & 1) * (kTile / 2) + (live + (i >> 4)) * 128 + 16 * (i & 7)) = make_uint4(0, 0, 0, 0);
-}
-
 constexpr int kThreads = 28 * 32;
-// Registers per thread by warpgroup; 256 * (112 + 48) + 128 * (72 + 56 + 56) is
+// Registers per thread by warpgroup; 256 * (104 + 64) + 128 * (72 + 48 + 48) is
 // the 896 * 72 the CTA is launched with.
-constexpr int kRegsState = 112, kRegsScale = 48, kRegsOut = 72, kRegsRest = 56;
+constexpr int kRegsState = 104, kRegsScale = 64, kRegsOut = 72, kRegsRest = 48;
 static_assert(256 * (kRegsState + kRegsScale) + 128 * (kRegsOut + 2 * kRegsRest) <= kThreads * 72, "register split");
 
 // Shared memory, in bytes from its start.
@@ -158,11 +165,10 @@ struct L {
     static constexpr int kStages = 3;
     static constexpr int kGates = kStages + 2;  // gates outlive their tiles (read by the state and output warps)
     static constexpr uint32_t kStage = 3 * kTile, oK = kTile, oV = 2 * kTile;  // a stage: q, k, v
-    static constexpr uint32_t kw = kStages * kStage;  // the scaled k's two lower terms (the first takes k's own place)
-    static constexpr uint32_t ps = kw + 2 * kTile;    // two buffers of P
+    static constexpr uint32_t ps = kStages * kStage;  // two buffers of P
     static constexpr uint32_t kP = C * C * 2;
-    static constexpr uint32_t os = ps + 2 * kP;       // a chunk's outputs, [token][v]
-    static constexpr uint32_t tail = os + kTile;      // the last piece of a state on its way out
+    static constexpr uint32_t os = ps + 2 * kP;       // two buffers of a chunk's outputs, [token][v]
+    static constexpr uint32_t tail = os + 2 * kTile;  // the last piece of a state on its way out
     static constexpr uint32_t gates = tail + 8 * 1024;
     static constexpr uint32_t bars = gates + kGates * 832;
     static constexpr uint32_t total = bars + 320;
@@ -189,8 +195,8 @@ struct Gate {
 static_assert(sizeof(Gate) <= 832, "gate slot");
 
 struct Bars {
-    uint64_t full[3], empty[3], pv_done[5], qk_full[2], u_full, u_free, p_read, p_ready[2], p_free[2], kw_ready, s_ready, s_free,
-        o_full[2], o_free[2], st_full, st_free, drain[2];
+    uint64_t full[3], empty[3], pv_done[2], qk_full[2], u_full[2], u_free, p_read, p_ready[2], p_free[2], v_ready[2], s_ready, s_free,
+        o_full, o_free, st_full, st_free, drain[2];
     uint32_t tmem;
     volatile int abort;
     int none;
@@ -198,26 +204,77 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 320, "barrier block");
 
-// Bounded wait: false once it, or any other wait of this CTA, has run out (2^30
-// cycles, about half a second).  Kept short and rolled: the warps run some 25
-// waits, and the kernel's instructions should fit the instruction cache.
+// Bounded wait: false once it has run out (2^30 cycles, about half a second; the
+// CTA is then given up).  Kept short: the warps run some 25 waits, and
+// instructions that do not fit the instruction cache cost more than anything else
+// here (64 KiB of them: 2.7 warps a scheduler waited for instructions at any time,
+// 104 us at 8,192 tokens; 56 KiB, mostly by shorter waits: 0.5 warps, 98 us).
 __device__ __forceinline__ bool wait_one(Bars& B, uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity & 1u)) return true;
-    const int t0 = (int)clock();
-#pragma unroll 1
-    while (!mbar_try_wait(bar, parity & 1u))
-        if (B.abort || (int)clock() - t0 > 1 << 30) {
-            B.abort = 1;
-            return false;
-        }
-    return true;
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 t0, t;\n\t"
+        "mov.u32 t0, %%clock;\n"
+        "AGAIN:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra DONE;\n\t"
+        "mov.u32 t, %%clock;\n\t"
+        "sub.u32 t, t, t0;\n\t"
+        "setp.lt.u32 q, t, 0x40000000;\n\t"
+        "@q bra AGAIN;\n"
+        "DONE:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity & 1u)
+        : "memory");
+    if (!ok) B.abort = 1;
+    return ok != 0;
 }
 // The same for a whole warp, which goes on together.
 __device__ __forceinline__ bool wait_bar(Bars& B, uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, wait_one(B, bar, parity));
 }
+// Waits for one, and says in `too` whether another one's phase is over as well.
+__device__ __forceinline__ bool wait_and_test(Bars& B, uint64_t* bar, uint32_t parity, uint64_t* bar2, uint32_t parity2, bool& too) {
+    const bool ok = wait_one(B, bar, parity);
+    uint32_t over;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(over)
+                 : "r"(smem_u32(bar2)), "r"(parity2 & 1u)
+                 : "memory");
+    too = __all_sync(0xffffffffu, over != 0);
+    return __all_sync(0xffffffffu, ok);
+}
+// Both of two: a wait takes some 100 cycles where there is nothing to wait for, two at once hardly more.
+__device__ __forceinline__ bool wait_two(Bars& B, uint64_t* bar, uint32_t parity, uint64_t* bar2, uint32_t parity2) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 t0, t;\n\t"
+        "mov.u32 t0, %%clock;\n"
+        "AGAIN:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+        "and.pred p, p, q;\n\t"
+        "@p bra DONE;\n\t"
+        "mov.u32 t, %%clock;\n\t"
+        "sub.u32 t, t, t0;\n\t"
+        "setp.lt.u32 q, t, 0x40000000;\n\t"
+        "@q bra AGAIN;\n"
+        "DONE:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity & 1u), "r"(smem_u32(bar2)), "r"(parity2 & 1u)
+        : "memory");
+    if (!ok) B.abort = 1;
+    return __all_sync(0xffffffffu, ok != 0);
+}
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// The same for a whole warp's work, as one arrival: those of 32 lanes take their
+// turns in shared memory (8,192 tokens: 98 -> 94 us).
+__device__ __forceinline__ void arrive_warp(uint64_t* bar, int lane) {
+    __syncwarp();
+    if (lane == 0) arrive(bar);
 }
 
 // One [64 tokens][64] box of a [T, heads, 128] bf16 tensor, 128-byte swizzle.
@@ -238,22 +295,31 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// 16 lanes x 32 columns of two accumulators in the fragment layout: x[4 n + 2 r + i]
-// is lane lane / 4 + 8 r, column 8 n + 2 (lane % 4) + i.
-__device__ __forceinline__ void tmem_ld_frag2(uint32_t ta, uint32_t tb, float (&a)[16], float (&b)[16]) {
-    uint32_t r[32];
+// 16 lanes x 16 columns from the registers of 16 x 8 products' A operands: y[2 n + r] is
+// lane lane / 4 + 8 r, column 4 n + lane % 4.
+__device__ __forceinline__ void tmem_st_frag(uint32_t ta, const uint32_t (&y)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(ta), "r"(y[0]),
+                 "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                 : "memory");
+}
+
+// 16 lanes x 16 columns of two accumulators in the fragment layout, there after the wait: x[8 k + 4 n + 2 r + i]
+// is accumulator k, lane lane / 4 + 8 r, column 8 n + 2 (lane % 4) + i.
+__device__ __forceinline__ void tmem_ld_frag2(uint32_t ta, uint32_t tb, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(ta), "r"(tb)
         : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) a[i] = __uint_as_float(r[i]), b[i] = __uint_as_float(r[16 + i]);
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -262,7 +328,40 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+// Products issued by the lane of a converged warp that has a non-zero `me`.  The
+// low words of descriptors move by bytes >> 4, the high ones do not change.
+__device__ __forceinline__ void mma_ss(uint32_t me, uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], x, y, %6, p;\n\t}" ::"r"(me),
+        "r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t me, uint32_t d, uint32_t a, uint32_t b, uint32_t b_high, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 y, {%3, %4};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], y, %5, p;\n\t}" ::"r"(me),
+        "r"(d), "r"(a), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void commit_to(uint32_t me, uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(me),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// A barrier of n threads, and whether x holds for all of them.
+__device__ __forceinline__ bool bar_all(int id, int n, bool x) {
+    uint32_t y;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\tbar.red.and.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(y)
+                 : "r"(id), "r"(n), "r"((uint32_t)x)
+                 : "memory");
+    return y != 0;
+}
 
 // The launches of a call overlap: one may start its CTAs once every CTA of the one
 // before it has started, and waits for that one's end and its writes where it
@@ -280,7 +379,8 @@ __device__ __forceinline__ void fewer_registers() {
 }
 
 // Tensor-memory columns
-constexpr uint32_t kColU = 0, kColS = 128, kColP = 192, kColO1 = 256, kColO2 = 320;  // (O: a second buffer 128 on)
+constexpr uint32_t kColU = 0, kColS = 128, kColP = 192, kColO1 = 256, kColO2 = 320;
+constexpr uint32_t kColV = 384;  // V^T, and the three terms of V^T w: 32 each
 
 __global__ void __launch_bounds__(kThreads, 1)
     decay_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap mq,
@@ -301,15 +401,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 3; ++i) mbar_init(&B.full[i], 2), mbar_init(&B.empty[i], 2);
 #pragma unroll
-        for (int i = 0; i < 5; ++i) mbar_init(&B.pv_done[i], 1);
-#pragma unroll
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&B.qk_full[i], 1), mbar_init(&B.o_full[i], 1), mbar_init(&B.o_free[i], 128);
-            mbar_init(&B.p_ready[i], 96), mbar_init(&B.p_free[i], 1), mbar_init(&B.drain[i], 1);
+            mbar_init(&B.qk_full[i], 1), mbar_init(&B.pv_done[i], 1), mbar_init(&B.u_full[i], 1);
+            mbar_init(&B.p_ready[i], 3), mbar_init(&B.p_free[i], 1), mbar_init(&B.drain[i], 1), mbar_init(&B.v_ready[i], 8);
         }
-        mbar_init(&B.kw_ready, 256), mbar_init(&B.u_full, 1), mbar_init(&B.u_free, 256);
-        mbar_init(&B.p_read, 96), mbar_init(&B.s_ready, 256), mbar_init(&B.s_free, 1);
-        mbar_init(&B.st_full, 256), mbar_init(&B.st_free, 1);
+        mbar_init(&B.u_free, 8), mbar_init(&B.o_full, 1), mbar_init(&B.o_free, 4);
+        mbar_init(&B.p_read, 3), mbar_init(&B.s_ready, 8), mbar_init(&B.s_free, 1);
+        mbar_init(&B.st_full, 8), mbar_init(&B.st_free, 1);
         fence_mbar_init();
     }
     if (warp == 23) {
@@ -319,8 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-    const uint32_t tm = B.tmem;
-    const bool work = B.none == 0;
+    constexpr uint32_t tm = 0;  // all 512 columns, so they start at the first
+    const bool work = B.none == 0 && B.tmem == tm;
     let_next_launch_start();
 
     if (warp < 8) {
@@ -366,8 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
             fence_before_sync();
-            arrive(&B.s_ready);
-            if (!wait_bar(B, &B.u_full, m)) break;
+            arrive_warp(&B.s_ready, lane);
+            if (!wait_bar(B, &B.u_full[m & 1], m >> 1)) break;
             fence_after_sync();
             const float a = gt->a;
             const int flags = gt->flags, out = gt->out, decay = gt->decay;
@@ -383,13 +481,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             fence_before_sync();
-            arrive(&B.u_free);
+            arrive_warp(&B.u_free, lane);
             first = flags & kLast;
             if (first) {
                 // the state leaves by way of its last chunk's stage (48 KiB) and buffer of P (8 KiB), free after
                 // that chunk's last products, and 8 KiB beside them; the store warp sends it on and gives
                 // them back
-                if (!wait_bar(B, &B.pv_done[m % 5], m / 5)) break;
+                if (!wait_bar(B, &B.s_free, m)) break;
                 if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
                 ++stored;
                 if (out >= 0) {
@@ -408,56 +506,78 @@ __global__ void __launch_bounds__(kThreads, 1)
                     B.st_out = out, B.st_m = m, B.st_final = flags & kFinal;
                     if (decay >= 0) p.ws_decay[decay] = prod;
                 }
-                arrive(&B.st_full);
+                arrive_warp(&B.st_full, lane);
             }
             if (flags & kFinal) break;
         }
     } else if (warp < 16) {
-        // ---- w_j k_j in three terms of 8 bits each (exact), at the same place of three tiles ----
+        // ---- V^T, and V^T w in three terms of 8 bits each (exact), to tensor memory ----
         fewer_registers<kRegsScale>();
-        const int x = tid - 256;
+        const int th = (warp - 8) >> 2, v0 = 32 * (warp & 3);  // 32 tokens, 32 v
+        const uint32_t to = tm + ((uint32_t)v0 << 16) + kColV + 16 * th;
+        const int row = 32 * th + 8 * (lane >> 4) + (lane & 7), piece = v0 / 8 + (lane >> 3 & 1);
+        const uint32_t from = sb + L::oV + (piece >> 3) * (kTile / 2) + row * 128;
 #pragma unroll 1
         for (int m = 0; work; ++m) {
             const int st = m % L::kStages;
             if (!wait_bar(B, &B.full[st], m / L::kStages)) break;
             const Gate* gt = gate(m);
             const int live = gt->live, flags = gt->flags;
-            if (live < C) zero_rows(sm + st * L::kStage + L::oV, live, x, 256);  // before U
-            uint8_t* ks = sm + st * L::kStage + L::oK + 16 * x;
-            uint8_t* kw = sm + L::kw + 16 * x;
-            const int row = x >> 3;  // and row + 32, in two halves of K
-            uint4 k[4];
+            // transposed 8 x 8 matrices come in the layout in which 16 lanes x 4 columns are stored: y[i][2 n + r] is
+            // v 16 i + lane / 4 + 8 r, tokens 8 n + 2 (lane % 4) + {0, 1}
+            uint32_t y[2][8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const uint4*>(ks + 4096 * i);
-            const float w[2] = {gt->w[row], gt->w[row + 32]};
-            if (live < C) {
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (row + 32 * (i & 1) >= live) k[i] = make_uint4(0, 0, 0, 0);
-            }
-            // the lower terms' buffer is free after the last product with it, k's place after its scores
-            if (m > 0 && !wait_bar(B, &B.u_full, m - 1)) break;
-            if (!wait_bar(B, &B.qk_full[m & 1], m >> 1)) break;
+                for (int n = 0; n < 4; n += 2)
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(y[i][2 * n]), "=r"(y[i][2 * n + 1]), "=r"(y[i][2 * n + 2]), "=r"(y[i][2 * n + 3])
+                                 : "r"(from + st * L::kStage + 8 * n * 128 + ((((piece + 2 * i) ^ row) & 7) << 4))
+                                 : "memory");
+            float2 w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t in[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
-                uint32_t t0[4], t1[4], t2[4];
+            for (int n = 0; n < 4; ++n) w[n] = *reinterpret_cast<const float2*>(&gt->w[32 * th + 8 * n + 2 * (lane & 3)]);
+            if (live < C) {  // what follows the segment must not meet a zero weight as 0 * NaN, in neither operand
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float2 y = __fmul2_rn(make_float2(w[i & 1], w[i & 1]), widen2(in[e]));
-                    t0[e] = upper2(y);
-                    y = minus_bf16(y, t0[e]);
-                    t1[e] = upper2(y);
-                    t2[e] = upper2(minus_bf16(y, t1[e]));
+                for (int n = 0; n < 4; ++n) {
+                    const int left = live - (32 * th + 8 * n + 2 * (lane & 3));
+                    const uint32_t keep = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) y[i][2 * n] &= keep, y[i][2 * n + 1] &= keep;
                 }
-                *reinterpret_cast<uint4*>(ks + 4096 * i) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
-                *reinterpret_cast<uint4*>(kw + 4096 * i) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
-                *reinterpret_cast<uint4*>(kw + kTile + 4096 * i) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
+#pragma unroll 1
+                for (int i = tid - 256; i < (C - live) * 16; i += 256)
+                    *reinterpret_cast<uint4*>(sm + st * L::kStage + L::oK + (i >> 3 & 1) * (kTile / 2) + (live + (i >> 4)) * 128 + 16 * (i & 7)) =
+                        make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
             }
-            fence_proxy_async_smem();
-            arrive(&B.kw_ready);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t t0[8], t1[8], t2[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float2 x = __fmul2_rn(w[e >> 1], widen2(y[i][e]));
+                    t0[e] = upper2(x);
+                    x = minus_bf16(x, t0[e]);
+                    t1[e] = upper2(x);
+                    t2[e] = upper2(minus_bf16(x, t1[e]));
+                }
+                if (i == 0) {  // the products with the chunk before are done
+                    if (m > 0 && !wait_two(B, &B.pv_done[(m - 1) & 1], (m - 1) >> 1, &B.u_full[(m - 1) & 1], (m - 1) >> 1)) goto out;
+                    fence_after_sync();
+                }
+                const uint32_t at = to + ((uint32_t)(16 * i) << 16);
+                tmem_st_frag(at, y[i]);
+                tmem_st_frag(at + 32, t0);
+                tmem_st_frag(at + 64, t1);
+                tmem_st_frag(at + 96, t2);
+            }
+            tmem_wait_st();
+            fence_before_sync();
+            arrive_warp(&B.v_ready[m & 1], lane);
             if (flags & kFinal) break;
         }
+    out:;
     } else if (warp < 20) {
         fewer_registers<kRegsOut>();
         {
@@ -477,57 +597,64 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll 1
             for (int m = 0; work; ++m) {
-                if (!wait_bar(B, &B.o_full[m & 1], m >> 1)) break;
+                const bool ok = wait_bar(B, &B.o_full, m);
                 fence_after_sync();
+                const uint32_t os = L::os + (m & 1) * kTile;
                 const Gate* gt = gate(m);
                 const int rows = gt->rows, flags = gt->flags, t = gt->t, h = gt->h;
-                if (tid == 512) bulk_wait_read0();  // the last chunk's rows have left
-                bar_sync(1, 128);
-                // 16 v x 32 tokens at a time, in the fragment layout of 8 x 8 matrices, which stmatrix turns
-                // into 8 tokens x 8 v: 16 bytes of a token's row, at their place under the 128-byte swizzle
+                // 16 v x 16 tokens at a time, the next ones on their way, in the fragment layout of 8 x 8 matrices, which
+                // stmatrix turns into 8 tokens x 8 v: 16 bytes of a token's row, at their place under the 128-byte
+                // swizzle.  Matrices of a store: tokens 0, v 0 and 8; tokens 8, v 0 and 8; this lane's address: token
+                // lane % 8 of matrix lane / 8
+                uint32_t x[2][16];
+                auto load = [&](int b, uint32_t (&r)[16]) {  // v 16 (b & 1), tokens 16 (b >> 1)
+                    const uint32_t at = tl + ((uint32_t)(16 * (b & 1)) << 16) + 16 * (b >> 1);
+                    tmem_ld_frag2(at + kColO1, at + kColO2, r);
+                };
+                load(0, x[0]);
 #pragma unroll 1
-                for (int b = 0; b < 4; ++b) {
-                    const uint32_t at = tl + ((uint32_t)(16 * (b & 1)) << 16) + kColO1 + 128 * (m & 1) + 32 * (b >> 1);
-                    float x1[16], x2[16];
-                    tmem_ld_frag2(at, at + (kColO2 - kColO1), x1, x2);
-                    uint32_t y[8];  // tokens 8 n + 2 (lane % 4) + {0, 1}; v lane / 4 and 8 on
+                for (int c = 0; c < 4; ++c) {
+                    const float2 e[2] = {*reinterpret_cast<const float2*>(&gt->e[16 * c + 2 * (lane & 3)]),
+                                         *reinterpret_cast<const float2*>(&gt->e[16 * c + 8 + 2 * (lane & 3)])};
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float2 e = *reinterpret_cast<const float2*>(&gt->e[32 * (b >> 1) + 8 * n + 2 * (lane & 3)]);
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const float2 z = __ffma2_rn(e, make_float2(x2[4 * n + 2 * r], x2[4 * n + 2 * r + 1]),
-                                                        make_float2(x1[4 * n + 2 * r], x1[4 * n + 2 * r + 1]));
-                            y[2 * n + r] = pack_bf16(z.x, z.y);
+                    for (int b = 0; b < 2; ++b) {
+                        tmem_ld_wait(x[b]);
+                        if (b == 0)
+                            load(2 * c + 1, x[1]);
+                        else if (c < 3)
+                            load(2 * c + 2, x[0]);
+                        else {
+                            fence_before_sync();
+                            arrive_warp(&B.o_free, lane);
                         }
-                    }
-                    // matrices of a store: tokens 8 n, v 0 and 8; tokens 8 (n + 1), v 0 and 8.  This lane's address:
-                    // token lane % 8 of matrix lane / 8
-                    const int chunk = (4 * wq + 2 * (b & 1) + (lane >> 3 & 1)) & 7;
+                        uint32_t y[4];
 #pragma unroll
-                    for (int n = 0; n < 4; n += 2) {
-                        const int t8 = 32 * (b >> 1) + 8 * (n + (lane >> 4)) + (lane & 7);
-                        const uint32_t to = sb + L::os + (wq >> 1) * (kTile / 2) + t8 * 128 + ((chunk ^ (lane & 7)) << 4);
-                        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to),
-                                     "r"(y[2 * n]), "r"(y[2 * n + 1]), "r"(y[2 * n + 2]), "r"(y[2 * n + 3])
+                        for (int n = 0; n < 4; ++n) {  // tokens 8 (n / 2), v 8 (n % 2)
+                            const float2 z = __ffma2_rn(e[n >> 1], make_float2(__uint_as_float(x[b][8 + 2 * n]), __uint_as_float(x[b][9 + 2 * n])),
+                                                        make_float2(__uint_as_float(x[b][2 * n]), __uint_as_float(x[b][2 * n + 1])));
+                            y[n] = pack_bf16(z.x, z.y);
+                        }
+                        const int chunk = (4 * wq + 2 * b + (lane >> 3 & 1)) & 7, t8 = 16 * c + 8 * (lane >> 4) + (lane & 7);
+                        const uint32_t to = sb + os + (wq >> 1) * (kTile / 2) + t8 * 128 + ((chunk ^ (lane & 7)) << 4);
+                        asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(y[0]),
+                                     "r"(y[1]), "r"(y[2]), "r"(y[3])
                                      : "memory");
                     }
                 }
-                fence_before_sync();
-                arrive(&B.o_free[m & 1]);
                 fence_proxy_async_smem();
-                bar_sync(1, 128);
+                if (tid == 512) bulk_wait_read0();  // the rows of the chunk before have left: the other buffer is free
+                if (!bar_all(1, 128, ok)) break;    // (together: none is left at a barrier)
                 if (rows == C) {
                     if (tid == 512) {
-                        tma_store(&m_out, sb + L::os, 0, h, t);
-                        tma_store(&m_out, sb + L::os + kTile / 2, 64, h, t);
+                        tma_store(&m_out, sb + os, 0, h, t);
+                        tma_store(&m_out, sb + os + kTile / 2, 64, h, t);
                     }
                 } else {  // the segment ends in this chunk: its rows only
 #pragma unroll 1
                     for (int i = tid - 512; i < rows * 16; i += 128) {
                         const int r = i >> 4, x = i & 15;
                         *reinterpret_cast<uint4*>(p.out + ((size_t)(t + r) * p.HV + h) * kDim + 8 * x) =
-                            *reinterpret_cast<const uint4*>(sm + L::os + (x >> 3) * (kTile / 2) + r * 128 + (((x & 7) ^ (r & 7)) << 4));
+                            *reinterpret_cast<const uint4*>(sm + os + (x >> 3) * (kTile / 2) + r * 128 + (((x & 7) ^ (r & 7)) << 4));
                     }
                 }
                 if (flags & kFinal) break;
@@ -540,7 +667,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             {
                 // ---- decayed scores ----
                 const int wq = warp & 1, i = 32 * wq + lane, jb = warp == 25 ? 1 : 0;
-                const int x96 = 32 * (warp == 25 ? 2 : wq) + lane;
                 const uint32_t tl = tm + ((uint32_t)(32 * wq) << 16);
 #pragma unroll 1
                 for (int m = 0; work; ++m) {
@@ -549,41 +675,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const Gate* gt = gate(m);
                     const int flags = gt->flags;
                     const float ci = gt->c2[i];
-                    // before P V, which does not wait for the other warps that do this, for U
-                    if (gt->live < C) zero_rows(sm + (m % L::kStages) * L::kStage + L::oV, gt->live, x96, 96);
                     uint8_t* row = sm + L::ps + (m & 1) * L::kP + i * 128;
-                    float x[32];
-                    tmem_ld32(tl + kColP + 32 * jb, x);
-                    fence_before_sync();
-                    arrive(&B.p_read);  // the next chunk's scores may follow
                     // this buffer's last products are those of chunk m - 2
                     if (m > 1 && !wait_bar(B, &B.p_free[m & 1], (m >> 1) - 1)) break;
                     if (warp == 20)  // rows 0 .. 31: nothing in columns 32 .. 63
 #pragma unroll
                         for (int q = 4; q < 8; ++q) *reinterpret_cast<uint4*>(row + ((q ^ (i & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[32 * jb + j]);
-                        const float2 a = __fmul2_rn(make_float2(ex2(ci - cj.x), ex2(ci - cj.y)), make_float2(x[j], x[j + 1]));
-                        const float2 c = __fmul2_rn(make_float2(ex2(ci - cj.z), ex2(ci - cj.w)), make_float2(x[j + 2], x[j + 3]));
-                        x[j] = a.x, x[j + 1] = a.y, x[j + 2] = c.x, x[j + 3] = c.y;
-                    }
-                    if (warp != 21)  // the blocks on the diagonal
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = j <= lane ? x[j] : 0.f;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t t[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 z = __fmul2_rn(make_float2(p.scale, p.scale), make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]));
-                            t[e] = pack_bf16(z.x, z.y);
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        float x[16];
+                        tmem_ld16(tl + kColP + 32 * jb + 16 * c, x);
+                        if (c) {
+                            fence_before_sync();
+                            arrive_warp(&B.p_read, lane);  // the next chunk's scores may follow
                         }
-                        *reinterpret_cast<uint4*>(row + (((4 * jb + q) ^ (i & 7)) << 4)) = make_uint4(t[0], t[1], t[2], t[3]);
+                        const int low = warp == 21 ? 32 : lane - 16 * c;  // the blocks on the diagonal end there
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[32 * jb + 16 * c + j]);
+                            const float2 a = __fmul2_rn(make_float2(ex2(ci - cj.x), ex2(ci - cj.y)), make_float2(x[j], x[j + 1]));
+                            const float2 d = __fmul2_rn(make_float2(ex2(ci - cj.z), ex2(ci - cj.w)), make_float2(x[j + 2], x[j + 3]));
+                            x[j] = j <= low ? a.x : 0.f, x[j + 1] = j + 1 <= low ? a.y : 0.f, x[j + 2] = j + 2 <= low ? d.x : 0.f, x[j + 3] = j + 3 <= low ? d.y : 0.f;
+                        }
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t t[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 z = __fmul2_rn(make_float2(p.scale, p.scale), make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]));
+                                t[e] = pack_bf16(z.x, z.y);
+                            }
+                            *reinterpret_cast<uint4*>(row + (((4 * jb + 2 * c + q) ^ (i & 7)) << 4)) = make_uint4(t[0], t[1], t[2], t[3]);
+                        }
                     }
                     fence_before_sync();
                     fence_proxy_async_smem();
-                    arrive(&B.p_ready[m & 1]);
+                    arrive_warp(&B.p_ready[m & 1], lane);
                     if (flags & kFinal) break;
                 }
             }
@@ -697,23 +824,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (const int t0 = (int)clock(); !mbar_try_wait(&B.full[k % L::kStages], (k / L::kStages) & 1) && (int)clock() - t0 < 1 << 24;) {}
         } else if (warp == 23 || warp == 27) {
             // ---- products, each warp's issued by one elected thread: warp 23 the scores and U, warp 27 the outputs ----
-            constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 1, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0),
-                               id_qs = id_qk, id_pv = idesc_f16(128, 64, 1, 1, 1, 0);
-            const uint32_t tu = __shfl_sync(0xffffffffu, tm, 0), su = __shfl_sync(0xffffffffu, sb, 0);
-            const uint64_t dv0 = desc_mnmaj(su + L::oV, C, 0), dq0 = desc_kmaj(su, C, 0);
+            constexpr uint32_t id_u = idesc_f16(128, 128, 1, 1, 0, 1), id_qk = idesc_f16(128, 64, 1, 1, 0, 0);
+            const uint32_t me = elect_one();
+            const uint32_t q0 = (uint32_t)desc_kmaj(sb, C, 0), high = (uint32_t)(desc_kmaj(0, C, 0) >> 32);
             if (warp == 23) {
-                const uint64_t dkw = desc_mnmaj(su + L::kw, C, 0);
-                const uint64_t dk0 = desc_kmaj(su + L::oK, C, 0), dk0w = desc_mnmaj(su + L::oK, C, 0);  // k of the scores, of U
+                const uint64_t dk = desc_mnmaj(sb + L::oK, C, 0);
+                const uint32_t k0 = (uint32_t)desc_kmaj(sb + L::oK, C, 0), kt0 = (uint32_t)dk, mn_high = (uint32_t)(dk >> 32);
                 auto scores = [&](int st) {
-                    if (elect_one()) {
-                        const uint64_t dq = desc_add(dq0, st * L::kStage), dk = desc_add(dk0, st * L::kStage);
+                    const uint32_t at = st * (L::kStage >> 4);
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
+                    for (int x = 0; x < 2; ++x)
 #pragma unroll
-                            for (int ks = 0; ks < 4; ++ks)
-                                mma_f16(tu + kColP, desc_add(dq, x * (kTile / 2) + 32 * ks),
-                                        desc_add(dk, x * (kTile / 2) + 32 * ks), id_qk, (x | ks) > 0);
-                    }
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint32_t off = at + ((x * (kTile / 2) + 32 * ks) >> 4);
+                            mma_ss(me, tm + kColP, q0 + off, high, k0 + off, high, id_qk, (x | ks) > 0);
+                        }
                 };
                 bool ok = work;
                 if (ok) {
@@ -721,77 +846,63 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fence_after_sync();
                     if (ok) {
                         scores(0);
-                        if (elect_one()) mma_commit(&B.qk_full[0]);
-                        __syncwarp();
+                        commit_to(me, &B.qk_full[0]);
                     }
                 }
+                int st = 0;
 #pragma unroll 1
                 for (int m = 0; ok; ++m) {
-                    const int st = m % L::kStages;
-                    const uint64_t dv = desc_add(dv0, st * L::kStage), dk = desc_add(dk0w, st * L::kStage);
+                    const int st1 = st == L::kStages - 1 ? 0 : st + 1;
                     const bool final = gate(m)->flags & kFinal;
                     if (!final) {
-                        if (!wait_bar(B, &B.full[(m + 1) % L::kStages], (m + 1) / L::kStages)) break;
-                        if (!wait_bar(B, &B.p_read, m)) break;  // P's columns are free
+                        if (!wait_two(B, &B.full[st1], (m + 1) / L::kStages, &B.p_read, m)) break;  // P's columns are free
                         fence_after_sync();
-                        scores((m + 1) % L::kStages);
-                        if (elect_one()) mma_commit(&B.qk_full[(m + 1) & 1]);
-                        __syncwarp();
+                        scores(st1);
+                        commit_to(me, &B.qk_full[(m + 1) & 1]);
                     }
-                    if (!wait_bar(B, &B.kw_ready, m)) break;
-                    if (m > 0 && !wait_bar(B, &B.u_free, m - 1)) break;
+                    // (u_free: of the chunk before, or a phase that counts as over)
+                    if (!wait_two(B, &B.v_ready[m & 1], m >> 1, &B.u_free, m - 1)) break;
                     fence_after_sync();
-                    if (elect_one()) {
+                    const uint32_t kt = kt0 + st * (L::kStage >> 4);
 #pragma unroll
-                        for (int term = 2; term >= 0; --term)  // small terms first
-#pragma unroll
-                            for (int ks = 0; ks < 4; ++ks)
-                                mma_f16(tu + kColU, desc_add(dv, koff_mnmaj(16 * ks)),
-                                        desc_add(term ? desc_add(dkw, (term - 1) * kTile) : dk, koff_mnmaj(16 * ks)), id_u,
-                                        term < 2 || ks > 0);
-                        mma_commit(&B.u_full);
-                        mma_commit(&B.empty[st]);
-                    }
-                    __syncwarp();
-                    if (final) break;
-                }
-            } else {
-                const uint64_t dps = desc_kmaj(su + L::ps, C, 0);
-#pragma unroll 1
-                for (int m = 0; work; ++m) {
-                    const int st = m % L::kStages;
-                    const uint64_t dv = desc_add(dv0, st * L::kStage);
-                    if (!wait_bar(B, &B.s_ready, m)) break;
-                    if (m > 1 && !wait_bar(B, &B.o_free[m & 1], (m >> 1) - 1)) break;
-                    fence_after_sync();
-                    if (elect_one()) {
-                        const uint64_t dq = desc_add(dq0, st * L::kStage);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll
-                            for (int ks = 0; ks < 4; ++ks)
-                                mma_f16_ts(tu + kColO2 + 128 * (m & 1), tu + kColS + 32 * x + 8 * ks,
-                                           desc_add(dq, x * (kTile / 2) + 32 * ks), id_qs, (x | ks) > 0);
-                        mma_commit(&B.s_free);
-                    }
-                    __syncwarp();
-                    const int flags = gate(m)->flags;
-                    if (!wait_bar(B, &B.p_ready[m & 1], m >> 1)) break;
-                    fence_after_sync();
-                    if (elect_one()) {
-                        const uint64_t dp = desc_add(dps, (m & 1) * L::kP);
+                    for (int term = 3; term > 0; --term)  // small terms first
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
-                            mma_f16(tu + kColO1 + 128 * (m & 1), desc_add(dv, koff_mnmaj(16 * ks)),
-                                    desc_add(dp, koff_kmaj(C, 16 * ks)), id_pv, ks > 0);
-                        mma_commit(&B.o_full[m & 1]);
-                        mma_commit(&B.pv_done[m % 5]);
-                        if (!(flags & kLast)) {  // a last chunk's buffers take the state out first
-                            mma_commit(&B.empty[st]);
-                            mma_commit(&B.p_free[m & 1]);
-                        }
+                            mma_ts(me, tm + kColU, tm + kColV + 32 * term + 8 * ks, kt + (koff_mnmaj(16 * ks) >> 4), mn_high, id_u,
+                                   term < 3 || ks > 0);
+                    commit_to(me, &B.u_full[m & 1]);
+                    commit_to(me, &B.empty[st]);
+                    if (final) break;
+                    st = st1;
+                }
+            } else {
+                const uint32_t p0 = (uint32_t)desc_kmaj(sb + L::ps, C, 0);
+                int st = 0;
+#pragma unroll 1
+                for (int m = 0; work; ++m, st = st == L::kStages - 1 ? 0 : st + 1) {
+                    if (!wait_two(B, &B.v_ready[m & 1], m >> 1, &B.p_ready[m & 1], m >> 1)) break;
+                    bool s_too;  // (o_free: of the chunk before, or a phase that counts as over)
+                    if (!wait_and_test(B, &B.o_free, m - 1, &B.s_ready, m, s_too)) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        mma_ts(me, tm + kColO1, tm + kColV + 8 * ks, p0 + (m & 1) * (L::kP >> 4) + (koff_kmaj(C, 16 * ks) >> 4), high, id_qk, ks > 0);
+                    commit_to(me, &B.pv_done[m & 1]);
+                    const int flags = gate(m)->flags;
+                    if (!s_too && !wait_bar(B, &B.s_ready, m)) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_ts(me, tm + kColO2, tm + kColS + 32 * x + 8 * ks,
+                                   q0 + st * (L::kStage >> 4) + ((x * (kTile / 2) + 32 * ks) >> 4), high, id_qk, (x | ks) > 0);
+                    commit_to(me, &B.s_free);
+                    commit_to(me, &B.o_full);
+                    if (!(flags & kLast)) {  // a last chunk's buffers take the state out first
+                        commit_to(me, &B.empty[st]);
+                        commit_to(me, &B.p_free[m & 1]);
                     }
-                    __syncwarp();
                     if (flags & kFinal) break;
                 }
             }
@@ -823,8 +934,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
-    if (tid == 0 && B.abort) atomicOr(&g_device_status, kDevStatTimeout);
-    if (warp == 23) tmem_dealloc(tm, 512);
+    if (tid == 0 && (B.abort || B.tmem != tm)) atomicOr(&g_device_status, kDevStatTimeout);
+    if (warp == 23) tmem_dealloc(B.tmem, 512);
 }
 
 // The state before every segment of the sequences that have several: slot 1 holds
