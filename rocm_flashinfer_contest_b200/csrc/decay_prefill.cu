@@ -36,17 +36,23 @@
 // chunk).
 //
 // Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 92 us (its 205 MB alone
-// take 31), a chunk every 2,400 cycles in each CTA, of
-// which the products keep the tensor pipe for 1,408 at its full rate.  Half of
-// them have N = 64 and do not reach it, and what lies between two chunks' U (its
-// sums into S, S to bf16, or V's turn) is a chain of waits of 100 cycles and more
-// each, which the pipe waits for.  61 prompts of 82 tokens, 32 v-heads: 107 us,
-// bound by states (64 KiB in and 64 KiB out a prompt and head) that a CTA reads
-// and writes one after the other.  Tried and not kept, at those two: K scaled
-// instead of V, in shared memory (97 and 117 us); that with its lower terms
-// double-buffered (104); V turned by the state warps (100 and 117) or by the output
-// warps (111 and 117); scaling unrolled (96 and 113); the next state by TMA (95 and
-// 120, from 96 and 118).
+// take 31), a chunk every 2,400 cycles in each CTA.  The chunk's 32 products alone
+// take 1,540, issued without a pause and in turn (at the pipe's full rate 1,408);
+// those that add to one accumulator with N = 64 follow each other at 80 cycles, so
+// 12 for an output are 700 from the first to the end.  The rest are three loops of
+// nearly the same length, which share issue slots, shared memory and the pipe:
+// U's sums into S, S to bf16, S q, the next S; U, V's terms into the place that it
+// leaves, the next U; outputs out of the accumulators, the next output's products.
+// 61 prompts of 82 tokens, 32 v-heads: 107 us, bound by states (64 KiB in and 64
+// KiB out a prompt and head) that a CTA reads and writes one after the other.
+//
+// Tried and not kept, at those two: K scaled instead of V, in shared memory (97 and
+// 117 us); that with its lower terms double-buffered (104); V turned by the state
+// warps (100 and 117) or by the output warps (111 and 117); scaling unrolled (96 and
+// 113); eight output warps (91 and 109); all of V's terms made before the place is
+// free (92 and 108); an output's two chains of products issued in turn (92 and 108);
+// the next state by TMA into the place that the last one leaves (95 and 120, from 96
+// and 118 then).
 #include <cuda.h>
 
 #include <atomic>
