@@ -51,15 +51,17 @@ extern "C" {
 
 /* Version of this ABI (bumped on any signature change or addition; 3 adds
  * gdn_mtp_fwd and gdn_prefill_fwd_checkpointed, 4 gdn_decode_fwd_host,
- * gdn_prefill_fwd_host, gdn_prefill_fwd_ex and gdn_mtp_fwd's flags word). */
+ * gdn_prefill_fwd_host, gdn_prefill_fwd_ex and gdn_mtp_fwd's flags word) of
+ * this file.  The entry points of gdn_decay_b200.h are there where the library
+ * exports them; they came after version 4 and left it as it was. */
 int gdn_abi_version(void);
 
 /* Human-readable text for a status code. */
 const char *gdn_strerror(int status);
 
 /* Error bits recorded by the prefill kernels, the streaming multi-token decode
- * kernel and the decay operators' prefill and tree kernels since the last clear (1 = a bounded wait on an mbarrier timed
- * out); synchronises the device.  clear != 0 resets the word.  Returns -1 if
+ * kernel and the decay operators' prefill and tree kernels since the last
+ * clear (1 = a bounded wait on an mbarrier timed out); synchronises the device.  clear != 0 resets the word.  Returns -1 if
  * it cannot be read. */
 int gdn_device_status(int clear);
 

@@ -40,10 +40,11 @@ extern "C" {
  *
  * cu_seqlens is read on the device only; entries are clamped to [0, T] and an
  * end before its start counts as no tokens, so a malformed array reads and
- * writes nothing out of bounds.  A sequence without tokens keeps its state (zero when state is
- * NULL).  Tokens outside [cu_seqlens[0], cu_seqlens[N]) get a zero output and
+ * writes nothing out of bounds.  A sequence without tokens keeps its state
+ * (zero when state is NULL).  Tokens outside [cu_seqlens[0], cu_seqlens[N]) get a zero output and
  * are not read into any state, whatever they hold.  new_state may equal state
- * (in-place update); any other overlap of inputs and outputs is not allowed.
+ * (in-place update); any other overlap of inputs and outputs is not allowed
+ * (and refused for the states).
  * The products run on 64-token chunks, so a value of v that is not finite
  * spoils the outputs of its whole chunk, those of earlier tokens too.
  *

@@ -35,14 +35,16 @@
 // bring it to 0.0017 and cost 12 more products and 1,000 more instructions a
 // chunk).
 //
-// Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 92 us (its 205 MB alone
-// take 31), a chunk every 2,400 cycles in each CTA.  The chunk's 32 products alone
-// take 1,540, issued without a pause and in turn (at the pipe's full rate 1,408);
-// those that add to one accumulator with N = 64 follow each other at 80 cycles, so
-// 12 for an output are 700 from the first to the end.  The rest are three loops of
-// nearly the same length, which share issue slots, shared memory and the pipe:
-// U's sums into S, S to bf16, S q, the next S; U, V's terms into the place that it
-// leaves, the next U; outputs out of the accumulators, the next output's products.
+// Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 91 us (its 205 MB alone
+// take 31; called without a pause the GPU reaches its 1,000 W and lowers its clock
+// from 1.97 to 1.6 GHz: 105), a chunk every 2,400 cycles in each CTA.  The chunk's
+// 32 products alone take 1,540, issued without a pause and in turn (at the pipe's
+// full rate 1,408); those that add to one accumulator with N = 64 follow each other
+// at 80 cycles, so 12 for an output are 700 from the first to the end.  The rest are
+// three loops of nearly the same length, which share issue slots, shared memory and
+// the pipe: U's sums into S, S to bf16, S q, the next S; U, V's terms into the place
+// that it leaves, the next U; outputs out of the accumulators, the next output's
+// products.
 // 61 prompts of 82 tokens, 32 v-heads: 107 us, bound by states (64 KiB in and 64
 // KiB out a prompt and head) that a CTA reads and writes one after the other.
 //
@@ -52,7 +54,10 @@
 // 113); eight output warps (91 and 109); all of V's terms made before the place is
 // free (92 and 108); an output's two chains of products issued in turn (92 and 108);
 // the next state by TMA into the place that the last one leaves (95 and 120, from 96
-// and 118 then).
+// and 118 then); leaving out what only the dropped outputs need, in the first launch
+// (101 without a pause, but 112, and ragged prompts 61.5 from 60, as every chunk then
+// asks); that as a kernel of its own, with all outputs in the second launch (109, 115
+// and 77).
 #include <cuda.h>
 
 #include <atomic>

@@ -398,17 +398,24 @@ __global__ void __launch_bounds__(256, 2)
 }
 
 // ---------------------------------------------------------------------------
-// Commit: the decode kernel's streaming pass (32 rows of one v-head per CTA, 8
+// Commit: the decode kernel's streaming pass (64 rows of one v-head per CTA, 8
 // lanes to a row), with one update for each node of the accepted path.  The
 // state's read and write are the traffic (8 or 4 bytes an element); the path
 // costs 2 operations an element and node.  Every warp walks the path by itself:
 // lanes hold the parents and log decays of two nodes each, and a step is a
 // shuffle, so no warp waits for another.  The first walk, while the state is on
 // its way, finds the path's decay (and whether it reaches the cached state); the
-// second adds the nodes, newest first, with the next node's k and v on their way.
-// (With one thread walking for the CTA and k and v staged in shared memory, two
-// barriers and the longer chain of waits made the 64-entry commit 57 us, not 48.5;
-// 72 registers, 7 CTAs an SM: 8 of 64 registers spill, 51 us.)
+// second adds the nodes, newest first, with the next two nodes' k and v on their
+// way.
+//
+// 64 entries of 32 heads, fp32 (270 MB): 45 us with one node accepted, 48 with
+// four (5.7 TB/s), 57 with nine, 149 with 32, where the steps of a path, one after
+// the other, are what it takes; bf16 27, 34, 48 and 129.  With 32 rows a CTA, 45,
+// 48, 60 and 175; bf16 27, 35, 56 and 160 (a step's loads and shuffles serve half
+// the rows); with 128 rows 46, 52, 64 and 165.  With one node ahead only, 45, 48, 58
+// and 163.  With the path's k and v asked into L1 at the first walk, 45, 49, 72 and
+// 213 (of 32 rows).  With one thread walking for the CTA and k and v staged in shared
+// memory, the two barriers and the longer chain of waits made four nodes 57.
 // ---------------------------------------------------------------------------
 
 struct CommitParams {
@@ -423,10 +430,12 @@ struct CommitParams {
     int idx64, per_token, T, H, HV, rep, pool_size;
 };
 
+constexpr int kCommitRows = 64;
+
 template <bool kBf16>
-__global__ void __launch_bounds__(128, 7) decay_commit_kernel(const CommitParams p) {
+__global__ void __launch_bounds__(128, 4) decay_commit_kernel(const CommitParams p) {
     using Row = StateRow<kBf16>;
-    constexpr int kRows = 32, kPasses = kRows / 16, kBlocks = kDim / kRows;
+    constexpr int kRows = kCommitRows, kPasses = kRows / 16, kBlocks = kDim / kRows;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & 7;
     const int head = blockIdx.x / kBlocks, row = (blockIdx.x % kBlocks) * kRows + warp * (kRows / 4) + (lane >> 3);
     const int b = head / p.HV, h = head % p.HV, hq = h / p.rep, T = p.T;
@@ -464,17 +473,22 @@ __global__ void __launch_bounds__(128, 7) decay_commit_kernel(const CommitParams
         const float x = __shfl_sync(0xffffffffu, g[0], t & 31), y = __shfl_sync(0xffffffffu, g[1], t & 31);
         return t < 32 ? x : y;
     };
-    // the newest node's k and v come with the state
-    uint2 kn[4];
-    float vn[kPasses];
-    auto fetch = [&](int t) {
-        const __nv_bfloat16* kk = p.k + (((size_t)b * T + t) * p.H + hq) * kDim;
+    // k and v of the newest two nodes come with the state, those of the others two steps ahead
+    uint2 kn[2][4];
+    __nv_bfloat16 vn[2][kPasses];
+    auto fetch = [&](int t, uint2 (&kk)[4], __nv_bfloat16 (&vv)[kPasses]) {
+        if (t < 0) return;
+        const __nv_bfloat16* kp = p.k + (((size_t)b * T + t) * p.H + hq) * kDim;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) kn[j] = *reinterpret_cast<const uint2*>(kk + col_of<kBf16>(sub, j));
+        for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const uint2*>(kp + col_of<kBf16>(sub, j));
 #pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps) vn[ps] = bf16_to_f32(p.v[(((size_t)b * T + t) * p.HV + h) * kDim + row + 4 * ps]);
+        for (int ps = 0; ps < kPasses; ++ps) vv[ps] = p.v[(((size_t)b * T + t) * p.HV + h) * kDim + row + 4 * ps];
     };
-    if (some) fetch(last);
+    int t = some ? last : -1, ahead = -1;  // the node that is next, and the one after it
+    if (some) {
+        ahead = parent_of(t);
+        fetch(t, kn[0], vn[0]), fetch(ahead, kn[1], vn[1]);
+    }
     float all = 0.f;
     int end = some ? last : -2;
     while (end >= 0) {
@@ -493,24 +507,30 @@ __global__ void __launch_bounds__(128, 7) decay_commit_kernel(const CommitParams
         for (int j = 0; j < 4; ++j) s[ps][j].x *= a, s[ps][j].y *= a, s[ps][j].z *= a, s[ps][j].w *= a;
     }
     float behind = 0.f;  // log decays of the nodes behind this one
-    for (int t = path ? last : -1; t >= 0;) {
-        float2 k[8];
-        float2 f[kPasses];
-        const float w = expf(behind);
+    if (!path) t = -1;
+    while (t >= 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[2 * j] = widen2(kn[j].x), k[2 * j + 1] = widen2(kn[j].y);
+        for (int u = 0; u < 2; ++u) {
+            if (t < 0) break;
+            float2 k[8];
+            float2 f[kPasses];
+            const float w = expf(behind);
 #pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps) f[ps] = make_float2(w * vn[ps], w * vn[ps]);
-        behind += decay_of(t);
-        t = parent_of(t);
-        if (t >= 0) fetch(t);
+            for (int j = 0; j < 4; ++j) k[2 * j] = widen2(kn[u][j].x), k[2 * j + 1] = widen2(kn[u][j].y);
 #pragma unroll
-        for (int ps = 0; ps < kPasses; ++ps)
+            for (int ps = 0; ps < kPasses; ++ps) f[ps].x = f[ps].y = w * bf16_to_f32(vn[u][ps]);
+            behind += decay_of(t);
+            t = ahead;
+            ahead = ahead >= 0 ? parent_of(ahead) : -1;
+            fetch(ahead, kn[u], vn[u]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 x = __ffma2_rn(f[ps], k[2 * j], lo2(s[ps][j])), y = __ffma2_rn(f[ps], k[2 * j + 1], hi2(s[ps][j]));
-                s[ps][j] = make_float4(x.x, x.y, y.x, y.y);
-            }
+            for (int ps = 0; ps < kPasses; ++ps)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 x = __ffma2_rn(f[ps], k[2 * j], lo2(s[ps][j])), y = __ffma2_rn(f[ps], k[2 * j + 1], hi2(s[ps][j]));
+                    s[ps][j] = make_float4(x.x, x.y, y.x, y.y);
+                }
+        }
     }
     const size_t drow = ((size_t)oslot * p.HV + h) * kDim + row;
 #pragma unroll
@@ -656,7 +676,7 @@ extern "C" int gdn_decay_commit(const void* k, const void* v, void* pool, int st
     p.rep = HV / H;
     p.pool_size = pool_size;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const unsigned grid = (unsigned)((long long)B * HV * 4);
+    const unsigned grid = (unsigned)((long long)B * HV * (gdn::kDim / kCommitRows));
     if (state_bf16)
         decay_commit_kernel<true><<<grid, 128, 0, st>>>(p);
     else

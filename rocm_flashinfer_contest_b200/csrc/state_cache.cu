@@ -11,7 +11,10 @@
 // nothing re-read; bound by HBM bandwidth.  A warp takes 1,024 consecutive
 // values as 8 steps of 128: a lane reads 16 (8) bytes and writes 4 code bytes
 // a step, so 8 lanes share a group, its maximum takes three shuffles, and the
-// warp's 32 exponent bytes leave as one 32-byte store.
+// warp's 32 exponent bytes leave as one 32-byte store.  All 8 steps' loads are on
+// their way before the first is needed.  48 slots of 32 heads, fp32 to int8 and
+// back (248 MB): 47.4 us both, 5.2 TB/s, with two launches' starts and ends in it;
+// CTAs of 1, 2 and 8 warps instead of 4: 47.1, 47.5 and 47.9.
 #include <cuda_fp8.h>
 
 #include "decay_common.cuh"
