@@ -917,11 +917,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (flags & kFinal) break;
                 }
             }
-            if (B.abort && elect_one()) {  // products in flight end before the tensor memory is given back
-                uint64_t* drain = &B.drain[warp == 27];
-                mma_commit(drain);
-                for (const int t0 = (int)clock(); !mbar_try_wait(drain, 0) && (int)clock() - t0 < 1 << 30;) {}
-            }
         }
     }
     if (warp == 26 && lane == 0)
@@ -945,6 +940,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
+    if (B.abort) {  // given up: products in flight end before the tensor memory is given back
+        if ((warp == 23 || warp == 27) && elect_one()) {
+            uint64_t* drain = &B.drain[warp == 27];
+            mma_commit(drain);
+            for (const int t0 = (int)clock(); !mbar_try_wait(drain, 0) && (int)clock() - t0 < 1 << 30;) {}
+        }
+        __syncthreads();
+    }
     if (tid == 0 && (B.abort || B.tmem != tm)) atomicOr(&g_device_status, kDevStatTimeout);
     if (warp == 23) tmem_dealloc(B.tmem, 512);
 }
