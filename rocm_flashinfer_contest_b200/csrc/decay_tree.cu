@@ -26,23 +26,25 @@ constexpr int kTreeMax = GDN_DECAY_TREE_MAX;
 // memory while the CTA works on the item before it; a thread then turns half a
 // row into bf16 terms in tensor memory, where they are the A operand of
 // o^T[v, t] = S[v, :] . q_t on tcgen05, and the next state may come.  q, k and v of
-// the tree (3 T / 4 KiB) come through shared memory, asked for as soon as the last
-// item's products are done.  The scores and their product with v are small
-// (T x T x 128) and cut by the paths: warp-level products, which run beside the
-// tcgen05 ones.
-// (64 entries, 32 v-heads, 32 nodes: 43 us.  With S q on warp-level products
-// too, 54 us: two terms of a state times 32 tokens kept that path, an eighth of
-// tcgen05's rate, busy for 3,700 cycles a state, as long as its bytes take.)
+// the tree come by TMA too, each asked for as soon as the last item is done with
+// its place.  The scores and their product with v are small (T x T x 128) and cut
+// by the paths: warp-level products on operands from ldmatrix, which run beside the
+// tcgen05 ones.  One warp finds the next item's paths meanwhile.
+//
+// 64 entries, 32 v-heads, 32 nodes (182 MB): 37.6 us, 4.8 TB/s.  Two CTAs take turns
+// at load, conversion, products and outputs, 7,300 cycles an item each, and shared
+// memory holds no third.  With S q on warp-level products too, 54 us: two terms of a
+// state times 32 tokens kept that path, an eighth of tcgen05's rate, busy for 3,700
+// cycles a state, as long as its bytes take.  With q, k and v by 16-byte copies of all
+// threads 43, by a copy a row 54; operands of the small products by plain loads +2;
+// padding's v zeroed in shared memory, and every thread asking for the next slot,
+// +2; the next slot and output place found by every thread +1; the paths found by
+// one warp before the item +0.5.
 //
 // Precision: q, k, v are bf16 as given.  An fp32 state is split into two bf16
 // terms (hi + lo, off by at most 2^-17 of it) and the decayed scores P likewise,
 // so the products lose nothing next to the output's own rounding to bf16 (2^-8);
 // one bf16 term each would about double the output's error.
-//
-// Fragment layout: the contraction index may be permuted in both operands
-// alike, so that a lane's four k-slots {2c, 2c+1, 2c+8, 2c+9} of a 16-step hold
-// columns 4c..4c+3: the state comes by 16-byte (fp32) loads and q and k by 8-byte
-// loads from rows 288 bytes apart (no bank conflict).
 // ---------------------------------------------------------------------------
 
 struct VerifyParams {
@@ -57,17 +59,18 @@ struct VerifyParams {
     int idx64, per_token, T, Tp, H, HV, rep, pool_size, items;  // Tp: T rounded up to 16; items: entries * HV
 };
 
-constexpr int kQS = 144, kVS = 136, kPS = 72;  // row strides in bf16 elements of k, of v and the outputs, of P
+constexpr int kVS = 136, kPS = 72;  // row strides in bf16 elements of the outputs, of P
 
 // tensor-memory columns: S's two terms, o^T
 constexpr uint32_t kTmHi = 0, kTmLo = 64, kTmO = 128;
 
 // Shared memory: the next state in boxes of 128 rows x 128 bytes (128-byte swizzle),
-// then q (a K-major operand, same swizzle), k, v, outputs and the two terms of P.
+// then q, k and v in boxes of Tp rows x 128 bytes (same swizzle: q is a K-major
+// operand as it lies), outputs and the two terms of P.
 constexpr uint32_t kStateBox = 128 * 128;
 __host__ __device__ constexpr uint32_t state_bytes(bool bf16) { return bf16 ? 2 * kStateBox : 4 * kStateBox; }
 __host__ __device__ constexpr size_t verify_smem(int Tp, bool bf16) {
-    return state_bytes(bf16) + (size_t)Tp * 2 * (kDim + kQS + 2 * kVS + 2 * kPS);
+    return state_bytes(bf16) + (size_t)Tp * 2 * (3 * kDim + kVS + 2 * kPS);
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -80,8 +83,18 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+// Four 8 x 8 matrices, rows from the addresses of lanes 8 i .. 8 i + 7; turned or not.
+__device__ __forceinline__ void ldmatrix4(const void* p, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(const void* p, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
 }
 
 // hi + lo split of a pair: hi = the first 8 bits, lo = the rest rounded to bf16.
@@ -103,12 +116,16 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t ta, float (&a)[4], float (
 
 template <bool kBf16>
 __global__ void __launch_bounds__(256, 2)
-    decay_verify_kernel(const VerifyParams p, const __grid_constant__ CUtensorMap m_pool) {
+    decay_verify_kernel(const VerifyParams p, const __grid_constant__ CUtensorMap m_pool, const __grid_constant__ CUtensorMap m_q,
+                        const __grid_constant__ CUtensorMap m_k, const __grid_constant__ CUtensorMap m_v) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ unsigned long long s_path[kTreeMax];  // bit j: j is on the node's path; 0: padding
-    __shared__ float s_c[kTreeMax], s_e[kTreeMax];   // c_t and e^{c_t}
-    __shared__ int s_pad;  // some node is padding
-    __shared__ uint64_t s_full, s_done;
+    // of an item and the next one
+    __shared__ unsigned long long paths[2][kTreeMax];        // bit j: j is on the node's path; 0: padding
+    __shared__ float sums[2][kTreeMax], decays[2][kTreeMax];  // c_t and e^{c_t}
+    __shared__ unsigned long long used_nodes[2];              // bit t: node t is not padding
+    __shared__ size_t s_out;               // the next item's first output
+    __shared__ int s_padding;              // the next item has no state
+    __shared__ uint64_t s_full, s_done, s_qk, s_v;
     __shared__ uint32_t s_tmem;
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -116,9 +133,9 @@ __global__ void __launch_bounds__(256, 2)
     const int quarter = warp & 3, half = warp >> 2;  // tensor-memory lanes; columns of S, and rows of o^T
     const int rows = 32 * quarter + 16 * half;       // this warp's rows of o^T
     uint8_t* qs = smem_raw + state_bytes(kBf16);
-    __nv_bfloat16* ks_ = reinterpret_cast<__nv_bfloat16*>(qs + Tp * 256);
-    __nv_bfloat16* vs = ks_ + Tp * kQS;
-    __nv_bfloat16* os = vs + Tp * kVS;
+    uint8_t* ks_ = qs + Tp * 256;
+    uint8_t* vs = ks_ + Tp * 256;
+    __nv_bfloat16* os = reinterpret_cast<__nv_bfloat16*>(vs + Tp * 256);
     __nv_bfloat16* ph = os + Tp * kVS;
     __nv_bfloat16* pl = ph + Tp * kPS;
 
@@ -141,36 +158,103 @@ __global__ void __launch_bounds__(256, 2)
                 "l"(reinterpret_cast<uint64_t>(&m_pool)), "r"(x * (kBf16 ? 64 : 32)), "r"(0), "r"(number), "r"(smem_addr(&s_full))
                 : "memory");
     };
-    // all threads ask for the tree's q, k and v, warp 0 for its parents and log decays (nodes lane, lane + 32)
+    auto look_at = [&](int item) {
+        if (item >= p.items) return;
+        s_out = ((size_t)(item / p.HV) * T * p.HV + item % p.HV) * kDim;
+        s_padding = slot_of(item) < 0;
+    };
+    // one thread asks for the tree's q and k, and then for its v
+    auto ask_box = [&](uint8_t* dst, const CUtensorMap& map, int head, int b, uint64_t* bar) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                    smem_addr(dst) + x * Tp * 128),
+                "l"(reinterpret_cast<uint64_t>(&map)), "r"(64 * x), "r"(head), "r"(b * T), "r"(smem_addr(bar))
+                : "memory");
+    };
+    auto ask_qk = [&](int item) {
+        if (item >= p.items) return;
+        const int b = item / p.HV, hq = item % p.HV / p.rep;
+        umma::mbar_arrive_expect_tx(&s_qk, T * 512);
+        ask_box(qs, m_q, hq, b, &s_qk);
+        ask_box(ks_, m_k, hq, b, &s_qk);
+    };
+    auto ask_v = [&](int item) {
+        if (item >= p.items) return;
+        umma::mbar_arrive_expect_tx(&s_v, T * 256);
+        ask_box(vs, m_v, item % p.HV, item / p.HV, &s_v);
+    };
+    // warp 7 asks for its parents and log decays (nodes lane, lane + 32)
     int par[2];
     float gg[2];
-    auto ask_tree = [&](int item) {
+    auto ask_path = [&](int item) {
         if (item >= p.items) return;
-        const int b = item / p.HV, h = item % p.HV, hq = h / p.rep;
-#pragma unroll 1
-        for (int i = tid; i < T * 16; i += 256) {
-            const int t = i >> 4, x = 8 * (i & 15);
-            const size_t qk = (((size_t)b * T + t) * p.H + hq) * kDim + x, vv = (((size_t)b * T + t) * p.HV + h) * kDim + x;
-            cp_async16(qs + umma::kmaj_off(t, x, Tp), p.q + qk);
-            cp_async16(ks_ + t * kQS + x, p.k + qk);
-            cp_async16(vs + t * kVS + x, p.v + vv);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (warp == 0)
+        const int b = item / p.HV, h = item % p.HV;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = lane + 32 * i;
-                par[i] = -2, gg[i] = 0.f;
-                if (t < T) {
-                    par[i] = p.parents[(size_t)b * T + t];
-                    gg[i] = p.log_decay[p.per_token ? ((size_t)b * T + t) * p.HV + h : h];
+        for (int i = 0; i < 2; ++i) {
+            const int t = lane + 32 * i;
+            par[i] = -2, gg[i] = 0.f;
+            if (t < T) {
+                par[i] = p.parents[(size_t)b * T + t];
+                gg[i] = p.log_decay[p.per_token ? ((size_t)b * T + t) * p.HV + h : h];
+            }
+        }
+    };
+
+    // Paths and their decays by pointer doubling, a lane's two nodes in registers:
+    // after r rounds a node knows the last 2^r nodes of its path; -1 ends a path, -2
+    // marks padding.
+    auto find_paths = [&](int buf) {
+        unsigned long long m[2];
+        float cc[2];
+        int up[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = lane + 32 * i;
+            up[i] = par[i] < -1 || par[i] >= t ? -2 : par[i];
+            cc[i] = clamp_log_decay(gg[i]);
+            m[i] = t < T ? 1ull << t : 0ull;
+        }
+#pragma unroll 1
+        for (int hop = 1; hop < T; hop *= 2) {
+            unsigned long long mm[2];
+            float dc[2];
+            int uu[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // what node up[i] knows
+                const int u = up[i] & 31;
+                mm[i] = __shfl_sync(0xffffffffu, m[0], u);
+                dc[i] = __shfl_sync(0xffffffffu, cc[0], u);
+                uu[i] = __shfl_sync(0xffffffffu, up[0], u);
+                if (T > 32) {
+                    const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], u);
+                    const float d1 = __shfl_sync(0xffffffffu, cc[1], u);
+                    const int u1 = __shfl_sync(0xffffffffu, up[1], u);
+                    if (up[i] >= 32) mm[i] = m1, dc[i] = d1, uu[i] = u1;
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (up[i] >= 0) cc[i] += dc[i], m[i] |= mm[i], up[i] = uu[i];
+        }
+        unsigned used[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = lane + 32 * i;
+            paths[buf][t] = up[i] == -1 ? m[i] : 0ull;
+            sums[buf][t] = cc[i];
+            decays[buf][t] = expf(cc[i]);
+            used[i] = __ballot_sync(0xffffffffu, up[i] == -1);
+        }
+        if (lane == 0) used_nodes[buf] = (unsigned long long)used[1] << 32 | used[0];
     };
 
     if (tid == 0) {
         umma::mbar_init(&s_full, 1);
         umma::mbar_init(&s_done, 1);
+        umma::mbar_init(&s_qk, 1);
+        umma::mbar_init(&s_v, 1);
         umma::fence_mbar_init();
         ask_state(blockIdx.x);
     }
@@ -182,71 +266,27 @@ __global__ void __launch_bounds__(256, 2)
     for (int i = tid; i < (Tp - T) * 16; i += 256) {
         const int t = T + (i >> 4), x = 8 * (i & 15);
         *reinterpret_cast<uint4*>(qs + umma::kmaj_off(t, x, Tp)) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(ks_ + t * kQS + x) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(vs + t * kVS + x) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(ks_ + umma::kmaj_off(t, x, Tp)) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(vs + umma::kmaj_off(t, x, Tp)) = make_uint4(0, 0, 0, 0);
     }
-    ask_tree(blockIdx.x);
+    if (warp == 7) ask_path(blockIdx.x), find_paths(0), ask_path(blockIdx.x + gridDim.x);
+    if (tid == 192) look_at(blockIdx.x);
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
+    if (tid == 192) ask_qk(blockIdx.x), ask_v(blockIdx.x);
     const uint32_t tm = s_tmem;
-    uint32_t phase = 0;
+    uint32_t phase = 0, turn = 0;  // states and items so far
     bool lost = false;  // a wait has run out
 
 #pragma unroll 1
-    for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x, ++turn) {
         const int next = item + gridDim.x;
-        __nv_bfloat16* out = p.out + ((size_t)(item / p.HV) * T * p.HV + item % p.HV) * kDim;  // + t * HV * 128
-        const bool padding = slot_of(item) < 0;
+        __nv_bfloat16* out = p.out + s_out;  // + t * HV * 128
+        const bool padding = s_padding;
+        const unsigned long long* s_path = paths[turn & 1];
+        const float *s_c = sums[turn & 1], *s_e = decays[turn & 1];
 
-        // Paths and their decays by pointer doubling, a lane's two nodes in registers:
-        // after r rounds a node knows the last 2^r nodes of its path; -1 ends a path, -2
-        // marks padding.
-        if (warp == 0) {
-            unsigned long long m[2];
-            float cc[2];
-            int up[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = lane + 32 * i;
-                up[i] = par[i] < -1 || par[i] >= t || padding ? -2 : par[i];
-                cc[i] = clamp_log_decay(gg[i]);
-                m[i] = t < T ? 1ull << t : 0ull;
-            }
-#pragma unroll 1
-            for (int hop = 1; hop < T; hop *= 2) {
-                unsigned long long mm[2];
-                float dc[2];
-                int uu[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {  // what node up[i] knows
-                    const int u = up[i] & 31;
-                    mm[i] = __shfl_sync(0xffffffffu, m[0], u);
-                    dc[i] = __shfl_sync(0xffffffffu, cc[0], u);
-                    uu[i] = __shfl_sync(0xffffffffu, up[0], u);
-                    if (T > 32) {
-                        const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], u);
-                        const float d1 = __shfl_sync(0xffffffffu, cc[1], u);
-                        const int u1 = __shfl_sync(0xffffffffu, up[1], u);
-                        if (up[i] >= 32) mm[i] = m1, dc[i] = d1, uu[i] = u1;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (up[i] >= 0) cc[i] += dc[i], m[i] |= mm[i], up[i] = uu[i];
-            }
-            bool pad = false;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = lane + 32 * i;
-                s_path[t] = up[i] == -1 ? m[i] : 0ull;
-                s_c[t] = cc[i];
-                s_e[t] = expf(cc[i]);
-                pad |= t < T && up[i] != -1;
-            }
-            pad = __any_sync(0xffffffffu, pad);
-            if (lane == 0) s_pad = pad;
-        }
         float acc[8][4];  // o^T rows `rows` + {g, g + 8}, tokens 8 n + 2 c + {0, 1}
         if (!padding) {
             // half of state row 32 quarter + lane, in bf16 terms, into tensor memory
@@ -277,10 +317,11 @@ __global__ void __launch_bounds__(256, 2)
             umma::tmem_wait_st();
             umma::fence_before_sync();
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!umma::mbar_wait(&s_qk, turn & 1u)) lost = true;
         umma::fence_proxy_async_smem();  // q is read, and the state's place written, by the async proxy
         if (__syncthreads_or(lost)) break;
         if (tid == 0) ask_state(next);
+        if (tid == 192) look_at(next);
 
         if (!padding) {
             if (warp == 7) {  // the last to have a tile of scores
@@ -298,11 +339,9 @@ __global__ void __launch_bounds__(256, 2)
                 }
                 __syncwarp();
             }
-
-            // what padding nodes hold must not meet a zero weight as 0 * NaN
-            for (int i = tid; s_pad && i < T * 16; i += 256)
-                if (s_path[i >> 4] == 0ull)
-                    *reinterpret_cast<uint4*>(vs + (i >> 4) * kVS + 8 * (i & 15)) = make_uint4(0, 0, 0, 0);
+        }
+        if (warp == 7 && next < p.items) find_paths((turn + 1) & 1);
+        if (!padding) {
 
             // P[t, j] = e^{c_t - c_j} (q_t . k_j) on the paths, 0 elsewhere; nodes come after their parents, so
             // 16 x 8 tiles with every j > t stay out (they are not read either)
@@ -312,12 +351,14 @@ __global__ void __launch_bounds__(256, 2)
                 while (n >= 2 * (m + 1)) n -= 2 * (m + 1), ++m;
                 float x[4] = {0.f, 0.f, 0.f, 0.f}, x2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint2 a0 = *reinterpret_cast<const uint2*>(qs + umma::kmaj_off(16 * m + g, 16 * ks + 4 * c, Tp));
-                    const uint2 a1 = *reinterpret_cast<const uint2*>(qs + umma::kmaj_off(16 * m + g + 8, 16 * ks + 4 * c, Tp));
-                    const uint2 bb = *reinterpret_cast<const uint2*>(ks_ + (8 * n + g) * kQS + 16 * ks + 4 * c);
-                    const uint32_t a[4] = {a0.x, a1.x, a0.y, a1.y};
-                    mma16816(ks & 1 ? x2 : x, a, bb.x, bb.y);
+                for (int ks = 0; ks < 8; ks += 2) {
+                    uint32_t a[4], a2[4], bb[4];
+                    const int arow = 16 * m + (lane & 15), acol = 16 * ks + 8 * (lane >> 4);
+                    ldmatrix4(qs + umma::kmaj_off(arow, acol, Tp), a);
+                    ldmatrix4(qs + umma::kmaj_off(arow, acol + 16, Tp), a2);
+                    ldmatrix4(ks_ + umma::kmaj_off(8 * n + (lane & 7), 16 * ks + 8 * (lane >> 3), Tp), bb);
+                    mma16816(x, a, bb[0], bb[1]);
+                    mma16816(x2, a2, bb[2], bb[3]);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] += x2[e];
@@ -333,7 +374,7 @@ __global__ void __launch_bounds__(256, 2)
                     *reinterpret_cast<uint32_t*>(pl + t * kPS + j) = low;
                 }
             }
-            lost = !umma::mbar_wait(&s_done, phase & 1u);
+            if (!umma::mbar_wait(&s_done, phase & 1u)) lost = true;
             __syncwarp();
             ++phase;
             umma::fence_after_sync();
@@ -349,23 +390,33 @@ __global__ void __launch_bounds__(256, 2)
                 }
             umma::fence_before_sync();
         }
+        if (!umma::mbar_wait(&s_v, turn & 1u)) lost = true;
         if (__syncthreads_or(lost)) break;
+        if (tid == 192) ask_qk(next);  // their place is free
+        if (warp == 7) ask_path(next + gridDim.x);
         if (!padding) {
 #pragma unroll 1
             for (int js = 0; js < mt; ++js) {
                 uint32_t a[4];
-                const __nv_bfloat16* src = vs + (16 * js + (lane >> 4) * 8 + (lane & 7)) * kVS + rows + (lane >> 3 & 1) * 8;
-                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                             : "r"(smem_addr(src)));
+                ldmatrix4_trans(vs + umma::kmaj_off(16 * js + (lane >> 4) * 8 + (lane & 7), rows + (lane >> 3 & 1) * 8, Tp), a);
+                // what padding nodes hold must not meet a zero weight as 0 * NaN
+                const unsigned use = (unsigned)(used_nodes[turn & 1] >> (16 * js + 2 * c));
+                const uint32_t keep = (use & 1 ? 0xffffu : 0u) | (use & 2 ? 0xffff0000u : 0u);
+                const uint32_t keep8 = (use & 0x100 ? 0xffffu : 0u) | (use & 0x200 ? 0xffff0000u : 0u);
+                a[0] &= keep, a[1] &= keep, a[2] &= keep8, a[3] &= keep8;
+                // 16 tokens at a time: their two terms of P as two column blocks of 8 tokens each
+                const int at = ((lane >> 4) * 8 + (lane & 7)) * kPS + 16 * js + (lane >> 3 & 1) * 8;
 #pragma unroll
-                for (int term = 0; term < 2; ++term)
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                        if (n < 2 * mt && n >= 2 * js) {
-                            const uint32_t* x = reinterpret_cast<const uint32_t*>((term ? ph : pl) + (8 * n + g) * kPS + 16 * js + 2 * c);
-                            mma16816(acc[n], a, x[0], x[4]);
-                        }
+                for (int i = 0; i < 4; ++i)
+                    if (i < mt && i >= js) {
+                        uint32_t low[4], high[4];
+                        ldmatrix4(pl + 16 * i * kPS + at, low);
+                        ldmatrix4(ph + 16 * i * kPS + at, high);
+                        mma16816(acc[2 * i], a, low[0], low[1]);
+                        mma16816(acc[2 * i + 1], a, low[2], low[3]);
+                        mma16816(acc[2 * i], a, high[0], high[1]);
+                        mma16816(acc[2 * i + 1], a, high[2], high[3]);
+                    }
             }
 #pragma unroll
             for (int n = 0; n < 8; ++n)
@@ -380,18 +431,20 @@ __global__ void __launch_bounds__(256, 2)
                 }
         }
         __syncthreads();
-        ask_tree(next);
+        if (tid == 192) ask_v(next);
         for (int i = tid; i < T * 16; i += 256) {
             const int t = i >> 4, x = 8 * (i & 15);
             uint4 val = *reinterpret_cast<const uint4*>(os + t * kVS + x);
-            if (s_path[t] == 0ull) val = make_uint4(0, 0, 0, 0);
+            if (padding || s_path[t] == 0ull) val = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(out + (size_t)t * p.HV * kDim + x) = val;
         }
-        __syncthreads();  // the paths are written for the next item
+        __syncthreads();
     }
     if (__syncthreads_or(lost) && tid == 0) {  // given up: what is in flight gets as long again to end before the CTA does
         umma::mbar_wait(&s_full, phase & 1u);
         umma::mbar_wait(&s_done, phase & 1u);
+        umma::mbar_wait(&s_qk, turn & 1u), umma::mbar_wait(&s_qk, ~turn & 1u);
+        umma::mbar_wait(&s_v, turn & 1u), umma::mbar_wait(&s_v, ~turn & 1u);
     }
     __syncthreads();
     if (warp == 1) umma::tmem_dealloc(tm, 256);
@@ -576,6 +629,18 @@ static int launch_verify(const VerifyParams& p, const void* pool, cudaStream_t s
                dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return GDN_ERR_CUDA;
+    // q, k and v, [entries * T, heads, 128], in boxes of T nodes x 64
+    CUtensorMap m_qkv[3] = {};
+    const __nv_bfloat16* from[3] = {p.q, p.k, p.v};
+    for (int i = 0; i < 3; ++i) {
+        const cuuint64_t heads = i < 2 ? p.H : p.HV;
+        const cuuint64_t tdims[3] = {(cuuint64_t)kDim, heads, (cuuint64_t)(p.items / p.HV) * p.T}, tstrides[2] = {kDim * 2, heads * kDim * 2};
+        const cuuint32_t tbox[3] = {64u, 1u, (cuuint32_t)p.T};
+        if (encode(&m_qkv[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(from[i]), tdims, tstrides, tbox, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return GDN_ERR_CUDA;
+    }
     const size_t smem = verify_smem(p.Tp, kBf16);
     static std::atomic<unsigned long long> done{0};  // the kernel's attribute, once per device (again after a failure)
     int dev = 0;
@@ -590,7 +655,7 @@ static int launch_verify(const VerifyParams& p, const void* pool, cudaStream_t s
         if (dev < 64) done.fetch_or(bit);
     }
     const int per_sm = 2 * (smem + 4096) <= 227 * 1024 ? 2 : 1, most = per_sm * 148;
-    decay_verify_kernel<kBf16><<<p.items < most ? p.items : most, 256, smem, st>>>(p, map);
+    decay_verify_kernel<kBf16><<<p.items < most ? p.items : most, 256, smem, st>>>(p, map, m_qkv[0], m_qkv[1], m_qkv[2]);
     return gdn_launch_status();
 }
 
