@@ -45,8 +45,10 @@
 // the pipe: U's sums into S, S to bf16, S q, the next S; U, V's terms into the place
 // that it leaves, the next U; outputs out of the accumulators, the next output's
 // products.
-// 61 prompts of 82 tokens, 32 v-heads: 107 us, bound by states (64 KiB in and 64
-// KiB out a prompt and head) that a CTA reads and writes one after the other.
+// 61 prompts of 82 tokens, 32 v-heads: 106.5 us, bound by states (64 KiB in and 64
+// KiB out a prompt and head) that a CTA reads and writes one after the other: 4,700
+// of 8,500 cycles a segment of one chunk are the wait for its start state, 7 us in
+// all for its rows lying 512 bytes apart in a warp's loads.
 //
 // Tried and not kept, at those two: K scaled instead of V, in shared memory (97 and
 // 117 us); that with its lower terms double-buffered (104); V turned by the state
@@ -179,8 +181,8 @@ struct L {
     static constexpr uint32_t ps = kStages * kStage;  // two buffers of P
     static constexpr uint32_t kP = C * C * 2;
     static constexpr uint32_t os = ps + 2 * kP;       // two buffers of a chunk's outputs, [token][v]
-    static constexpr uint32_t tail = os + 2 * kTile;  // the last piece of a state on its way out
-    static constexpr uint32_t gates = tail + 8 * 1024;
+    static constexpr uint32_t tail = os + 2 * kTile;  // 24 KiB of a state on its way out
+    static constexpr uint32_t gates = tail + 24 * 1024;
     static constexpr uint32_t bars = gates + kGates * 832;
     static constexpr uint32_t total = bars + 320;
 };
@@ -495,17 +497,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             arrive_warp(&B.u_free, lane);
             first = flags & kLast;
             if (first) {
-                // the state leaves by way of its last chunk's stage (48 KiB) and buffer of P (8 KiB), free after
-                // that chunk's last products, and 8 KiB beside them; the store warp sends it on and gives
-                // them back
-                if (!wait_bar(B, &B.s_free, m)) break;
+                // the state leaves by way of its last chunk's k and v (32 KiB) and buffer of P (8 KiB), free after
+                // that chunk's U and P V, and 24 KiB beside them; the store warp sends it on and gives them back
+                if (!wait_bar(B, &B.pv_done[m & 1], m >> 1)) break;
                 if (stored > 0 && !wait_bar(B, &B.st_free, stored - 1)) break;
                 ++stored;
                 if (out >= 0) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const uint32_t box = half && x ? (v < 64 ? L::ps + (m & 1) * L::kP : L::tail - 64 * 128)
-                                                       : (m % L::kStages) * L::kStage + (2 * half + x) * kBox;
+                        const uint32_t box = !half            ? (m % L::kStages) * L::kStage + L::oK + x * kBox
+                                             : !x || v < 64 ? L::tail + x * kBox
+                                                            : L::ps + (m & 1) * L::kP - 64 * 128;
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             *reinterpret_cast<float4*>(sm + box + v * 128 + ((i ^ (v & 7)) << 4)) =
@@ -864,7 +866,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                 for (int m = 0; ok; ++m) {
                     const int st1 = st == L::kStages - 1 ? 0 : st + 1;
-                    const bool final = gate(m)->flags & kFinal;
+                    const int flags = gate(m)->flags;
+                    const bool final = flags & kFinal;
                     if (!final) {
                         if (!wait_two(B, &B.full[st1], (m + 1) / L::kStages, &B.p_read, m)) break;  // P's columns are free
                         fence_after_sync();
@@ -882,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mma_ts(me, tm + kColU, tm + kColV + 32 * term + 8 * ks, kt + (koff_mnmaj(16 * ks) >> 4), mn_high, id_u,
                                    term < 3 || ks > 0);
                     commit_to(me, &B.u_full[m & 1]);
-                    commit_to(me, &B.empty[st]);
+                    if (!(flags & kLast)) commit_to(me, &B.empty[st]);  // a last chunk's k and v take the state out first
                     if (final) break;
                     st = st1;
                 }
@@ -910,10 +913,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    q0 + st * (L::kStage >> 4) + ((x * (kTile / 2) + 32 * ks) >> 4), high, id_qk, (x | ks) > 0);
                     commit_to(me, &B.s_free);
                     commit_to(me, &B.o_full);
-                    if (!(flags & kLast)) {  // a last chunk's buffers take the state out first
-                        commit_to(me, &B.empty[st]);
-                        commit_to(me, &B.p_free[m & 1]);
-                    }
+                    commit_to(me, &B.empty[st]);
+                    if (!(flags & kLast)) commit_to(me, &B.p_free[m & 1]);  // (nor is this free)
                     if (flags & kFinal) break;
                 }
             }
@@ -927,7 +928,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (out >= 0) {
 #pragma unroll
                 for (int x = 0; x < 8; ++x)
-                    tma_store(&m_state, sb + (x == 7 ? L::tail : x == 6 ? L::ps + (m & 1) * L::kP : st * L::kStage + x * (kBox / 2)),
+                    tma_store(&m_state,
+                              sb + (x < 4   ? st * L::kStage + L::oK + x * (kBox / 2)
+                                    : x < 7 ? L::tail + (x - 4) * (kBox / 2)
+                                            : L::ps + (m & 1) * L::kP),
                               32 * (x >> 1), 64 * (x & 1), out);
                 bulk_wait_read0();
             }
