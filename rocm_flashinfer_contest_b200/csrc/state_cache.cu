@@ -8,13 +8,13 @@
 // 2^(e-6)).
 //
 // Both directions stream: 4 + 33/32 bytes (fp32) or 2 + 33/32 (bf16) a value,
-// nothing re-read; bound by HBM bandwidth.  A warp takes 1,024 consecutive
-// values as 8 steps of 128: a lane reads 16 (8) bytes and writes 4 code bytes
-// a step, so 8 lanes share a group, its maximum takes three shuffles, and the
-// warp's 32 exponent bytes leave as one 32-byte store.  All 8 steps' loads are on
-// their way before the first is needed.  48 slots of 32 heads, fp32 to int8 and
-// back (248 MB): 47.4 us both, 5.2 TB/s, with two launches' starts and ends in it;
-// CTAs of 1, 2 and 8 warps instead of 4: 47.1, 47.5 and 47.9.
+// nothing re-read; bound by HBM bandwidth.  A warp takes 512 consecutive values as
+// 4 steps of 128: a lane reads 16 (8) bytes and writes 4 code bytes a step, so 8
+// lanes share a group, its maximum takes three shuffles, and the warp's 16 exponent
+// bytes leave as one store.  All 4 steps' loads are on their way before the first is
+// needed.  48 slots of 32 heads, fp32 to int8 and back (248 MB): 45.8 us both, 5.4
+// TB/s, with two launches' starts and ends in it; 8 steps a warp 47.4, 2 steps 49.4;
+// CTAs of 1, 2 and 8 warps instead of 4 (8 steps): 47.1, 47.5 and 47.9.
 #include <cuda_fp8.h>
 
 #include "decay_common.cuh"
@@ -23,7 +23,7 @@ namespace gdn {
 namespace cache {
 
 constexpr int kGroup = GDN_STATE_CACHE_GROUP;
-constexpr int kSteps = 8, kWarpElems = kSteps * 128, kWarps = 4;
+constexpr int kSteps = 4, kWarpElems = kSteps * 128, kWarps = 4;
 
 struct Params {
     void* pool;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(32 * kWarps) store_kernel(const Params p) {
         const int got = __shfl_sync(0xffffffffu, byte, 8 * (lane & 3));
         if (lane >> 2 == u) mine = got;
     }
-    if (kGroup * lane < left) p.exps[(cslot * p.elems + at) / kGroup + lane] = (uint8_t)mine;
+    if (lane < 4 * kSteps && kGroup * lane < left) p.exps[(cslot * p.elems + at) / kGroup + lane] = (uint8_t)mine;
 }
 
 template <bool kBf16, bool kE4m3>
