@@ -188,7 +188,7 @@ struct L {
 };
 static_assert(L::total <= 227 * 1024, "shared memory");
 
-enum : int { kFirst = 1, kLast = 2, kFinal = 4 };
+enum : int { kLast = 1, kFinal = 2 };
 
 // What a chunk's warps need to know of it.
 struct Gate {
@@ -196,7 +196,7 @@ struct Gate {
     float e[C];   // scale * e^{c_i}
     float w[C];   // e^{c_63 - c_i}
     float a;      // e^{c_63}
-    int flags;    // first / last chunk of its segment, last chunk of this CTA
+    int flags;    // last chunk of its segment, last chunk of this CTA
     int t, live;  // first token; tokens of the segment from there on, at most 64
     int rows;     // rows of output to write: live, or none
     int h;
@@ -819,8 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     *reinterpret_cast<float2*>(&gt->w[2 * lane]) = w;
                     if (lane == 0) {
                         gt->a = all;
-                        gt->flags = (c == 0 ? kFirst : 0) | (c == nch - 1 ? kLast : 0) |
-                                    (c == nch - 1 && next.n >= p.N ? kFinal : 0);
+                        gt->flags = c < nch - 1 ? 0 : next.n >= p.N ? kLast | kFinal : kLast;
                         gt->t = it.t0 + c * C, gt->live = min(C, len - c * C);
                         gt->rows = p.first && it.s > 0 ? 0 : gt->live;
                         gt->h = h, gt->src = src, gt->out = out, gt->decay = decay;
