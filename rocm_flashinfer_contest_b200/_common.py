@@ -124,11 +124,21 @@ def require_pool(pool, HV: int, V: int, K: int, device: torch.device, name: str 
     return pool
 
 
-def require_indices(idx, B: int, device: torch.device, name: str, like=None):
-    """[B] int32/int64 indices on the device, as the type of ``like`` where given."""
+def require_indices(idx, B: int, device: torch.device, name: str):
+    """[B] int32/int64 indices on the device."""
     if not isinstance(idx, torch.Tensor) or idx.dtype not in (torch.int32, torch.int64) \
             or idx.device != device or tuple(idx.shape) != (B,):
         raise ValueError(f"{name} must be an int32/int64 [{B}] tensor on {device}")
-    if like is not None and idx.dtype != like.dtype:
-        idx = idx.to(like.dtype)
     return idx.contiguous()
+
+
+def require_index_pair(a, b, B: int, device: torch.device, names):
+    """Two index tensors (``b`` may be None) as one type: the kernels take one.  Where
+    they differ int32 becomes int64, never the other way: 2^32 narrowed would be
+    slot 0."""
+    a = require_indices(a, B, device, names[0])
+    if b is not None:
+        b = require_indices(b, B, device, names[1])
+        if a.dtype != b.dtype:
+            a, b = a.to(torch.int64), b.to(torch.int64)
+    return a, b

@@ -107,9 +107,8 @@ def run_pool(q, k, v, initial_state, initial_state_indices, log_decay, scale=Non
     inputs = _inputs(q, k, v, log_decay)
     dev, q, k, v, _, _, B, H, HV, K, V = inputs
     C.require_pool(initial_state, HV, V, K, dev)
-    idx = C.require_indices(initial_state_indices, B, dev, "initial_state_indices")
-    out_idx = None if output_state_indices is None else \
-        C.require_indices(output_state_indices, B, dev, "output_state_indices", like=idx)
+    idx, out_idx = C.require_index_pair(initial_state_indices, output_state_indices, B, dev,
+                                        ("initial_state_indices", "output_state_indices"))
     if output is None:
         output = torch.empty_like(v)
     else:

@@ -43,7 +43,7 @@ MAX_NODES = 64  # GDN_DECAY_TREE_MAX (include/gdn_decay_b200.h)
 _BF16, _F32 = torch.bfloat16, torch.float32
 
 
-def _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay):
+def _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay, output_state_indices=None):
     dev = C.cuda_device_of(k)
     ready = C.ready
     if q is not None and not ready(q, _BF16, dev):
@@ -66,19 +66,20 @@ def _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay):
     else:
         g, per_token = C.require_log_decay(log_decay, (B, T), HV, dev)
     C.require_pool(initial_state, HV, V, K, dev)
-    idx = C.require_indices(initial_state_indices, B, dev, "initial_state_indices")
+    idx, out_idx = C.require_index_pair(initial_state_indices, output_state_indices, B, dev,
+                                        ("initial_state_indices", "output_state_indices"))
     if not ready(parents, torch.int32, dev):
         parents = C.require(parents, "parents", torch.int32, dev)
     if parents.shape != (B, T):
         raise ValueError(f"parents must be {(B, T)}, got {tuple(parents.shape)}")
-    return dev, q, k, v, initial_state, idx, parents, g, per_token, B, T, H, HV, K, V
+    return (dev, q, k, v, initial_state, idx, parents, g, per_token, B, T, H, HV, K, V), out_idx
 
 
 def run(q, k, v, initial_state, initial_state_indices, parents, log_decay, scale=None, output=None):
     """See the module docstring."""
     if q is None:
         raise TypeError("q must be a torch.Tensor, got NoneType")
-    inputs = _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay)
+    inputs, _ = _inputs(q, k, v, initial_state, initial_state_indices, parents, log_decay)
     if output is None:
         output = torch.empty_like(inputs[3])
     else:
@@ -102,14 +103,13 @@ def _run(inputs, scale, output):
 
 def commit(k, v, initial_state, initial_state_indices, parents, accepted, log_decay, output_state_indices=None):
     """See the module docstring."""
-    inputs = _inputs(None, k, v, initial_state, initial_state_indices, parents, log_decay)
-    dev, idx, B = inputs[0], inputs[5], inputs[9]
+    inputs, out_idx = _inputs(None, k, v, initial_state, initial_state_indices, parents, log_decay,
+                              output_state_indices)
+    dev, B = inputs[0], inputs[9]
     if not C.ready(accepted, torch.int32, dev):
         accepted = C.require(accepted, "accepted", torch.int32, dev)
     if accepted.shape != (B,):
         raise ValueError(f"accepted must be {(B,)}, got {tuple(accepted.shape)}")
-    out_idx = None if output_state_indices is None else \
-        C.require_indices(output_state_indices, B, dev, "output_state_indices", like=idx)
     _commit(inputs, accepted, out_idx)
     return initial_state
 

@@ -17,7 +17,7 @@ an fp32 pool's bytes.  ``empty`` allocates them.
 ``load(codes, exponents, cache_slots, pool, slots) -> pool``
     Reads them back: pool value = code * 2^e.
 
-slots and cache_slots: [B] int32 or int64 of one type, on the device.  A pair
+slots and cache_slots: [B] int32 or int64, on the device.  A pair
 with either index outside its tensor (-1) is padding and skipped; otherwise no
 two pairs may write the same slot.  One kernel launch each on the current stream of the
 pool's device, no host synchronisation.
@@ -68,8 +68,7 @@ def _check(pool, slots, codes, exponents, cache_slots):
     B = slots.shape[0]
     if max(B, shape[0], cshape[0]) >= 2 ** 31:
         raise ValueError("fewer than 2^31 pairs and slots are needed")
-    slots = C.require_indices(slots, B, dev, "slots")
-    cache_slots = C.require_indices(cache_slots, B, dev, "cache_slots", like=slots)
+    slots, cache_slots = C.require_index_pair(slots, cache_slots, B, dev, ("slots", "cache_slots"))
     return dev, pool, slots, codes, exponents, cache_slots, B, math.prod(shape[1:])
 
 
