@@ -90,15 +90,6 @@ def _validate(q, k, v, initial_state, initial_state_indices, A_log, a, dt_bias, 
     return dev, (q, k, v, idx, A_log, a, dt_bias, b), (B, T, H, HV, K, V), (slots, steps)
 
 
-def _out_indices(out_idx, idx, B, dev):
-    if out_idx is None:
-        return None
-    if not isinstance(out_idx, torch.Tensor) or out_idx.device != dev or tuple(out_idx.shape) != (B,) \
-            or out_idx.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"output_state_indices must be an int32/int64 [{B}] tensor on {dev}")
-    return out_idx.to(idx.dtype).contiguous()
-
-
 GDN_MTP_QK_L2NORM = 1           # gdn_mtp_fwd flags (include/gdn_b200.h)
 GDN_MTP_SNAPSHOTS_BY_ENTRY = 2
 
@@ -140,7 +131,9 @@ def run_into(q, k, v, initial_state, initial_state_indices, A_log, a, dt_bias, b
                                     or tuple(final_state.shape) != tuple(initial_state.shape)
                                     or not final_state.is_contiguous()):
         raise ValueError("final_state must be a contiguous tensor shaped and typed like initial_state")
-    oidx = _out_indices(output_state_indices, tensors[3], B, dev)
+    idx, oidx = C.require_index_pair(tensors[3], output_state_indices, B, dev,
+                                     ("initial_state_indices", "output_state_indices"))
+    tensors = (*tensors[:3], idx, *tensors[4:])
     _launch(dev, tensors, dims, initial_state, final_state, scale, output,
             intermediate_states_buffer, slots, steps, qk_l2norm, oidx)
     return output, final_state

@@ -65,3 +65,17 @@ def test_an_index_past_32_bits_touches_no_slot(far_first):
     assert (codes == 5).all() and (exps == 127).all()
     state_cache.load(codes, exps, idx, pool, dst)
     assert torch.equal(pool, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [3, 64])
+def test_mtp_output_index_past_32_bits_touches_no_slot(B):
+    from rocm_flashinfer_contest_b200 import gdn_mtp, inputs
+    args = inputs.to_device(inputs.mtp_inputs(B, 2, B + 2, 2, 4, seed=1), torch.device("cuda"))   # int32 indices
+    pool, before = args[3], args[3].clone()
+    far = torch.arange(B, device="cuda") + FAR
+    out = torch.empty(B, 2, 4, 128, dtype=torch.bfloat16, device="cuda")
+    gdn_mtp.run_into(*args[:10], out, pool, output_state_indices=far)
+    assert torch.equal(pool, before)
+    want, _ = gdn_mtp.run(*args[:10])
+    assert torch.equal(out, want)
