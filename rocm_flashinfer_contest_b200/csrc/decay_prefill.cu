@@ -1110,8 +1110,9 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         (decay_per_token != 0 && decay_per_token != 1))
         return GDN_ERR_INVALID;
     if (K != gdn::kDim || V != gdn::kDim || HV % H != 0) return GDN_ERR_UNSUPPORTED;
-    const int seg = segment_tokens(T, HV), slots = T / seg + N, ws_slots = N > 0 ? workspace_slots(T, HV) : 0;
-    if (((long long)slots + 1) * HV > (1ll << 26)) return GDN_ERR_UNSUPPORTED;  // grid index
+    const int seg = segment_tokens(T, HV), ws_slots = N > 0 ? workspace_slots(T, HV) : 0;
+    const long long slots = (long long)(T / seg) + N;                // (an int could overflow)
+    if (slots + 1 > (1ll << 26) / HV) return GDN_ERR_UNSUPPORTED;  // grid index
     if (N == 0 && T == 0) return GDN_OK;
     if (!cu_seqlens || (T > 0 && (!q || !k || !v || !out || !log_decay)) || (N > 0 && !new_state)) return GDN_ERR_INVALID;
     if (!gdn_aligned(q, 16) || !gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(out, 16) ||
@@ -1180,7 +1181,7 @@ extern "C" int gdn_decay_prefill_fwd(const void* q, const void* k, const void* v
         }
         p.first = 0;
     }
-    const int items = slots * HV;
+    const int items = (int)(slots * HV);
     cfg.gridDim = dim3(items < kSms ? (items > 0 ? items : 1) : kSms), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = L::total;
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, decay_prefill_kernel, p, mq, mk, mv, mn, mo);
     if (e != cudaSuccess) {
