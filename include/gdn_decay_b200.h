@@ -73,6 +73,8 @@ size_t gdn_decay_prefill_workspace_bytes(int N, int T, int HV);
  * An index outside [0, pool_size) marks padding: its output is zero and no
  * state is read or written.  An output slot outside the pool skips the write.
  * No slot may be written by one entry and read or written by another.
+ * A pool (here and below) may have no slots, and then no address: every entry
+ * is padding.
  */
 int gdn_decay_decode_fwd(const void *q, const void *k, const void *v, const void *pool_in,
                          void *pool_out, int state_bf16, const void *indices,

@@ -117,7 +117,8 @@ extern "C" int gdn_decay_decode_fwd(const void* q, const void* k, const void* v,
     if (bad) return bad;
     if ((long long)B * HV > (1ll << 27)) return GDN_ERR_UNSUPPORTED;  // grid index
     if (B == 0) return GDN_OK;
-    if (!q || !k || !v || !log_decay || !out || !pool_out) return GDN_ERR_INVALID;
+    // (a pool without slots may have no address: every entry is padding then)
+    if (!q || !k || !v || !log_decay || !out || (!pool_out && pool_size > 0)) return GDN_ERR_INVALID;
     if (!gdn_aligned(q, 16) || !gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(out, 16) ||
         !gdn_aligned(pool_in, 16) || !gdn_aligned(pool_out, 16) || !gdn_aligned(log_decay, 4) ||
         !gdn_aligned(indices, indices_int64 ? 8 : 4) || !gdn_aligned(out_indices, indices_int64 ? 8 : 4))

@@ -622,7 +622,7 @@ static int launch_verify(const VerifyParams& p, const void* pool, cudaStream_t s
     const EncodeFn encode = tree_encode_fn();
     if (encode == nullptr) return GDN_ERR_CUDA;
     CUtensorMap map{};
-    const cuuint64_t el = kBf16 ? 2 : 4, n = (cuuint64_t)(p.pool_size > 0 ? p.pool_size : 1) * p.HV;
+    const cuuint64_t el = kBf16 ? 2 : 4, n = (cuuint64_t)p.pool_size * p.HV;
     const cuuint64_t dims[3] = {(cuuint64_t)kDim, (cuuint64_t)kDim, n}, strides[2] = {kDim * el, kDim * kDim * el};
     const cuuint32_t box[3] = {(cuuint32_t)(128 / el), (cuuint32_t)kDim, 1u}, estr[3] = {1u, 1u, 1u};
     if (encode(&map, kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(pool),
@@ -684,11 +684,15 @@ extern "C" int gdn_decay_verify_fwd(const void* q, const void* k, const void* v,
     if (bad) return bad;
     if ((long long)pool_size * HV > 0x7fffffffll) return GDN_ERR_UNSUPPORTED;  // state number
     if (B == 0 || T == 0) return GDN_OK;
-    if (!q || !k || !v || !pool || !indices || !parents || !log_decay || !out) return GDN_ERR_INVALID;
+    if (!q || !k || !v || (!pool && pool_size > 0) || !indices || !parents || !log_decay || !out) return GDN_ERR_INVALID;
     if (!gdn_aligned(q, 16) || !gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(out, 16) ||
         !gdn_aligned(pool, 16) || !gdn_aligned(log_decay, 4) || !gdn_aligned(parents, 4) ||
         !gdn_aligned(indices, indices_int64 ? 8 : 4))
         return GDN_ERR_ALIGN;
+    if (pool_size == 0)  // every entry is padding, and there is no state to make a tensor map of
+        return cudaMemsetAsync(out, 0, (size_t)B * T * HV * gdn::kDim * 2, static_cast<cudaStream_t>(stream)) == cudaSuccess
+                   ? GDN_OK
+                   : GDN_ERR_CUDA;
     VerifyParams p;
     p.q = static_cast<const __nv_bfloat16*>(q);
     p.k = static_cast<const __nv_bfloat16*>(k);
@@ -719,11 +723,12 @@ extern "C" int gdn_decay_commit(const void* k, const void* v, void* pool, int st
     const int bad = check_tree(state_bf16, indices_int64, decay_per_token, B, T, H, HV, K, V, pool_size);
     if (bad) return bad;
     if (B == 0) return GDN_OK;
-    if (!pool || !indices || !accepted || (T > 0 && (!k || !v || !parents || !log_decay))) return GDN_ERR_INVALID;
+    if ((!pool && pool_size > 0) || !indices || !accepted || (T > 0 && (!k || !v || !parents || !log_decay))) return GDN_ERR_INVALID;
     if (!gdn_aligned(k, 16) || !gdn_aligned(v, 16) || !gdn_aligned(pool, 16) || !gdn_aligned(log_decay, 4) ||
         !gdn_aligned(parents, 4) || !gdn_aligned(accepted, 4) || !gdn_aligned(indices, indices_int64 ? 8 : 4) ||
         !gdn_aligned(out_indices, indices_int64 ? 8 : 4))
         return GDN_ERR_ALIGN;
+    if (pool_size == 0) return GDN_OK;  // every entry is padding
     CommitParams p;
     p.k = static_cast<const __nv_bfloat16*>(k);
     p.v = static_cast<const __nv_bfloat16*>(v);

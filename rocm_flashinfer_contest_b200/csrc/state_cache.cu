@@ -201,10 +201,12 @@ static int entry(const void* pool, int bf16, const void* slots, const void* cach
     const long long per = (long long)kWarps * kWarpElems, tiles = (elems + per - 1) / per;
     if (tiles > (1ll << 30) || tiles * B > (1ll << 30)) return GDN_ERR_UNSUPPORTED;  // grid index
     if (B == 0) return GDN_OK;
-    if (!pool || !slots || !cache_slots || !codes || !exps) return GDN_ERR_INVALID;
+    // (without slots on a side there may be no address)
+    if (!slots || !cache_slots || (pool_size > 0 && !pool) || (cache_size > 0 && (!codes || !exps))) return GDN_ERR_INVALID;
     if (!gdn_aligned(pool, 16) || !gdn_aligned(codes, 16) || !gdn_aligned(slots, idx64 ? 8 : 4) ||
         !gdn_aligned(cache_slots, idx64 ? 8 : 4))
         return GDN_ERR_ALIGN;
+    if (pool_size == 0 || cache_size == 0) return GDN_OK;  // every pair is padding
     Params p;
     p.pool = const_cast<void*>(pool);
     p.codes = static_cast<uint8_t*>(const_cast<void*>(codes));
