@@ -14,6 +14,25 @@ constexpr float kMinLogDecay = -104.0f;
 
 __device__ __forceinline__ float clamp_log_decay(float g) { return g < kMinLogDecay ? kMinLogDecay : g; }
 
+// A clamped log decay as a multiple of 2^-10 and the rest, at most 2^-11.  Up to 64
+// of them are summed part by part: the first sum is exact (at most 64 * 151 in
+// magnitude, so 24 bits hold it), the second is off by 2^-28 at most, and so
+// differences of two sums are as exact as the decays between them.  In one float
+// each, behind gates that forget (-104), a sum is in the thousands and a difference
+// of a tenth was off by 5e-4.
+constexpr float kPartUnit = 12288.0f;  // 1.5 * 2^13: its last bit is 2^-10
+__device__ __forceinline__ float2 split_log_decay(float g) {
+    const float x = (g + kPartUnit) - kPartUnit;
+    return make_float2(x, g - x);
+}
+// The same of g / ln 2, 1 / ln 2 itself in two floats.
+__device__ __forceinline__ float2 split_log2_decay(float g) {
+    constexpr double kLog2e = 1.4426950408889634;
+    constexpr float kNear = (float)kLog2e, kRest = (float)(kLog2e - (double)kNear);
+    const float x = fmaf(g, kNear, kPartUnit) - kPartUnit;
+    return make_float2(x, fmaf(g, kRest, fmaf(g, kNear, -x)));
+}
+
 __device__ __forceinline__ long long slot_at(const void* idx, int is64, int i) {
     if (idx == nullptr) return i;
     return is64 ? static_cast<const long long*>(idx)[i] : (long long)static_cast<const int*>(idx)[i];

@@ -183,7 +183,8 @@ struct L {
     static constexpr uint32_t os = ps + 2 * kP;       // two buffers of a chunk's outputs, [token][v]
     static constexpr uint32_t tail = os + 2 * kTile;  // 24 KiB of a state on its way out
     static constexpr uint32_t gates = tail + 24 * 1024;
-    static constexpr uint32_t bars = gates + kGates * 832;
+    static constexpr uint32_t kGate = 1088;
+    static constexpr uint32_t bars = gates + kGates * kGate;
     static constexpr uint32_t total = bars + 320;
 };
 static_assert(L::total <= 227 * 1024, "shared memory");
@@ -192,7 +193,8 @@ enum : int { kLast = 1, kFinal = 2 };
 
 // What a chunk's warps need to know of it.
 struct Gate {
-    float c2[C];  // c_i / ln 2
+    float minus[C];  // the first part of c_i / ln 2 (split_log2_decay), negated
+    float near[C];   // 2^-(the second part)
     float e[C];   // scale * e^{c_i}
     float w[C];   // e^{c_63 - c_i}
     float a;      // e^{c_63}
@@ -205,7 +207,7 @@ struct Gate {
                        // new_state, or nowhere (-1)
     int decay;         // last chunk: the number in the workspace where the segment's decay goes, or -1
 };
-static_assert(sizeof(Gate) <= 832, "gate slot");
+static_assert(sizeof(Gate) <= L::kGate, "gate slot");
 
 struct Bars {
     uint64_t full[3], empty[3], pv_done[2], qk_full[2], u_full[2], u_free, p_read, p_ready[2], p_free[2], v_ready[2], s_ready, s_free,
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Bars& B = *reinterpret_cast<Bars*>(sm + L::bars);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t sb = smem_u32(sm);
-    auto gate = [&](int m) { return reinterpret_cast<Gate*>(sm + L::gates + (m % L::kGates) * 832); };
+    auto gate = [&](int m) { return reinterpret_cast<Gate*>(sm + L::gates + (m % L::kGates) * L::kGate); };
 
     Finder finder;
     Item it{p.N, 0, 0, 0, 0, 0};
@@ -687,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fence_after_sync();
                     const Gate* gt = gate(m);
                     const int flags = gt->flags;
-                    const float ci = gt->c2[i];
+                    const float ci = -gt->minus[i], f = __fdividef(p.scale, gt->near[i]);
                     uint8_t* row = sm + L::ps + (m & 1) * L::kP + i * 128;
                     // this buffer's last products are those of chunk m - 2
                     if (m > 1 && !wait_bar(B, &B.p_free[m & 1], (m >> 1) - 1)) break;
@@ -705,9 +707,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int low = warp == 21 ? 32 : lane - 16 * c;  // the blocks on the diagonal end there
 #pragma unroll
                         for (int j = 0; j < 16; j += 4) {
-                            const float4 cj = *reinterpret_cast<const float4*>(&gt->c2[32 * jb + 16 * c + j]);
-                            const float2 a = __fmul2_rn(make_float2(ex2(ci - cj.x), ex2(ci - cj.y)), make_float2(x[j], x[j + 1]));
-                            const float2 d = __fmul2_rn(make_float2(ex2(ci - cj.z), ex2(ci - cj.w)), make_float2(x[j + 2], x[j + 3]));
+                            // e^{c_i - c_j}: the first parts' difference is exact, the second parts are factors near 1
+                            const float4 cj = *reinterpret_cast<const float4*>(&gt->minus[32 * jb + 16 * c + j]);
+                            const float4 nj = *reinterpret_cast<const float4*>(&gt->near[32 * jb + 16 * c + j]);
+                            const float2 y = __fadd2_rn(make_float2(ci, ci), make_float2(cj.x, cj.y)), z = __fadd2_rn(make_float2(ci, ci), make_float2(cj.z, cj.w));
+                            const float2 a = __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __fmul2_rn(make_float2(nj.x, nj.y), make_float2(x[j], x[j + 1])));
+                            const float2 d = __fmul2_rn(make_float2(ex2(z.x), ex2(z.y)), __fmul2_rn(make_float2(nj.z, nj.w), make_float2(x[j + 2], x[j + 3])));
                             x[j] = j <= low ? a.x : 0.f, x[j + 1] = j + 1 <= low ? a.y : 0.f, x[j + 2] = j + 2 <= low ? d.x : 0.f, x[j + 3] = j + 3 <= low ? d.y : 0.f;
                         }
 #pragma unroll
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             uint32_t t[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float2 z = __fmul2_rn(make_float2(p.scale, p.scale), make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]));
+                                const float2 z = __fmul2_rn(make_float2(f, f), make_float2(x[8 * q + 2 * e], x[8 * q + 2 * e + 1]));
                                 t[e] = pack_bf16(z.x, z.y);
                             }
                             *reinterpret_cast<uint4*>(row + (((4 * jb + 2 * c + q) ^ (i & 7)) << 4)) = make_uint4(t[0], t[1], t[2], t[3]);
@@ -793,20 +798,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < nch; ++c, ++m) {
                     const float g0 = clamp_log_decay(n0), g1 = clamp_log_decay(n1);
                     if (c + 1 < nch) ask(c + 1, n0, n1);
-                    float pre = g0 + g1, suf = g0 + g1;  // inclusive sums up to and from this lane
+                    // sums to base 2 up to and including token 2 l + 1, in two parts (split_log2_decay)
+                    const float2 x0 = split_log2_decay(g0), x1 = split_log2_decay(g1);
+                    float2 c1 = make_float2(x0.x + x1.x, x0.y + x1.y);
 #pragma unroll
                     for (int d = 1; d < 32; d *= 2) {
-                        const float a = __shfl_up_sync(0xffffffffu, pre, d), b = __shfl_down_sync(0xffffffffu, suf, d);
-                        if (lane >= d) pre += a;
-                        if (lane + d < 32) suf += b;
+                        const float a = __shfl_up_sync(0xffffffffu, c1.x, d), r = __shfl_up_sync(0xffffffffu, c1.y, d);
+                        if (lane >= d) c1.x += a, c1.y += r;
                     }
-                    float behind = __shfl_down_sync(0xffffffffu, suf, 1);
-                    if (lane == 31) behind = 0.f;
-                    const float c0 = lane == 0 ? g0 : pre - g1;
-                    constexpr float kLog2e = 1.4426950408889634f;
-                    const float2 e = make_float2(p.scale * expf(c0), p.scale * expf(pre));
-                    const float2 w = make_float2(expf(behind + g1), expf(behind));
-                    const float all = expf(suf);
+                    const float2 c0 = make_float2(c1.x - x1.x, c1.y - x1.y);
+                    const float2 end = make_float2(__shfl_sync(0xffffffffu, c1.x, 31), __shfl_sync(0xffffffffu, c1.y, 31));
+                    const float2 e = make_float2(p.scale * exp2f(c0.x + c0.y), p.scale * exp2f(c1.x + c1.y));
+                    // (these weigh the fp32 state: expf is a few times as accurate as exp2f)
+                    constexpr float kLn2 = 0.6931471805599453f;
+                    const float2 w = make_float2(expf(kLn2 * ((end.x - c0.x) + (end.y - c0.y))), expf(kLn2 * ((end.x - c1.x) + (end.y - c1.y))));
+                    const float all = expf(kLn2 * (end.x + end.y));
                     // the stage is free, so the products of chunk m - 3 are done, and before them the last reader of
                     // gate slot m - 5 was
                     if (m >= L::kStages && !wait_bar(B, &B.empty[m % L::kStages], m / L::kStages - 1)) {
@@ -814,7 +820,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                     Gate* gt = gate(m);
-                    *reinterpret_cast<float2*>(&gt->c2[2 * lane]) = make_float2(c0 * kLog2e, pre * kLog2e);
+                    *reinterpret_cast<float2*>(&gt->minus[2 * lane]) = make_float2(-c0.x, -c1.x);
+                    *reinterpret_cast<float2*>(&gt->near[2 * lane]) = make_float2(ex2(-c0.y), ex2(-c1.y));
                     *reinterpret_cast<float2*>(&gt->e[2 * lane]) = e;
                     *reinterpret_cast<float2*>(&gt->w[2 * lane]) = w;
                     if (lane == 0) {

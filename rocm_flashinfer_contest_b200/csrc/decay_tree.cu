@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(256, 2)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     // of an item and the next one
     __shared__ unsigned long long paths[2][kTreeMax];        // bit j: j is on the node's path; 0: padding
-    __shared__ float sums[2][kTreeMax], decays[2][kTreeMax];  // c_t and e^{c_t}
+    __shared__ float2 sums[2][kTreeMax];                      // c_t in two parts (split_log_decay)
+    __shared__ float decays[2][kTreeMax];                     // e^{c_t}
     __shared__ unsigned long long used_nodes[2];              // bit t: node t is not padding
     __shared__ size_t s_out;               // the next item's first output
     __shared__ int s_padding;              // the next item has no state
@@ -207,36 +208,36 @@ __global__ void __launch_bounds__(256, 2)
     // marks padding.
     auto find_paths = [&](int buf) {
         unsigned long long m[2];
-        float cc[2];
+        float2 cc[2];
         int up[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int t = lane + 32 * i;
             up[i] = par[i] < -1 || par[i] >= t ? -2 : par[i];
-            cc[i] = clamp_log_decay(gg[i]);
+            cc[i] = split_log_decay(clamp_log_decay(gg[i]));
             m[i] = t < T ? 1ull << t : 0ull;
         }
 #pragma unroll 1
         for (int hop = 1; hop < T; hop *= 2) {
             unsigned long long mm[2];
-            float dc[2];
+            float2 dc[2];
             int uu[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {  // what node up[i] knows
                 const int u = up[i] & 31;
                 mm[i] = __shfl_sync(0xffffffffu, m[0], u);
-                dc[i] = __shfl_sync(0xffffffffu, cc[0], u);
+                dc[i].x = __shfl_sync(0xffffffffu, cc[0].x, u), dc[i].y = __shfl_sync(0xffffffffu, cc[0].y, u);
                 uu[i] = __shfl_sync(0xffffffffu, up[0], u);
                 if (T > 32) {
                     const unsigned long long m1 = __shfl_sync(0xffffffffu, m[1], u);
-                    const float d1 = __shfl_sync(0xffffffffu, cc[1], u);
+                    const float2 d1 = make_float2(__shfl_sync(0xffffffffu, cc[1].x, u), __shfl_sync(0xffffffffu, cc[1].y, u));
                     const int u1 = __shfl_sync(0xffffffffu, up[1], u);
                     if (up[i] >= 32) mm[i] = m1, dc[i] = d1, uu[i] = u1;
                 }
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (up[i] >= 0) cc[i] += dc[i], m[i] |= mm[i], up[i] = uu[i];
+                if (up[i] >= 0) cc[i].x += dc[i].x, cc[i].y += dc[i].y, m[i] |= mm[i], up[i] = uu[i];
         }
         unsigned used[2];
 #pragma unroll
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(256, 2)
             const int t = lane + 32 * i;
             paths[buf][t] = up[i] == -1 ? m[i] : 0ull;
             sums[buf][t] = cc[i];
-            decays[buf][t] = expf(cc[i]);
+            decays[buf][t] = expf(cc[i].x + cc[i].y);
             used[i] = __ballot_sync(0xffffffffu, up[i] == -1);
         }
         if (lane == 0) used_nodes[buf] = (unsigned long long)used[1] << 32 | used[0];
@@ -285,7 +286,8 @@ __global__ void __launch_bounds__(256, 2)
         __nv_bfloat16* out = p.out + s_out;  // + t * HV * 128
         const bool padding = s_padding;
         const unsigned long long* s_path = paths[turn & 1];
-        const float *s_c = sums[turn & 1], *s_e = decays[turn & 1];
+        const float2* s_c = sums[turn & 1];
+        const float* s_e = decays[turn & 1];
 
         float acc[8][4];  // o^T rows `rows` + {g, g + 8}, tokens 8 n + 2 c + {0, 1}
         if (!padding) {
@@ -366,8 +368,9 @@ __global__ void __launch_bounds__(256, 2)
                 for (int r = 0; r < 2; ++r) {
                     const int t = 16 * m + g + 8 * r, j = 8 * n + 2 * c;
                     const unsigned long long path = s_path[t];
-                    const float y = path >> j & 1 ? x[2 * r] * expf(s_c[t] - s_c[j]) : 0.f;
-                    const float z = path >> (j + 1) & 1 ? x[2 * r + 1] * expf(s_c[t] - s_c[j + 1]) : 0.f;
+                    const float2 ct = s_c[t], cj = s_c[j], cj1 = s_c[j + 1];
+                    const float y = path >> j & 1 ? x[2 * r] * expf((ct.x - cj.x) + (ct.y - cj.y)) : 0.f;
+                    const float z = path >> (j + 1) & 1 ? x[2 * r + 1] * expf((ct.x - cj1.x) + (ct.y - cj1.y)) : 0.f;
                     uint32_t hi, low;
                     split2(y, z, hi, low);
                     *reinterpret_cast<uint32_t*>(ph + t * kPS + j) = hi;
