@@ -20,6 +20,11 @@
  * workspaces 16-byte aligned (the prefill's states and workspace 32),
  * log_decay 4 bytes, index arrays their own size.
  * The reference project has no counterpart of these operators.
+ *
+ * Values that are not finite reach the outputs and states that the formula lets
+ * them reach, and no others but where it is said below.  In the prefill and the
+ * verification they may arrive as NaN where the formula has an infinity: operands
+ * are split into terms, and infinity times a zero term is NaN.
  */
 #ifndef GDN_DECAY_B200_H_
 #define GDN_DECAY_B200_H_
@@ -47,6 +52,11 @@ extern "C" {
  * (and refused for the states).
  * The products run on 64-token chunks, so a value of v that is not finite
  * spoils the outputs of its whole chunk, those of earlier tokens too.
+ *
+ * Precision: new_state is advanced in fp32.  For the outputs the state before a
+ * chunk and the decayed scores are rounded to bf16 once each, so an output is
+ * off by up to 2^-8 of scale * (|S| |q| + sum |decayed score| |v|) beside its own
+ * rounding; the other operators keep two bf16 terms (2^-16) or fp32 there.
  *
  * workspace: device memory, 32-byte aligned, at least
  * gdn_decay_prefill_workspace_bytes(N, T, HV) bytes (which may be 0; the

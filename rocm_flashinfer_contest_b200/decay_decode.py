@@ -23,7 +23,7 @@ q, k [B, 1, H, 128] bf16; v, output [B, 1, HV, 128] bf16; log_decay [HV] or
 or 0-d tensor, None / 0 -> 1/sqrt(128); indices [B] int32 or int64.  One kernel
 launch on the current stream of the inputs' device, no host synchronisation
 (unless ``scale`` is a device tensor, which is read with ``.item()``), no
-gradients.
+gradients.  ``output`` must not overlap an input.
 """
 from __future__ import annotations
 

@@ -27,8 +27,10 @@ q, k [B, T, H, 128] bf16; v, output [B, T, HV, 128] bf16; T <= 64; pool
 and accepted [B] int32; log_decay [HV] or [B, T, HV] fp32; scale float or 0-d
 tensor, None / 0 -> 1/sqrt(128).  One kernel launch each on the current stream
 of the inputs' device, no host synchronisation (unless ``scale`` is a device
-tensor, which is read with ``.item()``), no gradients.  A value of v that is not
-finite, at a node that is not padding, spoils the outputs of its entry's tree.
+tensor, which is read with ``.item()``), no gradients.  ``output`` must not overlap
+an input.  A value of v that is not finite, at a node that is not padding, spoils
+the outputs of its entry's tree; other values that are not finite reach what the
+formula lets them reach, but may arrive in ``output`` as NaN where it has an infinity.
 """
 from __future__ import annotations
 
