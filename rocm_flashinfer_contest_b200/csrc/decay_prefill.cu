@@ -33,11 +33,13 @@
 // the output's two parts, so the output's error is sqrt(2) times that of the last
 // rounding alone (measured 0.0023 against 0.0017 of the output; second terms
 // bring it to 0.0017 and cost 12 more products and 1,000 more instructions a
-// chunk).
+// chunk).  It is bounded by 2^-8 of scale (|S| |q| + |P| |v|), so an output that
+// cancels loses more of itself.  Sums of log decays are exact to 2^-28
+// (split_log2_decay).
 //
-// Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 91 us (its 205 MB alone
+// Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 92 us (its 205 MB alone
 // take 31; called without a pause the GPU reaches its 1,000 W and lowers its clock
-// from 1.97 to 1.6 GHz: 105), a chunk every 2,400 cycles in each CTA.  The chunk's
+// from 1.97 to 1.6 GHz: 104), a chunk every 2,400 cycles in each CTA.  The chunk's
 // 32 products alone take 1,540, issued without a pause and in turn (at the pipe's
 // full rate 1,408); those that add to one accumulator with N = 64 follow each other
 // at 80 cycles, so 12 for an output are 700 from the first to the end.  The rest are
@@ -45,13 +47,19 @@
 // the pipe: U's sums into S, S to bf16, S q, the next S; U, V's terms into the place
 // that it leaves, the next U; outputs out of the accumulators, the next output's
 // products.
-// 61 prompts of 82 tokens, 32 v-heads: 106.5 us, bound by states (64 KiB in and 64
-// KiB out a prompt and head) that a CTA reads and writes one after the other: 4,700
-// of 8,500 cycles a segment of one chunk are the wait for its start state, 7 us in
-// all for its rows lying 512 bytes apart in a warp's loads.
+// 61 prompts of 1 to 640 tokens (82 on average), 32 v-heads: 107 us, for two
+// reasons.  States (64 KiB in and 64 KiB out a prompt and head) are read and written
+// one after the other: in a segment of one chunk 4,700 of 8,500 cycles are the wait
+// for its start state, 7 us in all for its rows lying 512 bytes apart in a warp's
+// loads.  And a CTA has every 148th segment, whatever their lengths: the busiest has
+// 36 chunks, the mean is 24.6.
+// 13 prompts of 7 to 3,353 tokens, 8 v-heads: 62 us.  Two launches of 96 and 152
+// segments on 148 SMs: 1.3 passes over the chunks, but the busiest CTAs have 14 and
+// 14 chunks, 34 us, where the means are 9.1 and 9.6; the rest are the two launches'
+// starts and ends and the kernel between them.
 //
-// Tried and not kept, at those two: K scaled instead of V, in shared memory (97 and
-// 117 us); that with its lower terms double-buffered (104); V turned by the state
+// Tried and not kept, at the first two (91 and 106.5 us then): K scaled instead of
+// V, in shared memory (97 and 117 us); that with its lower terms double-buffered (104); V turned by the state
 // warps (100 and 117) or by the output warps (111 and 117); scaling unrolled (96 and
 // 113); eight output warps (91 and 109); all of V's terms made before the place is
 // free (92 and 108); an output's two chains of products issued in turn (92 and 108);

@@ -39,12 +39,18 @@ constexpr int kTreeMax = GDN_DECAY_TREE_MAX;
 // threads 43, by a copy a row 54; operands of the small products by plain loads +2;
 // padding's v zeroed in shared memory, and every thread asking for the next slot,
 // +2; the next slot and output place found by every thread +1; the paths found by
-// one warp before the item +0.5.
+// one warp before the item +0.5.  64 such entries without a pause between calls, fp32
+// / bf16 states: 8 nodes 32.0 / 25.3 us, 16 33.7 / 27.0, 32 38.3 / 31.4, 64 (one CTA
+// an SM) 74 / 68.
+// bf16 and 16 nodes would leave shared memory for four CTAs; their 256 columns of
+// tensor memory each let two run.
 //
 // Precision: q, k, v are bf16 as given.  An fp32 state is split into two bf16
-// terms (hi + lo, off by at most 2^-17 of it) and the decayed scores P likewise,
+// terms (hi, its first 8 bits, and lo, what is left, below 2^-7 of its power of two,
+// rounded to 8 bits: off by at most 2^-16 of it) and the decayed scores P likewise,
 // so the products lose nothing next to the output's own rounding to bf16 (2^-8);
-// one bf16 term each would about double the output's error.
+// one bf16 term each would about double the output's error.  Sums of log decays
+// are exact to 2^-28 (split_log_decay).
 // ---------------------------------------------------------------------------
 
 struct VerifyParams {

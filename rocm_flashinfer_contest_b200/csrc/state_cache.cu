@@ -13,8 +13,10 @@
 // lanes share a group, its maximum takes three shuffles, and the warp's 16 exponent
 // bytes leave as one store.  All 4 steps' loads are on their way before the first is
 // needed.  48 slots of 32 heads, fp32 to int8 and back (248 MB): 45.8 us both, 5.4
-// TB/s, with two launches' starts and ends in it; 8 steps a warp 47.4, 2 steps 49.4;
-// CTAs of 1, 2 and 8 warps instead of 4 (8 steps): 47.1, 47.5 and 47.9.
+// TB/s, with two launches' starts and ends in it (back alone 24.9); 8 steps a warp
+// 47.4, 2 steps 49.4; CTAs of 1, 2 and 8 warps instead of 4 (8 steps): 47.1, 47.5 and
+// 47.9.  bf16 to int8 and back (150 MB) 38.4, back alone 18.2, with half the bytes
+// of a state on their way in a lane; e4m3 takes the same in both.
 #include <cuda_fp8.h>
 
 #include "decay_common.cuh"
