@@ -814,7 +814,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float a = __shfl_up_sync(0xffffffffu, c1.x, d), r = __shfl_up_sync(0xffffffffu, c1.y, d);
                         if (lane >= d) c1.x += a, c1.y += r;
                     }
-                    const float2 c0 = make_float2(c1.x - x1.x, c1.y - x1.y);
+                    // (not c1 - x1: a gate that is NaN stays out of the token before it)
+                    float2 c0 = make_float2(__shfl_up_sync(0xffffffffu, c1.x, 1), __shfl_up_sync(0xffffffffu, c1.y, 1));
+                    c0 = lane == 0 ? x0 : make_float2(c0.x + x0.x, c0.y + x0.y);
                     const float2 end = make_float2(__shfl_sync(0xffffffffu, c1.x, 31), __shfl_sync(0xffffffffu, c1.y, 31));
                     const float2 e = make_float2(p.scale * exp2f(c0.x + c0.y), p.scale * exp2f(c1.x + c1.y));
                     // (these weigh the fp32 state: expf is a few times as accurate as exp2f)

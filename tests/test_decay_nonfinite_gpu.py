@@ -49,6 +49,37 @@ def test_prefill(bad, where):
     check(got_s, s, ss, "new_state")
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("token", [0, 1, 64, 70, 71, 127, 299])
+def test_prefill_gates(bad, token):
+    """A gate that is not finite (nor -inf, which forgets) reaches its token and what follows, not the token before."""
+    from rocm_flashinfer_contest_b200 import decay_prefill
+    q, k, v, st, g, cu = prefill_case([100, 300, 70], 2, 4, "token", 17)
+    cu_t = torch.tensor(cu, device="cuda")
+    o, s = decay_prefill.run(q, k, v, st, g, cu_t, SCALE)
+    g[100 + token, 2] = bad
+    so, ss = torch.zeros_like(o, dtype=torch.bool), torch.zeros_like(s, dtype=torch.bool)
+    so[100 + token:400, 2] = True
+    ss[1, 2] = True
+    got_o, got_s = decay_prefill.run(q, k, v, st, g, cu_t, SCALE)
+    check(got_o, o, so, "output")
+    check(got_s, s, ss, "new_state")
+
+
+@pytest.mark.parametrize("node", [0, 2, 12, 19])
+def test_tree_gates(node):
+    from rocm_flashinfer_contest_b200 import decay_tree
+    gen, pool, idx, q, k, v, g = pool_case(2, 20, 2, 4, "token", 19, False, 3)
+    parents = torch.tensor([[-1, *range(9), 2, *range(10, 19)]] * 2, dtype=torch.int32, device="cuda")
+    o = decay_tree.run(q, k, v, pool, idx, parents, g, SCALE)
+    g[0, node, 2] = float("nan")
+    so = torch.zeros_like(o, dtype=torch.bool)
+    so[0, node:, 2] = True
+    if node == 0:
+        so[0, :, 2] = True
+    check(decay_tree.run(q, k, v, pool, idx, parents, g, SCALE), o, so, "output")
+
+
 @pytest.mark.parametrize("bad", BAD)
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("where", ["q", "k", "v", "pool"])
