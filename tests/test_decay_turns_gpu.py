@@ -58,3 +58,26 @@ def test_prefill_takes_turns(lens, H, HV, kind, state):
     q, k, v, st, g, cu = case = prefill_case(lens, H, HV, kind, seed=len(lens) + HV, state=state)
     o, s = decay_prefill.run(q, k, v, st, g, torch.tensor(cu, device="cuda"), SCALE)
     check_prefill(o, s, case)
+
+
+@pytest.mark.parametrize("lens,H,HV,kind", [
+    ([120_001, 1, 30_000], 1, 2, "token"),          # a hundred segments, one joined to the other
+    ([65_537], 1, 1, "strong"),
+    ([i % 4 for i in range(2500)], 1, 1, "head"),   # more sequences than CTAs, by far
+])
+def test_prefill_of_long_and_of_many(lens, H, HV, kind):
+    from rocm_flashinfer_contest_b200 import decay_prefill
+    q, k, v, st, g, cu = case = prefill_case(lens, H, HV, kind, seed=len(lens), state=True)
+    o, s = decay_prefill.run(q, k, v, st, g, torch.tensor(cu, device="cuda"), SCALE)
+    check_prefill(o, s, case)
+
+
+@pytest.mark.parametrize("B,T,HV,bf16", [(900, 2, 1, False), (700, 1, 2, True), (350, 35, 1, False)])
+def test_verify_takes_many_turns(B, T, HV, bf16):
+    from rocm_flashinfer_contest_b200 import decay_tree
+    gen, pool, idx, q, k, v, g = pool_case(B, T, 1, HV, "token", B, bf16, B)
+    parents = tree_parents(gen, B, T, "mixed")
+    idx[torch.rand(B, generator=gen, device="cuda") < 0.4] = -1
+    ro, rm = verify_reference(pool, idx, parents, q, k, v, g, SCALE)
+    o = decay_tree.run(q, k, v, pool, idx, parents, g, SCALE)
+    close(o, ro, U_BF16 * ro.abs() + SLACK * rm + 1e-30, "output")
