@@ -39,7 +39,7 @@
 //
 // Measured: 8,192 tokens of 32 v-heads and 16 q/k heads 92 us (its 205 MB alone
 // take 31; called without a pause the GPU reaches its 1,000 W and lowers its clock
-// from 1.97 to 1.6 GHz: 104), a chunk every 2,400 cycles in each CTA.  The chunk's
+// from 1.97 to 1.6 GHz: 104 to 107), a chunk every 2,400 cycles in each CTA.  The chunk's
 // 32 products alone take 1,540, issued without a pause and in turn (at the pipe's
 // full rate 1,408); those that add to one accumulator with N = 64 follow each other
 // at 80 cycles, so 12 for an output are 700 from the first to the end.  The rest are
@@ -47,7 +47,7 @@
 // the pipe: U's sums into S, S to bf16, S q, the next S; U, V's terms into the place
 // that it leaves, the next U; outputs out of the accumulators, the next output's
 // products.
-// 61 prompts of 1 to 640 tokens (82 on average), 32 v-heads: 107 us, for two
+// 61 prompts of 1 to 640 tokens (82 on average), 32 v-heads: 108 us, for two
 // reasons.  States (64 KiB in and 64 KiB out a prompt and head) are read and written
 // one after the other: in a segment of one chunk 4,700 of 8,500 cycles are the wait
 // for its start state, 7 us in all for its rows lying 512 bytes apart in a warp's
